@@ -52,26 +52,26 @@ def listed():
     rng = random.Random(11)
     return [
         # --- the `small` preset's row of 512 tokens that holds four documents: launches and host time count
-        _attention("attention small, 4 documents in 512", [1, 130, 77, 304], 2, 2, 128),
+        _attention("attention small 4 documents in 512", [1, 130, 77, 304], 2, 2, 128),
         # --- rows of the 119.5 M model (4 heads, context 2048) packed with documents of 32 to 2048 tokens
-        _attention("attention 4 heads, documents in 16384", _documents(rng, 16384, 32, 2048), 4, 4, 128),
+        _attention("attention 4 heads documents in 16384", _documents(rng, 16384, 32, 2048), 4, 4, 128),
         # --- long documents under a sliding window of 256, the short window of every preset; grouped heads
-        _attention("attention 8/4 heads, window 256, 32768", _documents(rng, 32768, 512, 8192), 8, 4, 128, window=256),
+        _attention("attention 8/4 heads window 256 32768", _documents(rng, 32768, 512, 8192), 8, 4, 128, window=256),
         # --- a whole prompt of 32768 tokens scored at once, 16 heads on two key heads
-        _attention("attention 16/2 heads, prompt 32768", [32768], 16, 2, 128, grad=False),
+        _attention("attention 16/2 heads prompt 32768", [32768], 16, 2, 128, grad=False),
         # --- odd: three query heads a key head, heads of 64, odd lengths, rows behind the last sequence
-        _attention("attention 9/3 heads of 64, odd", _documents(rng, 7001, 3, 1999), 9, 3, 64, pad=191),
+        _attention("attention 9/3 heads of 64 odd", _documents(rng, 7001, 3, 1999), 9, 3, 64, pad=191),
         # --- the `small` preset's loss: 512 tokens, 1024 ids
-        _loss("loss small, 512 x 1024 ids", 512, 256, 1024, 15.0),
+        _loss("loss small 512 x 1024 ids", 512, 256, 1024, 15.0),
         # --- a vocabulary that is no multiple of anything, a tenth of the tokens not counted, no soft cap
-        _loss("loss odd, 4099 x 50021 ids", 4099, 384, 50021, 0.0, ignored=0.1),
+        _loss("loss odd 4099 x 50021 ids", 4099, 384, 50021, 0.0, ignored=0.1),
         # --- a training micro-step with a large vocabulary, and the scoring pass of an evaluation
         _loss("loss 16384 x 65536 ids", 16384, 1024, 65536, 15.0),
-        _loss("loss scoring, 16384 x 131072 ids", 16384, 1024, 131072, 15.0, grad=False),
+        _loss("loss scoring 16384 x 131072 ids", 16384, 1024, 131072, 15.0, grad=False),
         # --- gradients of the `small` preset; of the 119.5 M model, clipped into bf16 buckets for the exchange; of a wide one
-        _clip("clip small, fp32", 256, 4, 1024, "float32", "float32", 3.0),
-        _clip("clip 119M, fp32 to bf16", 512, 30, 8191, "float32", "bfloat16", 2.5),
-        _clip("norm wide, bf16", 2048, 16, 8192, "bfloat16", "", 0.0),
+        _clip("clip small fp32", 256, 4, 1024, "float32", "float32", 3.0),
+        _clip("clip 119M fp32 to bf16", 512, 30, 8191, "float32", "bfloat16", 2.5),
+        _clip("norm wide bf16", 2048, 16, 8192, "bfloat16", "", 0.0),
     ]
 
 
