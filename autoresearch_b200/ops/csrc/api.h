@@ -28,6 +28,7 @@ enum ArbError {
   ERR_COMM_TIMEOUT = 3,
   ERR_MOE_TIMEOUT = 4,
   ERR_SMEM_ALIGN = 5,   // dynamic shared memory base not 1 KB aligned (kernel returned before doing any work)
+  ERR_SEQLENS = 6,      // packed sequence bounds that descend or lie outside of the rows (they were moved inside)
 };
 
 // Function attributes (dynamic shared memory size) belong to a device's context: a launcher sets them the first
@@ -114,6 +115,30 @@ int arb_attn_bwd(const void* q, const void* k, const void* v, const void* o, con
                  void* dq, void* dk, void* dv, float* delta, float* dq_accum, int B, int T, int H, long long ldq,
                  long long ldk, long long ldv, long long ldo, long long lddo, long long lddq, long long lddk,
                  long long lddv, int window, float scale, int* err_flag, cudaStream_t stream);
+
+// ---- attention over packed sequences, grouped heads (attn_packed_sm100.cu) ---------------------------------
+// Rows [cu[i], cu[i + 1]) of q, k, v are sequence i; key j is visible to query i of the same sequence iff i - window <= j <= i.
+// KV key heads, G query heads each (query head h reads key head h / G), D = 64 or 128.  Strides in elements; o, dq, dk, dv have
+// their heads D apart.  lse, delta: [rows, KV * G] fp32.  Rows of no sequence get zero outputs (lse -inf).
+// arb_packed_plan writes the work lists that both directions read: cap_q >= rows / (128 / G) + n_seq + 2 and
+// cap_k >= rows / 128 + n_seq + 2 items of 16 bytes; scratch: 4 (n_seq + 3) ints; span_rows: rows whose keys and values
+// together stay in L2.
+typedef struct ArbPacked {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;
+  const void* d_o;                   // backward, as everything down to dv
+  float* delta;                      // scratch
+  void *dq, *dk, *dv;
+  const void* items;
+  long long rows, KV, G, D, window, cap_q, cap_k;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, o_row, do_row, do_head, dq_row, dk_row, dv_row;
+  double scale;
+} ArbPacked;
+int arb_packed_plan(const int* cu, int n_seq, int rows, int G, int span_rows, void* items, int cap_q, int cap_k, int* scratch,
+                    int* err_flag, cudaStream_t stream);
+int arb_packed_attn_fwd(const ArbPacked* a, int* err_flag, cudaStream_t stream);
+int arb_packed_attn_bwd(const ArbPacked* a, int* err_flag, cudaStream_t stream);
 
 // ---- row-wise fused norm / residual kernels (elementwise.cu) --------------------------------
 int arb_rmsnorm_fwd(const void* x, void* y, long long rows, int D, float eps, cudaStream_t s);

@@ -186,6 +186,48 @@ __device__ __forceinline__ float max32(const uint32_t (&s)[32], int col0, int ml
   return fmaxf(a, b);
 }
 
+// Exponentials of 32 scores of a row: e = 2^(s*c - mc), bf16 pairs into pk[16], row sum into the packed accumulator
+template <bool MASK>
+__device__ __forceinline__ void exp32_mufu(const uint32_t (&s)[32], uint32_t* pk, unsigned long long c2, unsigned long long nmc2,
+                                           int col0, int mlo, unsigned span, unsigned long long& rs2) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    float x0, x1;
+    unpk2(fma2(pk2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), c2, nmc2), x0, x1);
+    float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+    if constexpr (MASK) {
+      e0 = (unsigned(col0 + 2 * j - mlo) <= span) ? e0 : 0.f;
+      e1 = (unsigned(col0 + 2 * j + 1 - mlo) <= span) ? e1 : 0.f;
+    }
+    rs2 = add2(rs2, pk2(e0, e1));
+    pk[j] = pack_bf16(e0, e1);
+  }
+}
+
+// exp2 of 64 scores of one row/lane; the offsets are one per-row value or 64 per-column values
+template <bool ROW_STAT>
+__device__ __forceinline__ void exp2_64(const uint32_t (&s0)[32], const uint32_t (&s1)[32], float c, float row_off,
+                                        const float4* col_off, float (&pr)[64]) {
+#pragma unroll
+  for (int g = 0; g < 16; ++g) {
+    float4 o = make_float4(row_off, row_off, row_off, row_off);
+    if (!ROW_STAT) o = col_off[g];
+    const float off[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = g * 4 + u;
+      const float x = __uint_as_float(j < 32 ? s0[j] : s1[j - 32]) * c - off[u];
+      pr[j] = fast_exp2(x);
+    }
+  }
+}
+
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&a)[32], uint32_t (&b)[32]) {
+  tmem_ld32(taddr, a);
+  tmem_ld32(taddr + 32, b);
+  tmem_wait_ld();
+}
+
 __device__ __forceinline__ void named_bar_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }

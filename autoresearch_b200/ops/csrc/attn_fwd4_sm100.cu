@@ -27,24 +27,6 @@ struct Fwd4Smem {
 };
 static_assert(2 * (Fwd4Smem::TOTAL + 1024) <= 233472, "two CTAs must fit the 228 KB of an SM");
 
-// Exponentials of 32 scores of a row: e = 2^(s*c - mc), bf16 pairs into pk[16], row sum into the packed accumulator
-template <bool MASK>
-__device__ __forceinline__ void exp32_mufu(const uint32_t (&s)[32], uint32_t* pk, unsigned long long c2, unsigned long long nmc2,
-                                           int col0, int mlo, unsigned span, unsigned long long& rs2) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    float x0, x1;
-    unpk2(fma2(pk2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), c2, nmc2), x0, x1);
-    float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
-    if constexpr (MASK) {
-      e0 = (unsigned(col0 + 2 * j - mlo) <= span) ? e0 : 0.f;
-      e1 = (unsigned(col0 + 2 * j + 1 - mlo) <= span) ? e1 : 0.f;
-    }
-    rs2 = add2(rs2, pk2(e0, e1));
-    pk[j] = pack_bf16(e0, e1);
-  }
-}
-
 __global__ void __launch_bounds__(ATT_THREADS, 2)
 attn_fwd4_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
             const __grid_constant__ CUtensorMap tmV, const AttnArgs p) {

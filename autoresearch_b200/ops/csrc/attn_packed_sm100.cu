@@ -1,0 +1,1113 @@
+// Causal attention over packed sequences of different lengths with grouped heads, forward and backward, head_dim 64 or 128.
+//
+//   rows [cu[i], cu[i+1]) are sequence i;  key j is visible to query i of the same sequence iff i - window <= j <= i
+//   O = softmax(scale Q K^T) V per query head; G = H / KV query heads read one key head
+//   dP = dO V^T;  dS = P (dP - rowsum(dO o O));  dQ = scale dS K;  dK = scale dS^T Q;  dV = P^T dO, the last two summed over
+//   the G query heads of a key head
+//
+// A query tile is P = 128 / G positions x the G heads of one key head (row = position * G + head): one K / V tile serves the whole
+// group, a short sequence fills more of a tile, and the key-stationary backward sums over the group inside its accumulators, in a
+// fixed order and without atomics.  A TMA box {64, G, 1, P} over the [D, G, KV, rows] view of the queries lays that tile out.
+//
+// Tiles never span two sequences.  Which tiles there are depends on lengths that only the device knows, so a plan kernel writes
+// two work lists (query tiles, key tiles), longest first within a span of rows whose K and V stay in L2; the grids are sized by
+// the bound rows / P + sequences + 2 and a CTA without a tile returns.  What a tile loads beyond the end of its sequence (another
+// sequence's rows, or rows behind the last one, with any values in them) is set to zero in shared memory before a product sums
+// over it, so the results of a sequence do not depend on what surrounds it, bit for bit.
+//
+// The pipelines are those of attn_fwd4_sm100.cu (forward: two CTAs per SM) and attn_wide_sm100.cu (backward: ten warps, two-phase
+// softmax, dK/dV and dQ in one grid); what is said there about the MMA order, the TMEM reuse and their bounds holds here too.
+#include "attn_common.cuh"
+
+namespace arb {
+
+constexpr long long PACKED_MAX_ROWS = 1ll << 30;
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_LEVELS = 64, PLAN_SPANS = 32, PLAN_BINS = PLAN_LEVELS * PLAN_SPANS;
+
+// One tile: rows [start, start + len) are its sequence and `tile` its number there.  tile < 0: rows that belong to no sequence and
+// whose outputs are zero; len = 0: nothing.
+struct PackedItem { int start, len, tile, pad; };
+static_assert(sizeof(PackedItem) == 16, "read as one 16-byte word");
+
+struct PackedArgs {
+  const PackedItem* items_q;
+  const PackedItem* items_k;
+  int n_q, n_k;                      // capacities of the lists
+  int KV, G, P;                      // key heads, query heads per key head, positions per query tile
+  int head_span;                     // key heads whose tiles are interleaved
+  int window;
+  float scale;
+  __nv_bfloat16* o;                  // forward: O; backward: dQ.  Row stride in elements, heads D apart
+  long long ldo;
+  float* lse;                        // [rows, H]
+  const float* delta;                // [rows, H]
+  __nv_bfloat16* dk;
+  __nv_bfloat16* dv;
+  long long lddk, lddv;
+  int* err;
+};
+
+// -----------------------------------------------------------------------------------------------
+// plan
+// -----------------------------------------------------------------------------------------------
+struct PlanArgs {
+  const int* cu;                     // [n + 1]
+  int n, rows, P;
+  int span_rows[2];                  // rows per span of the query and of the key list
+  int* bound;                        // [2][n + 3] scratch: first row of each sequence, the rows before and behind them included
+  int* first;                        // [2][n + 3] scratch: first tile of each
+  PackedItem* items[2];
+  int cap[2];
+  int* err;
+};
+
+// inclusive scan over the block, v in thread order; `shared` holds 32 values
+template <typename Op>
+__device__ __forceinline__ int block_scan(int v, int* shared, Op op, int neutral) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = op(u, v);
+  }
+  __syncthreads();
+  if (lane == 31) shared[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    int w = shared[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w = op(u, w);
+    }
+    shared[lane] = w;
+  }
+  __syncthreads();
+  return op(warp ? shared[warp - 1] : neutral, v);
+}
+
+// Block 0 writes the query tiles, block 1 the key tiles.  Three passes over the sequences (their bounds, made ascending and kept
+// within the rows whatever cu holds; tile counts) and two over the tiles (a counting sort by span of rows, then work).
+__global__ void __launch_bounds__(PLAN_THREADS) packed_plan_k(const PlanArgs p) {
+  __shared__ int bins[PLAN_BINS];
+  __shared__ int shared[32];
+  __shared__ int s_carry, s_longest, s_bad;
+  const int tid = threadIdx.x, which = blockIdx.x;
+  const int step = which ? 128 : p.P;                    // positions per tile
+  const int n_seq = p.n + 2;                             // rows before the first sequence, the sequences, rows behind the last
+  int* bound = p.bound + (long long)which * (p.n + 3);
+  int* first = p.first + (long long)which * (p.n + 3);
+  auto add = [](int a, int b) { return a + b; };
+  auto most = [](int a, int b) { return max(a, b); };
+  grid_enter();
+  for (int i = tid; i < PLAN_BINS; i += PLAN_THREADS) bins[i] = 0;
+  if (tid == 0) { s_carry = 0; s_longest = 0; s_bad = 0; }
+  __syncthreads();
+  // bounds: 0, cu[0], ..., cu[n], rows
+  for (int base = 0; base < p.n + 3; base += PLAN_THREADS) {
+    const int i = base + tid;
+    int v = 0;
+    if (i >= 1 && i <= p.n + 1) {
+      const int c = p.cu[i - 1];
+      v = min(max(c, 0), p.rows);
+      if (c != v || (i > 1 && c < p.cu[i - 2])) s_bad = 1;
+    } else if (i > p.n + 1) {
+      v = p.rows;
+    }
+    const int carry = s_carry;
+    const int b = max(carry, block_scan(v, shared, most, 0));
+    if (i < p.n + 3) bound[i] = b;
+    __syncthreads();
+    if (tid == PLAN_THREADS - 1) s_carry = b;
+    __syncthreads();
+  }
+  if (tid == 0) s_carry = 0;
+  __syncthreads();
+  for (int base = 0; base < n_seq; base += PLAN_THREADS) {
+    const int i = base + tid;
+    int t = 0;
+    if (i < n_seq) {
+      const int len = bound[i + 1] - bound[i];
+      t = (len + step - 1) / step;
+      if (i > 0 && i < n_seq - 1) atomicMax(&s_longest, len);
+    }
+    const int carry = s_carry;
+    const int s = carry + block_scan(t, shared, add, 0);
+    if (i < n_seq) first[i + 1] = s;
+    __syncthreads();
+    if (tid == PLAN_THREADS - 1) s_carry = s;
+    __syncthreads();
+  }
+  if (tid == 0) first[0] = 0;
+  __syncthreads();
+  const int tiles = min(s_carry, p.cap[which]);
+  const int other = which ? p.P : 128;                   // positions per tile of the other side
+  const int most_work = s_longest / other + 2;
+  auto item_of = [&](int t, PackedItem& it) -> int {     // the tile and its bin
+    int lo = 0, hi = n_seq - 1;                          // last sequence whose first tile is <= t; empty ones share theirs with the next
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    const bool dead = lo == 0 || lo == n_seq - 1;
+    const int start = bound[lo], len = bound[lo + 1] - start, k = t - first[lo];
+    it.pad = 0;
+    if (dead) {
+      it.start = start + k * step; it.len = min(step, len - k * step); it.tile = -1;
+      return PLAN_BINS - 1;
+    }
+    it.start = start; it.len = len; it.tile = k;
+    const int work = which ? (len - k * 128 - 1) / other + 1 : min(len - 1, k * step + step - 1) / 128 + 1;
+    const int level = min(PLAN_LEVELS - 1, int((long long)work * PLAN_LEVELS / most_work));
+    return min(start / p.span_rows[which], PLAN_SPANS - 1) * PLAN_LEVELS + (PLAN_LEVELS - 1 - level);
+  };
+  for (int t = tid; t < tiles; t += PLAN_THREADS) {
+    PackedItem it;
+    atomicAdd(&bins[item_of(t, it)], 1);
+  }
+  __syncthreads();
+  if (tid == 0) s_carry = 0;
+  __syncthreads();
+  for (int base = 0; base < PLAN_BINS; base += PLAN_THREADS) {
+    const int v = bins[base + tid];
+    const int carry = s_carry;
+    const int s = carry + block_scan(v, shared, add, 0);
+    bins[base + tid] = s - v;
+    __syncthreads();
+    if (tid == PLAN_THREADS - 1) s_carry = s;
+    __syncthreads();
+  }
+  for (int t = tid; t < tiles; t += PLAN_THREADS) {
+    PackedItem it;
+    const int b = item_of(t, it);
+    p.items[which][atomicAdd(&bins[b], 1)] = it;          // the order inside a bin decides when a tile runs, not what it computes
+  }
+  for (int t = tiles + tid; t < p.cap[which]; t += PLAN_THREADS) p.items[which][t] = PackedItem{0, 0, 0, 0};
+  if (tid == 0 && which == 0 && s_bad && p.err) atomicExch(p.err, ERR_SEQLENS);
+}
+
+// -----------------------------------------------------------------------------------------------
+// shared pieces
+// -----------------------------------------------------------------------------------------------
+// Which tile of which key head a CTA of the flat grid takes: spans of heads one after the other, inside them the head changes
+// fastest, so that the list's order (long tiles first) holds across heads.
+struct PackedTile { PackedItem it; int kv; };
+__device__ __forceinline__ PackedTile packed_tile(const PackedArgs& p, const PackedItem* items, int n, int block) {
+  const int per = p.head_span * n, g = block / per, i = block - g * per;
+  const int heads = min(p.head_span, p.KV - g * p.head_span);
+  PackedTile t;
+  const int k = i / heads;
+  const int4 v = k < n ? *reinterpret_cast<const int4*>(items + k) : make_int4(0, 0, 0, 0);
+  t.it = PackedItem{v.x, v.y, v.z, v.w};
+  t.kv = g * p.head_span + i - k * heads;
+  return t;
+}
+
+// Rows [from, to) of a 128-row tile of D columns, set to zero by the 32 lanes of a warp
+template <int D>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int lane) {
+  const uint32_t base = smem_u32(tile);
+  const int n = (to - from) * (D / 8);                    // 16-byte pieces: eight per row and 64-column half
+  for (int i = lane; i < n; i += 32) {
+    const int r = from + i / (D / 8), c = i % (D / 8);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + uint32_t(c >> 3) * 16384u + uint32_t(r) * 128u + uint32_t(c & 7) * 16u), "r"(0) : "memory");
+  }
+}
+// ... and made visible to the tensor core before `bar` is arrived on
+template <int D>
+__device__ __forceinline__ void clean_tile(uint8_t* tile, int from, int to, uint64_t* bar, int lane) {
+  zero_rows<D>(tile, from, to, lane);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+template <int D>
+__device__ __forceinline__ void load_kv(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int kv, int row) {
+  tma_load_3d(dst, m, bar, 0, kv, row);
+  if (D == 128) tma_load_3d(dst + 16384, m, bar, 64, kv, row);
+}
+template <int D>
+__device__ __forceinline__ void load_q(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int kv, int row) {
+  tma_load_4d(dst, m, bar, 0, 0, kv, row);
+  if (D == 128) tma_load_4d(dst + 16384, m, bar, 64, 0, kv, row);
+}
+
+// 32 accumulator columns of one row as bf16
+__device__ __forceinline__ void store32(__nv_bfloat16* dst, const uint32_t (&v)[32], float s) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    uint4 u;
+    u.x = pack_bf16(__uint_as_float(v[j]) * s, __uint_as_float(v[j + 1]) * s);
+    u.y = pack_bf16(__uint_as_float(v[j + 2]) * s, __uint_as_float(v[j + 3]) * s);
+    u.z = pack_bf16(__uint_as_float(v[j + 4]) * s, __uint_as_float(v[j + 5]) * s);
+    u.w = pack_bf16(__uint_as_float(v[j + 6]) * s, __uint_as_float(v[j + 7]) * s);
+    *reinterpret_cast<uint4*>(dst + j) = u;
+  }
+}
+// `n` rows from `row` of `width` elements each, zero
+__device__ __forceinline__ void zero_out(__nv_bfloat16* dst, long long ld, int row, int n, int width) {
+  const int per = width / 8;
+  for (int i = threadIdx.x; i < n * per; i += blockDim.x)
+    *reinterpret_cast<uint4*>(dst + (long long)(row + i / per) * ld + (i % per) * 8) = make_uint4(0, 0, 0, 0);
+}
+
+// -----------------------------------------------------------------------------------------------
+// forward
+// -----------------------------------------------------------------------------------------------
+template <int D>
+struct PackedFwdSmem {
+  static constexpr int TILE = 128 * D * 2;
+  static constexpr int Q = 0, K = TILE, V = 2 * TILE;
+  static constexpr int BAR = 3 * TILE;
+  static constexpr int TOTAL = BAR + 128 + 1024;         // + alignment slack
+};
+
+template <int D>
+__global__ void __launch_bounds__(ATT_THREADS, 2)
+attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const PackedArgs p) {
+  using L = PackedFwdSmem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* q_full = bars;
+  uint64_t* k_full = bars + 1;
+  uint64_t* v_full = bars + 2;
+  uint64_t* s_full = bars + 3;        // S(t) complete: scores readable, K slot free
+  uint64_t* p_full = bars + 4;        // [2] P(t) of keys 64..127, then of keys 0..63, written (4 arrivals)
+  uint64_t* pv_done = bars + 6;       // P V(t) complete: V slot free, after the last one O is final
+  uint64_t* v_land = bars + 7;        // a V tile that has to be cleaned has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1); mbar_init(k_full, 1); mbar_init(v_full, 1);
+    mbar_init(s_full, 1); mbar_init(&p_full[0], 4); mbar_init(&p_full[1], 4); mbar_init(pv_done, 1); mbar_init(v_land, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, 256); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_enter();                 // global memory is not touched above
+  const uint32_t TM_S = tmem, TM_P = tmem + 64, TM_O = tmem + 128;
+
+  const PackedTile tile = packed_tile(p, p.items_q, p.n_q, int(blockIdx.x));
+  const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+  const int H = p.KV * p.G;
+  if (len > 0 && tile.it.tile < 0) {                     // rows of no sequence
+    zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D);
+    for (int i = threadIdx.x; i < len * p.G; i += blockDim.x)
+      p.lse[(long long)(start + i / p.G) * H + kv * p.G + i % p.G] = -INFINITY;
+  } else if (len > 0) {
+    const int m0 = tile.it.tile * p.P, m_last = min(m0 + p.P, len) - 1;       // first and last position of the tile
+    const int j_lo = max(0, m0 - p.window) / 128;
+    const int n_tiles = m_last / 128 - j_lo + 1;
+    const int live = len - (j_lo + n_tiles - 1) * 128;   // rows of the last key tile that belong to the sequence
+    const bool clean = live < 128;
+    if (warp == 0) {
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+        mbar_expect_tx(q_full, uint32_t(p.P * p.G * D * 2));          // rows past the end of the tensor are zero-filled
+        load_q<D>(smem + L::Q, &tmQ, q_full, kv, start + m0);
+        for (int t = 0; t < n_tiles; ++t) {
+          const int row = start + (j_lo + t) * 128;
+          if (t > 0 && !mbar_wait(s_full, uint32_t(t - 1) & 1u, abort_flag)) break;
+          mbar_expect_tx(k_full, L::TILE);
+          load_kv<D>(smem + L::K, &tmK, k_full, kv, row);
+          if (t > 0 && !mbar_wait(pv_done, uint32_t(t - 1) & 1u, abort_flag)) break;
+          uint64_t* bar = (clean && t == n_tiles - 1) ? v_land : v_full;
+          mbar_expect_tx(bar, L::TILE);
+          load_kv<D>(smem + L::V, &tmV, bar, kv, row);
+        }
+      }
+      __syncwarp();
+      if (clean && mbar_wait(v_land, 0, abort_flag)) clean_tile<D>(smem + L::V, live, 128, v_full, lane);
+    } else if (warp == 1) {
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
+        constexpr uint32_t idesc_o = make_idesc_bf16(128, D, false, true);
+        // descriptor words once; a K slice is a 32-bit add on the low word (start address >> 4)
+        const uint32_t hi_k = uint32_t(make_smem_desc(0, 0, 1024) >> 32), hi_v = uint32_t(make_smem_desc(0, 16384, 1024) >> 32);
+        const uint32_t q_lo = uint32_t(make_smem_desc(smem_u32(smem + L::Q), 0, 1024));
+        const uint32_t k_lo = uint32_t(make_smem_desc(smem_u32(smem + L::K), 0, 1024));
+        const uint32_t v_lo = uint32_t(make_smem_desc(smem_u32(smem + L::V), 16384, 1024));
+        bool ok = mbar_wait(q_full, 0, abort_flag);
+        auto issue_s = [&](int t) {
+          if (!mbar_wait(k_full, uint32_t(t) & 1u, abort_flag)) { ok = false; return; }
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = uint32_t(k >> 2) * 1024u + uint32_t(k & 3) * 2u;     // (16 KB half, 32 B slice) >> 4
+            tc_mma_ss_lh(TM_S, q_lo + off, hi_k, k_lo + off, hi_k, idesc_s, k > 0);
+          }
+          tc_commit(s_full);
+        };
+        if (ok) issue_s(0);
+        for (int t = 0; t < n_tiles && ok; ++t) {
+          if (!mbar_wait(v_full, uint32_t(t) & 1u, abort_flag)) { ok = false; break; }
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {              // the upper keys' products run under the lower keys' exponentials
+            if (!mbar_wait(&p_full[hf], uint32_t(t) & 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t k = uint32_t(hf ? i : 4 + i);
+              tc_mma_ts_lh(TM_O, TM_P + k * 8u, v_lo + k * 128u, hi_v, idesc_o, (t > 0 || hf > 0 || i > 0) ? 1u : 0u);
+            }
+          }
+          if (!ok) break;
+          tc_commit(pv_done);
+          if (t + 1 < n_tiles) issue_s(t + 1);          // behind P V(t), which reads columns of the tile it overwrites
+        }
+      }
+    } else {
+      // ---------------- softmax / epilogue: thread <-> row of the tile = (position, head of the group) ----------------
+      const int q = warp & 3;
+      const int r = q * 32 + lane;
+      const int at = r / p.G, pos = m0 + at;
+      const bool live_row = at < p.P && pos < len;
+      const uint32_t lane_addr = uint32_t(q * 32) << 16;
+      const float c = p.scale * LOG2E;
+      float m_used = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int t = 0; t < n_tiles; ++t) {
+        const int n0 = (j_lo + t) * 128;
+        if (!mbar_wait(s_full, uint32_t(t) & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        // rows without a query see nothing, in the unmasked tiles too only their own, unused results differ
+        const bool need_mask = (n0 + 127 > m0) || (n0 < m_last - p.window);
+        // visible keys of this row inside the tile: column indices [mlo, mlo + span]
+        const int mlo = live_row ? pos - p.window - n0 : 128;
+        const unsigned span = live_row ? unsigned(p.window) : 0u;
+        uint32_t sc[32], sd[32];                           // columns 64..127 stay in registers
+        float mx;
+        {
+          uint32_t sa[32], sb[32];
+          tmem_ld32(TM_S + lane_addr, sa);
+          tmem_ld32(TM_S + lane_addr + 32u, sb);
+          tmem_wait_ld();
+          tmem_ld32(TM_S + lane_addr + 64u, sc);
+          tmem_ld32(TM_S + lane_addr + 96u, sd);
+          if (need_mask) mx = max32<true>(sb, 32, mlo, span, max32<true>(sa, 0, mlo, span, -INFINITY));
+          else mx = max32<false>(sb, 32, mlo, span, max32<false>(sa, 0, mlo, span, -INFINITY));
+          tmem_wait_ld();
+        }
+        if (need_mask) mx = max32<true>(sd, 96, mlo, span, max32<true>(sc, 64, mlo, span, mx));
+        else mx = max32<false>(sd, 96, mlo, span, max32<false>(sc, 64, mlo, span, mx));
+        const float m_new = fmaxf(m_used, mx);
+        bool resc = false;
+        if (m_used == -INFINITY) m_used = m_new;            // nothing accumulated for this row yet
+        else resc = (m_new - m_used) * c > 8.f;
+        if (t > 0 && __any_sync(0xffffffffu, resc)) {
+          // S(t) complete implies P V(t-1) complete: O is not in flight
+          const float alpha = resc ? fast_exp2((m_used - m_new) * c) : 1.f;
+          if (resc) { l *= alpha; m_used = m_new; }
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t v[32];
+            tmem_ld32(TM_O + lane_addr + uint32_t(cc * 32), v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+            tmem_st32(TM_O + lane_addr + uint32_t(cc * 32), v);
+          }
+          tmem_wait_st();
+        }
+        const float mc = (m_used == -INFINITY) ? 0.f : m_used * c;
+        const unsigned long long c2 = pk2(c, c), nmc2 = pk2(-mc, -mc);
+        unsigned long long rs2 = pk2(0.f, 0.f);
+        {
+          uint32_t pk[32];
+          if (need_mask) {
+            exp32_mufu<true>(sc, pk, c2, nmc2, 64, mlo, span, rs2);
+            exp32_mufu<true>(sd, pk + 16, c2, nmc2, 96, mlo, span, rs2);
+          } else {
+            exp32_mufu<false>(sc, pk, c2, nmc2, 64, mlo, span, rs2);
+            exp32_mufu<false>(sd, pk + 16, c2, nmc2, 96, mlo, span, rs2);
+          }
+          tmem_st32(TM_P + lane_addr + 32u, pk);           // over scores that have been read
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[0]);
+        {
+          uint32_t sa[32], sb[32], pk[32];
+          tmem_ld32(TM_S + lane_addr, sa);
+          tmem_ld32(TM_S + lane_addr + 32u, sb);
+          tmem_wait_ld();
+          if (need_mask) {
+            exp32_mufu<true>(sa, pk, c2, nmc2, 0, mlo, span, rs2);
+            exp32_mufu<true>(sb, pk + 16, c2, nmc2, 32, mlo, span, rs2);
+          } else {
+            exp32_mufu<false>(sa, pk, c2, nmc2, 0, mlo, span, rs2);
+            exp32_mufu<false>(sb, pk + 16, c2, nmc2, 32, mlo, span, rs2);
+          }
+          tmem_st32(TM_P + lane_addr, pk);
+        }
+        float r0, r1;
+        unpk2(rs2, r0, r1);
+        l += r0 + r1;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[1]);
+      }
+      if (ok && mbar_wait(pv_done, uint32_t(n_tiles - 1) & 1u, abort_flag)) {
+        tc_fence_after();
+        const float inv_l = (l > 0.f) ? 1.f / l : 0.f;
+        const int head = kv * p.G + (r - at * p.G);
+        __nv_bfloat16* orow = p.o + (long long)(start + pos) * p.ldo + (long long)head * D;
+#pragma unroll
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t v[32];
+          tmem_ld32(TM_O + lane_addr + uint32_t(cc * 32), v);
+          tmem_wait_ld();
+          if (live_row) store32(orow + cc * 32, v, inv_l);
+        }
+        if (live_row) p.lse[(long long)(start + pos) * H + head] = (l > 0.f) ? (m_used * p.scale + __logf(l)) : -INFINITY;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, ERR_ATTN_TIMEOUT);
+  if (warp == 1) { __syncwarp(); tc_fence_after(); tmem_dealloc(tmem, 256); }
+}
+
+// -----------------------------------------------------------------------------------------------
+// backward
+// -----------------------------------------------------------------------------------------------
+// two resident tiles, a three-slot and a two-slot ring
+template <int D>
+struct PackedBwdSmem {
+  static constexpr int TILE = 128 * D * 2;
+  static constexpr int RES0 = 0, RES1 = TILE;
+  static constexpr int RING3 = 2 * TILE;
+  static constexpr int RING2 = 5 * TILE;
+  static constexpr int STAT = 7 * TILE;                  // lse2[2][128], delta[2][128] (dK/dV)
+  static constexpr int BAR = STAT + 4 * 128 * 4;
+  static constexpr int TOTAL = BAR + 512;
+};
+static_assert(PackedBwdSmem<128>::TOTAL <= 232448, "exceeds the 227 KB shared memory of one CTA");
+
+// 128 x 128 product over the D columns of two K-major tiles
+template <int D>
+__device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t sa, uint32_t sb) {
+  constexpr uint32_t idesc = make_idesc_bf16(128, 128, false, false);
+  const uint32_t hi = uint32_t(make_smem_desc(0, 0, 1024) >> 32);
+  const uint32_t al = uint32_t(make_smem_desc(sa, 0, 1024)), bl = uint32_t(make_smem_desc(sb, 0, 1024));
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    const uint32_t off = uint32_t(k >> 2) * 1024u + uint32_t(k & 3) * 2u;       // (16 KB half, 32 B slice) >> 4
+    tc_mma_ss_lh(d_tmem, al + off, hi, bl + off, hi, idesc, k > 0);
+  }
+}
+// 128 x D (+)= A[tmem, 128 x 128 bf16 as two groups of 32 columns] * B[128-row tile, rows are the summed dimension]
+template <int D>
+__device__ __forceinline__ void mma_sum(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t sb, bool accumulate) {
+  constexpr uint32_t idesc = make_idesc_bf16(128, D, false, true);
+  const uint32_t hi = uint32_t(make_smem_desc(0, 16384, 1024) >> 32), bl = uint32_t(make_smem_desc(sb, 16384, 1024));
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    tc_mma_ts_lh(d_tmem, (k < 4 ? a_lo : a_hi) + uint32_t(k & 3) * 8u, bl + uint32_t(k) * 128u, hi, idesc, (accumulate || k > 0) ? 1u : 0u);
+}
+
+// ---- dQ: query tile stationary -----------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
+                                              const CUtensorMap& tmDO, const PackedArgs& p, int block) {
+  using L = PackedBwdSmem<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* q_full = bars;            // Q + dO resident
+  uint64_t* k_full = bars + 1;        // [3]
+  uint64_t* v_full = bars + 4;        // [2]
+  uint64_t* s_full = bars + 6;        // S(t) complete
+  uint64_t* a_done = bars + 7;        // phase A(t) has read S(t)            (8 arrivals)
+  uint64_t* dp_full = bars + 8;       // [2] dP(t) complete; also frees V(t)'s slot
+  uint64_t* ds_full = bars + 10;      // [2] phase B(t) wrote dS(t) and has read dP(t) (8 arrivals)
+  uint64_t* dq_done = bars + 12;      // [6] dQ(t) MMAs complete: frees K(t)'s slot and dS buffer t&1
+  uint64_t* done = bars + 18;         // all dQ MMAs complete
+  uint64_t* land = bars + 19;         // [2] K / V tile that has to be cleaned has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&k_full[i], 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&v_full[i], 1); mbar_init(&dp_full[i], 1); mbar_init(&ds_full[i], 8); mbar_init(&land[i], 1); }
+    mbar_init(s_full, 1); mbar_init(a_done, 8);
+    for (int i = 0; i < 6; ++i) mbar_init(&dq_done[i], 1);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_enter();                 // global memory is not touched above
+  const uint32_t TM_S = tmem, TM_DP = tmem + 128, TM_DQ = tmem + 256, TM_DS = tmem + 384;
+
+  const PackedTile tile = packed_tile(p, p.items_q, p.n_q, block);
+  const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+  const int H = p.KV * p.G;
+  if (len > 0 && tile.it.tile < 0) {                     // rows of no sequence
+    zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D);
+  } else if (len > 0) {
+    const int m0 = tile.it.tile * p.P, m_last = min(m0 + p.P, len) - 1;
+    const int j_lo = max(0, m0 - p.window) / 128;
+    const int n_tiles = m_last / 128 - j_lo + 1;
+    const int live = len - (j_lo + n_tiles - 1) * 128;   // rows of the last key tile that belong to the sequence
+    const bool clean = live < 128;
+    if (warp == 0) {
+      const uint32_t q_bytes = uint32_t(p.P * p.G * D * 2);
+      auto k_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
+      auto v_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
+      // K(t) is requested when dQ(t-3) has released its slot, V(t) when dP(t-2) has
+      auto load_k_tile = [&](int t, uint64_t* bar) -> bool {
+        if (t >= 3 && !mbar_wait(&dq_done[(t - 3) % 6], uint32_t((t - 3) / 6) & 1u, abort_flag)) return false;
+        mbar_expect_tx(bar, L::TILE);
+        load_kv<D>(k_slot(t), &tmK, bar, kv, start + (j_lo + t) * 128);
+        return true;
+      };
+      auto load_v_tile = [&](int t, uint64_t* bar) -> bool {
+        if (t >= 2 && !mbar_wait(&dp_full[t & 1], uint32_t((t - 2) >> 1) & 1u, abort_flag)) return false;
+        mbar_expect_tx(bar, L::TILE);
+        load_kv<D>(v_slot(t), &tmV, bar, kv, start + (j_lo + t) * 128);
+        return true;
+      };
+      const int last = n_tiles - 1;
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmDO);
+        mbar_expect_tx(q_full, 2 * q_bytes);
+        load_q<D>(smem + L::RES0, &tmQ, q_full, kv, start + m0);
+        load_q<D>(smem + L::RES1, &tmDO, q_full, kv, start + m0);
+        bool ok = true;
+        for (int t = 0; ok && t < n_tiles - (clean ? 1 : 0); ++t)
+          ok = load_k_tile(t, &k_full[t % 3]) && load_v_tile(t, &v_full[t & 1]);
+        if (clean && ok) ok = load_k_tile(last, &land[0]) && load_v_tile(last, &land[1]);
+      }
+      __syncwarp();
+      // both are summed over or multiplied with: rows of other sequences must not leave a NaN behind
+      if (clean && mbar_wait(&land[0], 0, abort_flag)) {
+        clean_tile<D>(k_slot(last), live, 128, &k_full[last % 3], lane);
+        if (mbar_wait(&land[1], 0, abort_flag)) clean_tile<D>(v_slot(last), live, 128, &v_full[last & 1], lane);
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        const uint32_t sq = smem_u32(smem + L::RES0), sdo = smem_u32(smem + L::RES1);
+        const uint32_t sk0 = smem_u32(smem + L::RING3), sv0 = smem_u32(smem + L::RING2);
+        bool ok = mbar_wait(q_full, 0, abort_flag);
+        if (ok) ok = mbar_wait(&k_full[0], 0, abort_flag);
+        if (ok) {
+          tc_fence_after();
+          mma_scores<D>(TM_S, sq, sk0);
+          tc_commit(s_full);
+          ok = mbar_wait(&v_full[0], 0, abort_flag);
+        }
+        if (ok) {
+          tc_fence_after();
+          mma_scores<D>(TM_DP, sdo, sv0);
+          tc_commit(&dp_full[0]);
+        }
+        for (int t = 0; t < n_tiles && ok; ++t) {
+          const bool more = t + 1 < n_tiles;
+          if (more) {
+            if (!mbar_wait(a_done, uint32_t(t & 1), abort_flag)) { ok = false; break; }
+            if (!mbar_wait(&k_full[(t + 1) % 3], uint32_t((t + 1) / 3) & 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            mma_scores<D>(TM_S, sq, sk0 + uint32_t((t + 1) % 3) * L::TILE);
+            tc_commit(s_full);
+          }
+          if (!mbar_wait(&ds_full[t & 1], uint32_t(t >> 1) & 1u, abort_flag)) { ok = false; break; }
+          if (more) {
+            if (!mbar_wait(&v_full[(t + 1) & 1], uint32_t((t + 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            mma_scores<D>(TM_DP, sdo, sv0 + uint32_t((t + 1) & 1) * L::TILE);
+            tc_commit(&dp_full[(t + 1) & 1]);
+          }
+          tc_fence_after();
+          const uint32_t ds = TM_DS + uint32_t(t & 1) * 64u;
+          mma_sum<D>(TM_DQ, ds, ds + 32, sk0 + uint32_t(t % 3) * L::TILE, t > 0);
+          tc_commit(&dq_done[t % 6]);
+        }
+        if (ok) tc_commit(done);
+      }
+    } else {
+      const int sw = warp - 2;             // 0..7
+      const int q = warp & 3;              // TMEM lane quarter this warp may access
+      const int hf = sw >> 2;              // column half of the tile owned by this warp
+      const int r = q * 32 + lane;
+      const int at = r / p.G, pos = m0 + at;
+      const int head = kv * p.G + (r - at * p.G);
+      const bool live_row = at < p.P && pos < len;
+      const uint32_t lane_addr = uint32_t(q * 32) << 16;
+      const float c = p.scale * LOG2E;
+      const long long stat = (long long)(start + pos) * H + head;
+      const float lse2 = live_row ? p.lse[stat] * LOG2E : INFINITY;
+      const float dlt = live_row ? p.delta[stat] : 0.f;
+      bool ok = true;
+      for (int t = 0; t < n_tiles && ok; ++t) {
+        const int n0 = (j_lo + t) * 128 + hf * 64;   // first key of this thread's 64 columns
+        float pr[64];
+        // ---- phase A ----
+        if (!mbar_wait(s_full, uint32_t(t & 1), abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        {
+          uint32_t s0[32], s1[32];
+          tmem_ld64(TM_S + lane_addr + uint32_t(hf * 64), s0, s1);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(a_done);
+          exp2_64<true>(s0, s1, c, lse2, nullptr, pr);
+          if ((n0 + 63 > m0) || (n0 < m_last - p.window)) {
+            // the visible keys of a row are one interval of column indices
+            const int lo = live_row ? pos - p.window - n0 : 64;
+            const unsigned span = live_row ? unsigned(p.window) : 0u;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) pr[j] = (unsigned(j - lo) <= span) ? pr[j] : 0.f;
+          }
+        }
+        // ---- phase B ----
+        if (!mbar_wait(&dp_full[t & 1], uint32_t(t >> 1) & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t pk[32];
+        {
+          uint32_t d0[32], d1[32];
+          tmem_ld64(TM_DP + lane_addr + uint32_t(hf * 64), d0, d1);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            pk[j] = pack_bf16(pr[2 * j] * (__uint_as_float(d0[2 * j]) - dlt), pr[2 * j + 1] * (__uint_as_float(d0[2 * j + 1]) - dlt));
+            pk[16 + j] = pack_bf16(pr[32 + 2 * j] * (__uint_as_float(d1[2 * j]) - dlt),
+                                   pr[32 + 2 * j + 1] * (__uint_as_float(d1[2 * j + 1]) - dlt));
+          }
+        }
+        // dS buffer t&1 was last read by the dQ MMAs of tile t-2
+        if (t >= 2 && !mbar_wait(&dq_done[(t - 2) % 6], uint32_t((t - 2) / 6) & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        tmem_st32(TM_DS + lane_addr + uint32_t((t & 1) * 64 + hf * 32), pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[t & 1]);
+      }
+      if (ok && mbar_wait(done, 0, abort_flag)) {
+        tc_fence_after();
+        __nv_bfloat16* orow = p.o + (long long)(start + pos) * p.ldo + (long long)head * D + hf * (D / 2);
+#pragma unroll
+        for (int cc = 0; cc < D / 64; ++cc) {
+          uint32_t v[32];
+          tmem_ld32(TM_DQ + lane_addr + uint32_t(hf * (D / 2) + cc * 32), v);
+          tmem_wait_ld();
+          if (live_row) store32(orow + cc * 32, v, p.scale);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, ERR_ATTN_TIMEOUT);
+  if (warp == 1) { __syncwarp(); tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// ---- dK / dV: key tile stationary, transposed scores; the query tiles bring all heads of the group -------------------
+template <int D>
+__device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
+                                               const CUtensorMap& tmDO, const PackedArgs& p, int block) {
+  using L = PackedBwdSmem<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* kv_full = bars;           // K + V resident
+  uint64_t* q_full = bars + 1;        // [3]
+  uint64_t* q_empty = bars + 4;       // [3] dK(t) complete
+  uint64_t* do_full = bars + 7;       // [2]
+  uint64_t* do_empty = bars + 9;      // [2] dV(t) complete
+  uint64_t* s_full = bars + 11;       // S^T(t) complete
+  uint64_t* p_full = bars + 12;       // phase A(t) wrote P^T(t)              (8 arrivals)
+  uint64_t* dp_full = bars + 13;      // dP^T(t) complete
+  uint64_t* ds_full = bars + 14;      // phase B(t) wrote dS^T(t)             (8 arrivals)
+  uint64_t* done = bars + 15;
+  uint64_t* land = bars + 16;         // [2] Q / dO tile that has to be cleaned has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* stat_lse = reinterpret_cast<float*>(smem + L::STAT);   // [2][128]
+  float* stat_dl = stat_lse + 256;                               // [2][128]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int used = p.P * p.G;           // rows of a query tile that hold queries
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < 3; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&do_full[i], 1); mbar_init(&do_empty[i], 1); mbar_init(&land[i], 1); }
+    mbar_init(s_full, 1); mbar_init(p_full, 8); mbar_init(dp_full, 1); mbar_init(ds_full, 8); mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (used < 128 && warp >= 2 && warp < 7) {              // rows that no copy fills, in the five slots: they are summed over as well
+    zero_rows<D>(smem + L::RING3 + (warp - 2) * L::TILE, used, 128, lane);
+    fence_proxy_async_smem();
+  }
+  static_assert(L::RING2 == L::RING3 + 3 * L::TILE, "the rings follow one another");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_enter();                 // global memory is not touched above
+  const uint32_t TM_S = tmem, TM_DP = tmem + 128, TM_DV = tmem + 256, TM_DK = tmem + 384;
+
+  const PackedTile tile = packed_tile(p, p.items_k, p.n_k, block);
+  const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+  const int H = p.KV * p.G;
+  if (len > 0 && tile.it.tile < 0) {                     // rows of no sequence
+    zero_out(p.dk + (long long)kv * D, p.lddk, start, len, D);
+    zero_out(p.dv + (long long)kv * D, p.lddv, start, len, D);
+  } else if (len > 0) {
+    const int n0 = tile.it.tile * 128;
+    const int last_key = min(n0 + 127, len - 1);
+    const int last_q = min(len - 1, last_key + p.window);
+    const int i_lo = n0 / p.P;
+    const int n_tiles = last_q / p.P - i_lo + 1;
+    const int live = (len - (i_lo + n_tiles - 1) * p.P) * p.G;     // rows of the last query tile that belong to the sequence
+    const bool clean = live < used;
+    if (warp == 0) {
+      const uint32_t q_bytes = uint32_t(used * D * 2);
+      auto q_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
+      auto do_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
+      auto load_q_tile = [&](int t, uint64_t* bar) -> bool {
+        if (!mbar_wait(&q_empty[t % 3], (uint32_t(t / 3) & 1u) ^ 1u, abort_flag)) return false;
+        mbar_expect_tx(bar, q_bytes);
+        load_q<D>(q_slot(t), &tmQ, bar, kv, start + (i_lo + t) * p.P);
+        return true;
+      };
+      auto load_do_tile = [&](int t, uint64_t* bar) -> bool {
+        if (!mbar_wait(&do_empty[t & 1], (uint32_t(t >> 1) & 1u) ^ 1u, abort_flag)) return false;
+        mbar_expect_tx(bar, q_bytes);
+        load_q<D>(do_slot(t), &tmDO, bar, kv, start + (i_lo + t) * p.P);
+        return true;
+      };
+      const int last = n_tiles - 1;
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmDO);
+        mbar_expect_tx(kv_full, 2 * L::TILE);
+        load_kv<D>(smem + L::RES0, &tmK, kv_full, kv, start + n0);
+        load_kv<D>(smem + L::RES1, &tmV, kv_full, kv, start + n0);
+        bool ok = true;
+        for (int t = 0; ok && t < n_tiles - (clean ? 1 : 0); ++t)
+          ok = load_q_tile(t, &q_full[t % 3]) && load_do_tile(t, &do_full[t & 1]);
+        if (clean && ok) ok = load_q_tile(last, &land[0]) && load_do_tile(last, &land[1]);
+      }
+      __syncwarp();
+      if (clean && mbar_wait(&land[0], 0, abort_flag)) {
+        clean_tile<D>(q_slot(last), live, used, &q_full[last % 3], lane);
+        if (mbar_wait(&land[1], 0, abort_flag)) clean_tile<D>(do_slot(last), live, used, &do_full[last & 1], lane);
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        const uint32_t sk = smem_u32(smem + L::RES0), sv = smem_u32(smem + L::RES1);
+        const uint32_t sq0 = smem_u32(smem + L::RING3), sdo0 = smem_u32(smem + L::RING2);
+        bool ok = mbar_wait(kv_full, 0, abort_flag);
+        if (ok) ok = mbar_wait(&q_full[0], 0, abort_flag);
+        if (ok) {
+          tc_fence_after();
+          mma_scores<D>(TM_S, sk, sq0);
+          tc_commit(s_full);
+          ok = mbar_wait(&do_full[0], 0, abort_flag);
+        }
+        if (ok) {
+          tc_fence_after();
+          mma_scores<D>(TM_DP, sv, sdo0);
+          tc_commit(dp_full);
+        }
+        for (int t = 0; t < n_tiles && ok; ++t) {
+          const bool more = t + 1 < n_tiles;
+          const uint32_t sq = sq0 + uint32_t(t % 3) * L::TILE, sdo = sdo0 + uint32_t(t & 1) * L::TILE;
+          // dV(t) reads P^T(t) from the S^T tile; S^T(t+1) is issued after it and may then overwrite it
+          if (!mbar_wait(p_full, uint32_t(t & 1), abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          mma_sum<D>(TM_DV, TM_S, TM_S + 64, sdo, t > 0);
+          tc_commit(&do_empty[t & 1]);
+          if (more) {
+            if (!mbar_wait(&q_full[(t + 1) % 3], uint32_t((t + 1) / 3) & 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            mma_scores<D>(TM_S, sk, sq0 + uint32_t((t + 1) % 3) * L::TILE);
+            tc_commit(s_full);
+          }
+          if (!mbar_wait(ds_full, uint32_t(t & 1), abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          mma_sum<D>(TM_DK, TM_DP, TM_DP + 64, sq, t > 0);
+          tc_commit(&q_empty[t % 3]);
+          if (more) {
+            if (!mbar_wait(&do_full[(t + 1) & 1], uint32_t((t + 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            mma_scores<D>(TM_DP, sv, sdo0 + uint32_t((t + 1) & 1) * L::TILE);
+            tc_commit(dp_full);
+          }
+        }
+        if (ok) tc_commit(done);
+      }
+    } else {
+      const int sw = warp - 2;
+      const int q = warp & 3;
+      const int hf = sw >> 2;              // query-column half of the tile owned by this warp
+      const int r = q * 32 + lane;         // key row inside the tile
+      const int key = n0 + r;
+      const int tid = threadIdx.x - 64;    // 0..255
+      const uint32_t lane_addr = uint32_t(q * 32) << 16;
+      const float c = p.scale * LOG2E;
+      const int col = tid & 127, col_at = col / p.G, col_head = kv * p.G + (col - col_at * p.G);
+      auto load_stat = [&](int t) -> float {   // tid < 128: lse2 of column tid of tile t; else delta of column tid-128
+        const int pos = (i_lo + t) * p.P + col_at;
+        if (t >= n_tiles || col_at >= p.P || pos >= len) return (tid < 128) ? INFINITY : 0.f;
+        const long long at = (long long)(start + pos) * H + col_head;
+        return (tid < 128) ? p.lse[at] * LOG2E : p.delta[at];
+      };
+      (tid < 128 ? stat_lse : stat_dl)[col] = load_stat(0);
+      const int last_pos = min(key + min(p.window, len - 1 - n0), len - 1);      // last query that sees this key
+      bool ok = true;
+      for (int t = 0; t < n_tiles; ++t) {
+        const int q0 = (i_lo + t) * p.P;             // first position of the tile
+        const int buf = t & 1;
+        named_bar_sync(1, 256);                    // statistics of tile t are visible to all softmax warps
+        const float next_stat = load_stat(t + 1);  // in flight while this tile is processed
+        const float4* cl = reinterpret_cast<const float4*>(stat_lse + buf * 128 + hf * 64);
+        const float4* cd = reinterpret_cast<const float4*>(stat_dl + buf * 128 + hf * 64);
+        float pr[64];
+        // ---- phase A: P^T = exp2(S^T * c - lse2[query]) ----
+        if (ok && !mbar_wait(s_full, uint32_t(t & 1), abort_flag)) ok = false;
+        if (ok) {
+          tc_fence_after();
+          uint32_t s0[32], s1[32];
+          tmem_ld64(TM_S + lane_addr + uint32_t(hf * 64), s0, s1);
+          exp2_64<false>(s0, s1, c, 0.f, cl, pr);
+          if (q0 < n0 + 127 || q0 + p.P - 1 > n0 + p.window) {
+            // the queries that see a key are one interval of positions, key ... last_pos, and so of columns
+            const int lo = max(key - q0, 0) * p.G - hf * 64;
+            const int hi = (min(last_pos - q0, p.P - 1) + 1) * p.G - 1 - hf * 64;
+            const bool seen = key < len && last_pos >= q0 && hi >= lo;
+            const unsigned span = seen ? unsigned(hi - lo) : 0u;
+            const int lo_eff = seen ? lo : 64;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) pr[j] = (unsigned(j - lo_eff) <= span) ? pr[j] : 0.f;
+          }
+          uint32_t pk[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) pk[j] = pack_bf16(pr[2 * j], pr[2 * j + 1]);
+          tmem_st32(TM_S + lane_addr + uint32_t(hf * 64), pk);   // over this thread's own, already read, S^T columns
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full);
+        }
+        // ---- phase B: dS^T = P^T * (dP^T - delta[query]) ----
+        if (ok && !mbar_wait(dp_full, uint32_t(t & 1), abort_flag)) ok = false;
+        if (ok) {
+          tc_fence_after();
+          uint32_t d0[32], d1[32];
+          tmem_ld64(TM_DP + lane_addr + uint32_t(hf * 64), d0, d1);
+          uint32_t pk[32];
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const float4 e0 = cd[g], e1 = cd[8 + g];
+            pk[2 * g] = pack_bf16(pr[4 * g] * (__uint_as_float(d0[4 * g]) - e0.x), pr[4 * g + 1] * (__uint_as_float(d0[4 * g + 1]) - e0.y));
+            pk[2 * g + 1] = pack_bf16(pr[4 * g + 2] * (__uint_as_float(d0[4 * g + 2]) - e0.z),
+                                      pr[4 * g + 3] * (__uint_as_float(d0[4 * g + 3]) - e0.w));
+            pk[16 + 2 * g] = pack_bf16(pr[32 + 4 * g] * (__uint_as_float(d1[4 * g]) - e1.x),
+                                       pr[32 + 4 * g + 1] * (__uint_as_float(d1[4 * g + 1]) - e1.y));
+            pk[16 + 2 * g + 1] = pack_bf16(pr[32 + 4 * g + 2] * (__uint_as_float(d1[4 * g + 2]) - e1.z),
+                                           pr[32 + 4 * g + 3] * (__uint_as_float(d1[4 * g + 3]) - e1.w));
+          }
+          tmem_st32(TM_DP + lane_addr + uint32_t(hf * 64), pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ds_full);
+        }
+        (tid < 128 ? stat_lse : stat_dl)[((t + 1) & 1) * 128 + col] = next_stat;
+      }
+      if (ok && mbar_wait(done, 0, abort_flag)) {
+        tc_fence_after();
+        const long long at = kv * D + hf * (D / 2);
+        __nv_bfloat16* dkrow = p.dk + (long long)(start + key) * p.lddk + at;
+        __nv_bfloat16* dvrow = p.dv + (long long)(start + key) * p.lddv + at;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+#pragma unroll
+          for (int cc = 0; cc < D / 64; ++cc) {
+            uint32_t v[32];
+            tmem_ld32((which ? TM_DK : TM_DV) + lane_addr + uint32_t(hf * (D / 2) + cc * 32), v);
+            tmem_wait_ld();
+            if (key < len) store32((which ? dkrow : dvrow) + cc * 32, v, which ? p.scale : 1.f);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, ERR_ATTN_TIMEOUT);
+  if (warp == 1) { __syncwarp(); tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// One grid for both, the longer half first (attn_wide_sm100.cu).
+template <int D>
+__global__ void __launch_bounds__(ATT_WIDE_THREADS, 1)
+attn_packed_bwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ PackedArgs p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {   // the swizzled tiles need 1 KB alignment; nothing has been allocated yet
+    grid_wait();
+    if (threadIdx.x == 0 && p.err) atomicExch(p.err, ERR_SMEM_ALIGN);
+    return;
+  }
+  const int key_blocks = p.n_k * p.KV;
+  if (int(blockIdx.x) < key_blocks) packed_bwd_dkv<D>(tmQ, tmK, tmV, tmDO, p, int(blockIdx.x));
+  else packed_bwd_dq<D>(tmQ, tmK, tmV, tmDO, p, int(blockIdx.x) - key_blocks);
+}
+
+// delta[row, head] = sum_d dO * O in fp32: D / 8 lanes per (row, head)
+template <int D>
+__global__ void __launch_bounds__(256) attn_packed_delta_k(const __nv_bfloat16* o, long long ldo, const __nv_bfloat16* d_o, long long row_do,
+                                                           long long head_do, float* delta, long long n, int H) {
+  constexpr int LANES = D / 8;
+  grid_enter();
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const int l = threadIdx.x % LANES;
+  float acc = 0.f;
+  if (i < n) {
+    const long long row = i / H, head = i - row * H;
+    const uint4 a = *reinterpret_cast<const uint4*>(o + row * ldo + head * D + l * 8);
+    const uint4 b = *reinterpret_cast<const uint4*>(d_o + row * row_do + head * head_do + l * 8);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = unpack_bf16(aw[e]), y = unpack_bf16(bw[e]);
+      acc += x.x * y.x + x.y * y.y;
+    }
+  }
+#pragma unroll
+  for (int s = LANES / 2; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
+  if (l == 0 && i < n) delta[i] = acc;
+}
+
+// -----------------------------------------------------------------------------------------------
+// [D, G, KV, rows] view of the queries; one box is a query tile's 64-column half
+static int make_group_tmap(CUtensorMap* m, const void* base, const ArbPacked& a, long long row, long long head) {
+  const uint32_t P = 128 / uint32_t(a.G);
+  uint64_t dims[4] = {uint64_t(a.D), uint64_t(a.G), uint64_t(a.KV), uint64_t(a.rows)};
+  uint64_t str[3] = {uint64_t(head) * 2, uint64_t(head) * uint64_t(a.G) * 2, uint64_t(row) * 2};
+  uint32_t box[4] = {64, uint32_t(a.G), 1, P};
+  return make_tmap_bf16(m, base, 4, dims, str, box);
+}
+static int make_key_tmap(CUtensorMap* m, const void* base, const ArbPacked& a, long long row, long long head) {
+  uint64_t dims[3] = {uint64_t(a.D), uint64_t(a.KV), uint64_t(a.rows)};
+  uint64_t str[2] = {uint64_t(head) * 2, uint64_t(row) * 2};
+  uint32_t box[3] = {64, 1, 128};
+  return make_tmap_bf16(m, base, 3, dims, str, box);
+}
+
+static int check_packed(const ArbPacked& a) {
+  // positions plus a window stay within 31 bits
+  if (a.rows <= 0 || a.rows > PACKED_MAX_ROWS || a.KV <= 0 || a.KV > 65535 || a.G <= 0 || a.G > 128 || (a.D != 64 && a.D != 128) || a.window < 0) return -3;
+  if (!a.items || bad_ptr(a.items) || a.cap_q <= 0 || a.cap_k <= 0 || (a.cap_q + a.cap_k) * a.KV > 0x7fffffffll) return -3;
+  const void* ptrs[] = {a.q, a.k, a.v, a.o, a.d_o, a.dq, a.dk, a.dv};
+  const long long strides[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.v_row, a.v_head, a.o_row, a.do_row, a.do_head, a.dq_row, a.dk_row, a.dv_row};
+  for (const void* p : ptrs) if (bad_ptr(p)) return -4;
+  for (long long s : strides) if (s < 0 || (s & 7)) return -4;
+  return 0;
+}
+
+static PackedArgs packed_args(const ArbPacked& a, int* err) {
+  PackedArgs r{};
+  r.KV = int(a.KV); r.G = int(a.G); r.P = 128 / r.G;
+  r.items_q = reinterpret_cast<const PackedItem*>(a.items);
+  r.items_k = r.items_q + a.cap_q;
+  r.n_q = int(a.cap_q); r.n_k = int(a.cap_k);
+  r.head_span = r.KV < 8 ? r.KV : 8;
+  r.window = int(a.window < a.rows ? a.window : a.rows);
+  r.scale = float(a.scale);
+  r.lse = a.lse; r.delta = a.delta; r.err = err;
+  return r;
+}
+
+template <int D>
+static int packed_fwd(const ArbPacked& a, int* err, cudaStream_t stream) {
+  static PerDeviceOnce cfg;
+  if (cfg.first()) { if (int r = set_smem(attn_packed_fwd_k<D>, PackedFwdSmem<D>::TOTAL)) return r; }
+  CUtensorMap tq, tk, tv;
+  int r;
+  if ((r = make_group_tmap(&tq, a.q, a, a.q_row, a.q_head))) return 1000 + r;
+  if ((r = make_key_tmap(&tk, a.k, a, a.k_row, a.k_head))) return 1000 + r;
+  if ((r = make_key_tmap(&tv, a.v, a, a.v_row, a.v_head))) return 1000 + r;
+  PackedArgs p = packed_args(a, err);
+  p.o = reinterpret_cast<__nv_bfloat16*>(a.o); p.ldo = a.o_row;
+  return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(a.cap_q * a.KV), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk, tv, p);
+}
+
+template <int D>
+static int packed_bwd(const ArbPacked& a, int* err, cudaStream_t stream) {
+  static PerDeviceOnce cfg;
+  if (cfg.first()) { if (int r = set_smem(attn_packed_bwd_k<D>, PackedBwdSmem<D>::TOTAL)) return r; }
+  CUtensorMap tq, tk, tv, tdo;
+  int r;
+  if ((r = make_group_tmap(&tq, a.q, a, a.q_row, a.q_head))) return 1000 + r;
+  if ((r = make_key_tmap(&tk, a.k, a, a.k_row, a.k_head))) return 1000 + r;
+  if ((r = make_key_tmap(&tv, a.v, a, a.v_row, a.v_head))) return 1000 + r;
+  if ((r = make_group_tmap(&tdo, a.d_o, a, a.do_row, a.do_head))) return 1000 + r;
+  const int H = int(a.KV * a.G);
+  const long long n = a.rows * H, blocks = (n * (D / 8) + 255) / 256;
+  if (blocks > 0x7fffffffll) return -3;
+  if ((r = launch_dependent(n * D * 2 <= EARLY_BYTES, attn_packed_delta_k<D>, unsigned(blocks), 256, 0, stream,
+                            reinterpret_cast<const __nv_bfloat16*>(a.o), a.o_row, reinterpret_cast<const __nv_bfloat16*>(a.d_o), a.do_row,
+                            a.do_head, a.delta, n, H)))
+    return r;
+  PackedArgs p = packed_args(a, err);
+  p.o = reinterpret_cast<__nv_bfloat16*>(a.dq); p.ldo = a.dq_row;
+  p.dk = reinterpret_cast<__nv_bfloat16*>(a.dk); p.lddk = a.dk_row;
+  p.dv = reinterpret_cast<__nv_bfloat16*>(a.dv); p.lddv = a.dv_row;
+  return launch_dependent(true, attn_packed_bwd_k<D>, unsigned((a.cap_q + a.cap_k) * a.KV), ATT_WIDE_THREADS, PackedBwdSmem<D>::TOTAL, stream,
+                          tq, tk, tv, tdo, p);
+}
+
+}  // namespace arb
+
+using namespace arb;
+
+extern "C" int arb_packed_plan(const int* cu, int n_seq, int rows, int G, int span_rows, void* items, int cap_q, int cap_k, int* scratch,
+                               int* err_flag, cudaStream_t stream) {
+  if (!cu || !items || !scratch || n_seq < 0 || rows <= 0 || rows > PACKED_MAX_ROWS || G <= 0 || G > 128 || span_rows <= 0 || bad_ptr(items)) return -3;
+  PlanArgs p{};
+  p.cu = cu; p.n = n_seq; p.rows = rows; p.P = 128 / G;
+  // every sequence and the rows before and behind them end in at most one tile that is not full
+  const long long most_q = (long long)rows / p.P + n_seq + 2, most_k = (long long)rows / 128 + n_seq + 2;
+  if (cap_q < most_q || cap_k < most_k) return -6;
+  const long long n = (long long)n_seq + 3;
+  p.bound = scratch; p.first = scratch + 2 * n;
+  p.items[0] = reinterpret_cast<PackedItem*>(items); p.items[1] = p.items[0] + cap_q;
+  p.cap[0] = cap_q; p.cap[1] = cap_k;
+  p.span_rows[0] = p.span_rows[1] = span_rows;
+  p.err = err_flag;
+  return launch_dependent(true, packed_plan_k, 2, PLAN_THREADS, 0, stream, p);
+}
+
+extern "C" int arb_packed_attn_fwd(const ArbPacked* a, int* err_flag, cudaStream_t stream) {
+  if (!a || !a->q || !a->k || !a->v || !a->o || !a->lse) return -3;
+  if (int r = check_packed(*a)) return r;
+  return a->D == 64 ? packed_fwd<64>(*a, err_flag, stream) : packed_fwd<128>(*a, err_flag, stream);
+}
+
+extern "C" int arb_packed_attn_bwd(const ArbPacked* a, int* err_flag, cudaStream_t stream) {
+  if (!a || !a->q || !a->k || !a->v || !a->o || !a->lse || !a->d_o || !a->delta || !a->dq || !a->dk || !a->dv) return -3;
+  if (int r = check_packed(*a)) return r;
+  return a->D == 64 ? packed_bwd<64>(*a, err_flag, stream) : packed_bwd<128>(*a, err_flag, stream);
+}

@@ -75,30 +75,6 @@ __device__ __forceinline__ void mma_tile_ts(uint32_t d_tmem, uint32_t a_lo, uint
                  (accumulate || k > 0) ? 1u : 0u);
 }
 
-// exp2 of 64 scores of one row/lane; the offsets are one per-row value or 64 per-column values
-template <bool ROW_STAT>
-__device__ __forceinline__ void exp2_64(const uint32_t (&s0)[32], const uint32_t (&s1)[32], float c, float row_off,
-                                        const float4* col_off, float (&pr)[64]) {
-#pragma unroll
-  for (int g = 0; g < 16; ++g) {
-    float4 o = make_float4(row_off, row_off, row_off, row_off);
-    if (!ROW_STAT) o = col_off[g];
-    const float off[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int j = g * 4 + u;
-      const float x = __uint_as_float(j < 32 ? s0[j] : s1[j - 32]) * c - off[u];
-      pr[j] = fast_exp2(x);
-    }
-  }
-}
-
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&a)[32], uint32_t (&b)[32]) {
-  tmem_ld32(taddr, a);
-  tmem_ld32(taddr + 32, b);
-  tmem_wait_ld();
-}
-
 // ===============================================================================================
 // dQ
 // ===============================================================================================

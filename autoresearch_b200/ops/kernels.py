@@ -5,6 +5,7 @@ so a missing or failing native kernel is never silently replaced by a PyTorch fa
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import struct
@@ -22,7 +23,8 @@ _err_flag = {}
 EPI_STORE_BF16, EPI_RELU2, EPI_ATOMIC_F32, EPI_NS_COMBINE, EPI_RELU2_BWD, EPI_STORE_F32, EPI_ADD_AUX, EPI_QKV_POST, EPI_SYM_STORE, EPI_SYM_NS_COMBINE = range(10)
 ERR_NAMES = {1: "GEMM barrier wait timed out", 2: "attention barrier wait timed out",
              3: "peer barrier wait timed out", 4: "MoE dispatch wait timed out",
-             5: "dynamic shared memory base is not 1 KB aligned"}
+             5: "dynamic shared memory base is not 1 KB aligned",
+             6: "packed sequence bounds descend or lie outside of the rows"}
 
 launch_count = 0  # number of kernel-launching calls made through this module
 # B operands whose up-to-date copy still sits on another rank: data_ptr -> (peer pointer, bytes), registered by
@@ -69,6 +71,9 @@ def _signatures() -> dict:
                                  f32, f32, f32, vp, vp, vp, i64, vp, vp, i64, vp, i32, vp, i32],
         "arb_attn_fwd": [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, i32, f32, vp, vp],
         "arb_attn_bwd": [vp] * 11 + [i32, i32, i32] + [i64] * 8 + [i32, f32, vp, vp],
+        "arb_packed_plan": [vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, vp],
+        "arb_packed_attn_fwd": [vp, vp, vp],
+        "arb_packed_attn_bwd": [vp, vp, vp],
         "arb_rmsnorm_fwd": [vp, vp, i64, i32, f32, vp],
         "arb_rmsnorm_bwd": [vp, vp, vp, vp, i64, i32, f32, vp],
         "arb_resid_scale_norm_fwd": [vp, vp, vp, vp, i32, vp, vp, i64, i32, f32, vp],
@@ -128,6 +133,19 @@ def available() -> bool:
 
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one, so that a launch goes to that device and its current stream."""
+    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def count_launch(n: int = 1) -> None:
+    global launch_count
+    launch_count += n
 
 
 def _check(rc: int, what: str):

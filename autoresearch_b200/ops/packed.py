@@ -1,0 +1,220 @@
+"""Causal attention over packed sequences of different lengths, with grouped heads (csrc/attn_packed_sm100.cu).
+
+A packed batch is one [rows, heads, dim] tensor in which sequence i holds the rows ``cu_seqlens[i] .. cu_seqlens[i + 1]``;
+a query sees the keys of its own sequence at most ``window`` positions back:
+
+    o_i = sum_j softmax_j(scale * q_i . k_j) v_j,    i - window <= j <= i, same sequence
+
+``PackedSequences`` holds the tile lists of one packing; every layer of a model uses the same one in both directions::
+
+    seqs = PackedSequences(cu_seqlens, rows, n_head, n_kv_head)
+    out = packed_attention(q, k, v, seqs, window=256)            # differentiable in q, k, v
+"""
+from __future__ import annotations
+
+import math
+import struct
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import kernels as K
+
+_ARGS = struct.Struct("=30qd")          # ArbPacked of csrc/api.h: 11 pointers, 7 sizes, 12 strides, the scale
+MAX_ROWS = 1 << 30
+L2_SPAN_BYTES = 48 << 20                # keys and values whose tiles run together (126 MB of L2; attn_common.cuh)
+
+
+def check_bounds(bounds, rows: int) -> None:
+    """Raises unless ``bounds`` (host values) ascend from at least 0 to at most ``rows``."""
+    last = 0
+    for b in bounds:
+        if not last <= b <= rows:
+            raise ValueError(f"sequence bounds must ascend within [0, {rows}]: got {list(bounds)[:16]}")
+        last = b
+
+
+class PackedSequences:
+    """Which tiles the sequences of a packed batch have.
+
+    ``cu_seqlens``: n + 1 ascending row numbers, an int32 CUDA tensor, or host values (a list, a CPU tensor), which are checked
+    here.  Bounds that only the device knows are not read back: where they descend or leave the rows they are moved inside,
+    and ``kernels.check_err_flag()`` reports it.  Empty sequences are allowed.  Rows of no sequence (before the first bound
+    and behind the last) get zero outputs and gradients, whatever their inputs hold.
+
+    Made on the current stream; another stream has to wait for it, as for any tensor.  Under graph capture the lists are made
+    again with every replay, from what ``cu_seqlens`` holds then."""
+
+    def __init__(self, cu_seqlens, rows: int, n_head: int, n_kv_head: Optional[int] = None, device=None):
+        n_kv_head = n_head if n_kv_head is None else n_kv_head
+        if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head or n_head // n_kv_head > 128:
+            raise ValueError(f"{n_head} query heads do not form groups of at most 128 on {n_kv_head} key heads")
+        if not 0 <= rows <= MAX_ROWS:
+            raise ValueError(f"rows must lie in [0, {MAX_ROWS}], got {rows}")
+        if not (torch.is_tensor(cu_seqlens) and cu_seqlens.is_cuda):
+            values = cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else [int(b) for b in cu_seqlens]
+            if not values:
+                raise ValueError("cu_seqlens needs at least one bound")
+            check_bounds(values, rows)
+            cu_seqlens = torch.tensor(values, dtype=torch.int32, device=device if device is not None else "cuda")
+        elif cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype is not torch.int32:
+            raise TypeError("cu_seqlens must be a 1-D int32 tensor of at least one element")
+        self.cu_seqlens = cu_seqlens.contiguous()
+        self.rows, self.n_head, self.n_kv_head = rows, n_head, n_kv_head
+        self.n_seq = cu_seqlens.numel() - 1
+        self.group = n_head // n_kv_head
+        # bounds of the tile counts: every sequence and the rows before and behind them end in one tile that is not full
+        self.cap_q = rows // (128 // self.group) + self.n_seq + 2
+        self.cap_k = rows // 128 + self.n_seq + 2
+        self.device = cu_seqlens.device
+        if (self.cap_q + self.cap_k) * n_kv_head >= 1 << 31:
+            raise ValueError("too many tiles for one launch")
+        items = 4 * (self.cap_q + self.cap_k)
+        self.items = torch.empty(items + 4 * (self.n_seq + 3), dtype=torch.int32, device=self.device)
+        if rows:
+            span = max(128, L2_SPAN_BYTES // (512 * min(n_kv_head, 8)))
+            with K.on_device(self.device):
+                K._check(K.lib().arb_packed_plan(self.cu_seqlens.data_ptr(), self.n_seq, rows, self.group, span, self.items.data_ptr(),
+                                                 self.cap_q, self.cap_k, self.items.data_ptr() + 4 * items,
+                                                 K.err_flag(self.device).data_ptr(), K._stream()), "packed_plan")
+
+
+def _strided(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where the kernels can read it: unit inner stride, the others positive multiples of 8 elements, 16-byte
+    aligned; else a contiguous copy."""
+    s0, s1, s2 = t.stride()
+    n0, n1, _ = t.shape
+    if s2 == 1 and (n0 == 1 or (s0 > 0 and not s0 & 7)) and (n1 == 1 or (s1 > 0 and not s1 & 7)) and not t.data_ptr() & 15:
+        return t
+    return t.contiguous()
+
+
+def _strides(t: torch.Tensor):
+    """(row, head) stride; that of a dimension of size 1 is never used and may be anything."""
+    d = t.shape[2]
+    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * d), (t.stride(1) if t.shape[1] > 1 else d)
+
+
+def _call(entry: str, q, k, v, out, lse, seqs, window, scale, d_out=None, delta=None, dq=None, dk=None, dv=None) -> None:
+    strides = _strides(q) + _strides(k) + _strides(v) + (_strides(out)[0],)
+    if d_out is None:
+        ptrs, strides = (0, 0, 0, 0, 0), strides + (0, 0, 0, 0, 0)
+    else:
+        ptrs = (d_out.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+        strides += _strides(d_out) + (_strides(dq)[0], _strides(dk)[0], _strides(dv)[0])
+    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *ptrs, seqs.items.data_ptr(),
+                      seqs.rows, seqs.n_kv_head, seqs.group, q.shape[2], window, seqs.cap_q, seqs.cap_k, *strides, scale)
+    with K.on_device(q.device):
+        K._check(getattr(K.lib(), entry)(args, K.err_flag(q.device).data_ptr(), K._stream()), entry)
+
+
+def _forward(q, k, v, seqs, window, scale):
+    rows, H, d = q.shape
+    out = torch.empty(rows, H, d, dtype=q.dtype, device=q.device)
+    lse = torch.empty(rows, H, dtype=torch.float32, device=q.device)
+    if rows:
+        _call("arb_packed_attn_fwd", q, k, v, out, lse, seqs, window, scale)
+    return out, lse
+
+
+def _backward(q, k, v, out, lse, d_out, dq, dk, dv, seqs, window, scale):
+    if q.shape[0]:
+        d_out = _strided(d_out)
+        _call("arb_packed_attn_bwd", q, k, v, out, lse, seqs, window, scale, d_out, torch.empty_like(lse), dq, dk, dv)
+        K.count_launch()                 # the row sums of dO o O and the gradient grid
+
+
+class PackedAttentionFn(torch.autograd.Function):
+    """q [rows, H, d], k and v [rows, KV, d] -> [rows, H, d]."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, seqs, window, scale):
+        q, k, v = _strided(q), _strided(k), _strided(v)
+        out, lse = _forward(q, k, v, seqs, window, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.args = (seqs, window, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        q, k, v, out, lse = ctx.saved_tensors
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        _backward(q, k, v, out, lse, d_out, dq, dk, dv, *ctx.args)
+        return dq, dk, dv, None, None, None
+
+
+class PackedQKVAttentionFn(torch.autograd.Function):
+    """The same on the packed projection output [rows, (H + 2 KV) d]; its gradient is written in place of three tensors."""
+
+    @staticmethod
+    def forward(ctx, qkv, seqs, window, scale, d):
+        ctx.args, ctx.d = (seqs, window, scale), d
+        out, lse = _forward(*_blocks(qkv, seqs, d), seqs, window, scale)
+        ctx.save_for_backward(qkv, out, lse)
+        return out.view(qkv.shape[0], -1)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        qkv, out, lse = ctx.saved_tensors
+        seqs = ctx.args[0]
+        d_qkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _backward(*_blocks(qkv, seqs, ctx.d), out, lse, d_out.contiguous().view(out.shape), *_blocks(d_qkv, seqs, ctx.d), *ctx.args)
+        return d_qkv, None, None, None, None
+
+
+def _blocks(qkv, seqs, d):
+    H, KV = seqs.n_head, seqs.n_kv_head
+    t = qkv.view(qkv.shape[0], H + 2 * KV, d)
+    return t[:, :H], t[:, H:H + KV], t[:, H + KV:]
+
+
+def _common(device, rows, d, seqs, window, scale):
+    if not isinstance(seqs, PackedSequences):
+        raise TypeError("seqs must be a PackedSequences")
+    if d not in (64, 128):
+        raise ValueError(f"the kernels have head dimensions 64 and 128, not {d}")
+    if seqs.rows != rows or seqs.device != device:
+        raise ValueError(f"the sequences are packed in {seqs.rows} rows on {seqs.device}, the tensors have {rows} on {device}")
+    if window is None:
+        window = rows
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    return min(int(window), rows), 1.0 / math.sqrt(d) if scale is None else float(scale)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: PackedSequences, window: Optional[int] = None,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of packed sequences: q [rows, H, d], k and v [rows, KV, d], bf16, d = 64 or 128, any strides -> [rows, H, d].
+
+    Query head h reads key head h // (H / KV).  ``window``: how many positions back a query sees (None: all); ``scale``
+    defaults to 1 / sqrt(d).  The inputs of a sequence reach no other sequence's outputs or gradients, not even as NaN."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        K._bf16(t, name)
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [rows, heads, dim], got {tuple(t.shape)}")
+    rows, H, d = q.shape
+    window, scale = _common(q.device, rows, d, seqs, window, scale)
+    if H != seqs.n_head or k.shape != (rows, seqs.n_kv_head, d) or v.shape != k.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit {seqs.n_head} heads on "
+                         f"{seqs.n_kv_head} key heads")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must be on one device")
+    return PackedAttentionFn.apply(q, k, v, seqs, window, scale)
+
+
+def packed_qkv_attention(qkv: torch.Tensor, seqs: PackedSequences, window: Optional[int] = None, scale: Optional[float] = None,
+                         head_dim: int = 128) -> torch.Tensor:
+    """The same on the contiguous packed projection output [rows, (H + 2 KV) head_dim] -> [rows, H head_dim]."""
+    K._bf16(qkv, "qkv")
+    if qkv.dim() != 2 or not qkv.is_contiguous():
+        raise ValueError("qkv must be 2-D and contiguous")
+    rows = qkv.shape[0]
+    window, scale = _common(qkv.device, rows, head_dim, seqs, window, scale)
+    if qkv.shape[1] != (seqs.n_head + 2 * seqs.n_kv_head) * head_dim:
+        raise ValueError(f"qkv has {qkv.shape[1]} columns for {seqs.n_head} + 2 x {seqs.n_kv_head} heads of {head_dim}")
+    return PackedQKVAttentionFn.apply(qkv, seqs, window, scale, head_dim)

@@ -1,0 +1,82 @@
+"""Checks of packed sequences that need no device, and the backward formula of packed attention against differences."""
+import math
+
+import pytest
+import torch
+
+from autoresearch_b200.ops import kernels as K
+from autoresearch_b200.ops import packed as P
+
+
+@pytest.mark.parametrize("bounds,rows", [([0, 5, 3], 10), ([-1, 4], 10), ([0, 11], 10), ([4, 2], 10)])
+def test_host_bounds_are_checked(bounds, rows):
+    with pytest.raises(ValueError, match="ascend"):
+        P.PackedSequences(bounds, rows, 2, 1)
+    with pytest.raises(ValueError, match="ascend"):
+        P.PackedSequences(torch.tensor(bounds), rows, 2, 1)
+
+
+@pytest.mark.parametrize("heads,kv", [(3, 2), (0, 1), (4, 0), (129, 1), (-2, 1)])
+def test_head_layouts_that_do_not_group(heads, kv):
+    with pytest.raises(ValueError, match="group"):
+        P.PackedSequences([0, 4], 4, heads, kv)
+
+
+def test_empty_bounds_and_rows_out_of_range():
+    with pytest.raises(ValueError):
+        P.PackedSequences([], 4, 2, 1)
+    for rows in (-1, P.MAX_ROWS + 1):
+        with pytest.raises(ValueError, match="rows"):
+            P.PackedSequences([0], rows, 2, 1)
+
+
+def test_cpu_tensors_are_refused():
+    t = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="CUDA"):
+        P.packed_attention(t, t, t, None)
+    with pytest.raises(TypeError, match="CUDA"):
+        P.packed_qkv_attention(t.view(4, -1), None)
+
+
+def test_strides_that_the_copy_engine_can_read():
+    t = torch.zeros(6, 3, 64, dtype=torch.bfloat16)
+    assert P._strided(t) is t and P._strides(t) == (192, 64)
+    v = t.transpose(0, 1)
+    assert P._strided(v) is v
+    for bad in (t[:, :, ::2], t[:, :1].expand(6, 3, 64), t.view(-1)[:6 * 3 * 60].view(6, 3, 60)[:, :, :32]):
+        assert P._strided(bad).is_contiguous() and P._strided(bad) is not bad
+    one = torch.zeros(1, 1, 67, dtype=torch.bfloat16)[:, :, :64]
+    assert P._strides(one) == (64, 64)
+
+
+def test_argument_block_matches_the_header():
+    import re
+    from pathlib import Path
+    text = (Path(K.__file__).parent / "csrc" / "api.h").read_text()
+    body = re.sub(r"//[^\n]*", "", text[text.index("typedef struct ArbPacked"):text.index("} ArbPacked;")])
+    fields = [f for line in body[body.index("{") + 1:].split(";") for f in line.split(",") if f.strip()]
+    assert len(fields) == 31 and P._ARGS.size == 8 * len(fields)
+
+
+def test_backward_formula_against_differences():
+    """dS = P (dP - rowsum(dO o O)) and what follows from it, in 64 bits."""
+    g = torch.Generator().manual_seed(0)
+    q, k, v, w = (torch.randn(9, 4, generator=g, dtype=torch.float64) for _ in range(4))
+    i = torch.arange(9)
+    seen = (i[None] <= i[:, None]) & (i[None] >= i[:, None] - 5)
+    scale = 0.5
+
+    def f(q, k, v):
+        p = torch.softmax(torch.where(seen, q @ k.T * scale, -math.inf), 1)
+        return p, p @ v
+
+    p, o = f(q, k, v)
+    ds = p * (w @ v.T - (w * o).sum(1, keepdim=True))
+    grads = (scale * ds @ k, scale * ds.T @ q, p.T @ w)
+    for n, (x, dx) in enumerate(zip((q, k, v), grads)):
+        for idx in ((0, 0), (3, 2), (8, 3)):
+            e = torch.zeros_like(x)
+            e[idx] = 1e-5
+            hi, lo = ([t + e * s if m == n else t for m, t in enumerate((q, k, v))] for s in (1, -1))
+            diff = ((f(*hi)[1] - f(*lo)[1]) * w).sum() / 2e-5
+            assert abs(float(diff - dx[idx])) < 1e-7
