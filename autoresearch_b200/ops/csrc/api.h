@@ -19,6 +19,8 @@ enum ArbEpilogue {
                         // 2-CTA tiles, NT layout; parameters from arb_gemm_qkv_post_args
   EPI_SYM_STORE = 8,    // as EPI_STORE_BF16 / EPI_NS_COMBINE of a product that is symmetric (M = N, op(B) = op(A)^T, or A = A^T = B):
   EPI_SYM_NS_COMBINE = 9,  // above 768 a side the 2-CTA tiles below the diagonal are written as transposes
+  EPI_CE_STATS = 10,    // logits of a linear head: per tile and row their maximum and exponential sum, nothing else is written
+  EPI_CE_GRAD = 11,     // the gradient of its cross entropy with respect to the logits (bf16); both through arb_linear_ce_* only
 };
 
 enum ArbError {
@@ -99,6 +101,23 @@ int arb_gemm_bf16_ex(const void* A, const void* B, void* C, const void* aux, int
                      long long stride_c, int a_mn_major, int b_mn_major, int epi, int splitk, float alpha, float beta,
                      float gamma, int* err_flag, cudaStream_t stream, const void* pull_src, long long pull_bytes,
                      const void* ahead_src, void* ahead_dst, long long ahead_bytes);
+
+// ---- cross entropy of a linear head, without its logits in memory (gemm_sm100.cu) ------------------------------
+// s = softcap tanh(x w^T / softcap) (softcap 0: x w^T); loss[n] = log sum_v exp s[n, v] - s[n, target[n]].  A target outside of
+// [0, vocab) marks a row that does not count: loss 0, zero gradient.
+// fwd: all ids (cols = vocab, col0 = 0).  part: scratch of ceil(vocab / 256) x rows float pairs; lse: what the backward pass needs of a
+// row, log2 sum_v exp s.
+// grad: w holds the rows of the ids [col0, col0 + cols); d_logits[n, v] = weight[n] (softmax(s)[n, v] - [v = target]) ds/dx.
+typedef struct ArbLinearCE {
+  const void *x, *w, *targets;       // [rows, dim] bf16, [cols, dim] bf16, [rows] int32 or int64
+  float *part, *target_score, *lse, *loss;
+  const float* weight;
+  void* d_logits;                    // [rows, ldd] bf16
+  long long rows, cols, dim, vocab, col0, targets_64, ldx, ldw, ldd;
+  double softcap;
+} ArbLinearCE;
+int arb_linear_ce_fwd(const ArbLinearCE* a, int* err_flag, cudaStream_t stream);
+int arb_linear_ce_grad(const ArbLinearCE* a, int* err_flag, cudaStream_t stream);
 
 // ---- flash attention (attn_sm100.cu) ----------------------------------------------------------
 // q, k, v, o: [B, T, H, hd=128] bf16 with token stride `ld*` elements (head h at column

@@ -43,6 +43,18 @@ struct QkvPostArgs {
   float eps;
 };
 
+// EPI_CE_STATS / EPI_CE_GRAD: the logits of a linear head are used where they are computed and never written (see api.h)
+struct CeArgs {
+  const void* targets;          // [M] ids; outside of [0, vocabulary): the row does not count
+  int wide;                     // ids of 64 bits
+  int col0, vocab;              // id of the first column, number of ids
+  float cap;                    // soft cap, 0 = none
+  float2* part;                 // [n_tiles, M] maximum and sum of 2^(s - maximum) of a tile's row, s in units of log 2
+  float* target_score;          // [M]
+  const float* lse;             // [M]
+  const float* weight;          // [M] gradient of the row's loss
+};
+
 struct GemmArgs {
   int M, N, K, batch;
   int m_tiles, n_tiles, kb_total, kb_per_split, splitk;
@@ -77,6 +89,7 @@ struct GemmArgs {
   const int* k_valid;
   int k_seg_kb, k_nseg;
   QkvPostArgs qp;
+  CeArgs ce;
 };
 
 // The K blocks of [kb0, kb1) of batch item b that are multiplied, in order.  The bound of the current segment is read once
@@ -474,6 +487,43 @@ __device__ __forceinline__ void qkv_post_head(float (&f)[128], const QkvPostArgs
   }
 }
 
+// ---- cross entropy of a linear head -----------------------------------------------------------------------------------------
+// s = cap tanh(x / cap) = cap (1 - 2 r), r = 1 / (1 + e), e = exp(2 x / cap); ds/dx = 4 e r^2.  Two instructions of the special
+// function unit for the cap and one for the softmax; tanhf under fast math is one instruction with an error of 2^-11, 0.007 in a
+// logit at cap 15, which would go into the loss.  Scores, and what is kept of a row between the passes, are in units of log 2: a
+// probability is then one subtraction and one exponential away, without a rounding in between.
+constexpr float CE_LOG2E = 1.4426950408889634f, CE_LN2 = 0.6931471805599453f;
+// capped scores lie in [-cap, cap]: up to this cap 2^(s - cap) neither overflows nor vanishes in fp32 and no maximum is needed
+constexpr float CE_FIXED_MAX = 40.f;
+__device__ __forceinline__ float ce_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float ce_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+struct CeCap {
+  float k1, k2;                 // 2 log2(e) / cap, cap log2(e)
+  __device__ __forceinline__ explicit CeCap(float cap) : k1(cap > 0.f ? 2.f * CE_LOG2E / cap : 0.f), k2(cap * CE_LOG2E) {}
+  // e stays below 2^80, where r is zero to fp32 and e r still one
+  __device__ __forceinline__ float score(float x, float& e, float& r) const {
+    e = ce_ex2(fminf(x * k1, 80.f));
+    r = ce_rcp(1.f + e);
+    return fmaf(-2.f * k2, r, k2);
+  }
+};
+__device__ __forceinline__ long long ce_target(const CeArgs& c, int row) {
+  return c.wide ? reinterpret_cast<const long long*>(c.targets)[row] : (long long)reinterpret_cast<const int*>(c.targets)[row];
+}
+// column of the row's target relative to `col`, or -1 where it is not among the `n` columns from there
+__device__ __forceinline__ int ce_column(long long target, long long col, int n) {
+  const long long t = target - col;
+  return t >= 0 && t < n ? int(t) : -1;
+}
+
 // ------------------------------------------------------------------------------------------
 // 2-CTA variant: a cluster of two CTAs (one SM pair) owns a 256 x 256 tile.  Each CTA loads its
 // own 128 rows of A and 128 of the 256 rows of B (half the B traffic per SM of the 1-CTA kernel,
@@ -680,7 +730,59 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const int row = mt * 256 + int(rank) * 128 + q * 32 + lane;
       const bool row_ok = row < p.M;
       const long long row_off = (long long)b * p.stride_c + (long long)row * p.ldc;
-      if (!L::STAGED) {
+      if constexpr (EPI == EPI_CE_STATS) {
+        // a thread holds a row of the tile: running maximum and sum over its 256 scores, 32 at a time, the next 32 being fetched
+        const CeCap cap(p.ce.cap);
+        const bool capped = p.ce.cap > 0.f, fixed = capped && p.ce.cap <= CE_FIXED_MAX;
+        const long long target = row_ok ? ce_target(p.ce, row) : -1;
+        const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN2);
+        float mx = fixed ? cap.k2 : -INFINITY, sum = 0.f;
+        uint32_t v[2][32];
+        tmem_ld32(taddr, v[0]);
+#pragma unroll
+        for (int c = 0; c < BN2 / 32; ++c) {
+          uint32_t (&u)[32] = v[c & 1];
+          tmem_wait_ld();
+          if (c + 1 < BN2 / 32) tmem_ld32(taddr + uint32_t((c + 1) * 32), v[(c + 1) & 1]);
+          const int col = nt * BN2 + c * 32;
+          if (col >= p.N) continue;
+          float f[32];
+          if (capped) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) { float e, r; f[j] = cap.score(__uint_as_float(u[j]), e, r); }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(u[j]) * CE_LOG2E;
+          }
+          const int tc = ce_column(target, (long long)p.ce.col0 + col, min(32, p.N - col));
+          if (tc >= 0) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s = j == tc ? f[j] : s;
+            p.ce.target_score[row] = s;
+          }
+          if (col + 32 > p.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = col + j < p.N ? f[j] : -INFINITY;
+          }
+          if (!fixed) {
+            float a = mx, b2 = mx;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) { a = fmaxf(a, fmaxf(f[j], f[j + 1])); b2 = fmaxf(b2, fmaxf(f[j + 2], f[j + 3])); }
+            const float m = fmaxf(a, b2);
+            if (m > mx) { sum *= ce_ex2(mx - m); mx = m; }
+          }
+          const float off = mx == -INFINITY ? 0.f : mx;
+          float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            t0 += ce_ex2(f[j] - off); t1 += ce_ex2(f[j + 1] - off); t2 += ce_ex2(f[j + 2] - off); t3 += ce_ex2(f[j + 3] - off);
+          }
+          sum += (t0 + t1) + (t2 + t3);
+        }
+        tmem_wait_ld();
+        if (row_ok) p.ce.part[(long long)nt * p.M + row] = make_float2(mx, sum);
+      } else if (!L::STAGED) {
 #pragma unroll 1
         for (int c = 0; c < BN2 / 32; ++c) {
           uint32_t v[32];
@@ -694,6 +796,13 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const bool t0 = (threadIdx.x == 64);              // the thread that drives the TMA copies
         const int r_local = q * 32 + lane;
         const int row0 = mt * 256 + int(rank) * 128;
+        [[maybe_unused]] const CeCap cap(EPI == EPI_CE_GRAD ? p.ce.cap : 0.f);
+        [[maybe_unused]] long long target = -1;
+        [[maybe_unused]] float lse2 = INFINITY, weight = 0.f;
+        if (EPI == EPI_CE_GRAD && row_ok) {
+          target = ce_target(p.ce, row);
+          if (target >= 0 && target < p.ce.vocab) { lse2 = p.ce.lse[row]; weight = p.ce.weight[row]; }
+        }
         if (!epi_is_bf16(EPI)) {
           // fp32 output: eight slabs of 128 rows x 32 columns; accumulate-mode goes out as a TMA
           // reduce-add (full-line atomics at L2), store-mode as a TMA store
@@ -807,6 +916,25 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (EPI == EPI_RELU2) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) { const float r = fmaxf(f[j], 0.f); f[j] = r * r; }
+            }
+            if constexpr (EPI == EPI_CE_GRAD) {
+              // weight (softmax - [target]) ds/dx, rounded to bf16 as the operand of the two gradient products
+              const int tc = ce_column(target, (long long)p.ce.col0 + col_s + hc * 32, 32);
+              if (p.ce.cap > 0.f) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  float e, r;
+                  const float s = cap.score(f[j], e, r);
+                  const float pr = ce_ex2(s - lse2) - (j == tc ? 1.f : 0.f);
+                  f[j] = pr * (weight * (4.f * (e * r) * r));
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  const float pr = ce_ex2(fmaf(f[j], CE_LOG2E, -lse2)) - (j == tc ? 1.f : 0.f);
+                  f[j] = pr * weight;
+                }
+              }
             }
             if (L::AUX) {
 #pragma unroll
@@ -1113,7 +1241,7 @@ static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmA
   CUtensorMap tc, tx;
   std::memset(&tc, 0, sizeof tc);
   std::memset(&tx, 0, sizeof tx);
-  {
+  if (EPI != EPI_CE_STATS) {
     const uint64_t es = epi_is_bf16(EPI) ? 2 : 4;
     uint64_t dims[3] = {uint64_t(a.N), uint64_t(a.M), uint64_t(a.batch)};
     uint64_t str[2] = {uint64_t(a.ldc) * es, a.batch > 1 ? uint64_t(a.stride_c) * es : uint64_t(a.M) * uint64_t(a.ldc) * es};
@@ -1201,6 +1329,93 @@ extern "C" int arb_gemm_qkv_post_args(const void* cos_t, const void* sin_t, floa
   q.gate_w = (const __nv_bfloat16*)gate_w; q.gate = gate_out; q.gate_ch = gate_ch; q.eps = eps;
   g_qkv_post_set = true;
   return 0;
+}
+
+// loss[row] = log sum_v exp s - s[target] from the tiles' partial sums, in one fixed order: 8 threads per row, 32 rows per block
+__global__ void __launch_bounds__(256) ce_join_k(const float2* part, const float* target_score, CeArgs c, float* lse, float* loss, int rows,
+                                                 int tiles) {
+  __shared__ float2 sh[8][32];
+  grid_enter();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long row = (long long)blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  auto add = [&](float2 v) {
+    const float mm = fmaxf(m, v.x);
+    if (mm == -INFINITY) { s += v.y; return; }          // nothing but -inf so far; a NaN sum stays one
+    s = s * ce_ex2(m - mm) + v.y * ce_ex2(v.x - mm);
+    m = mm;
+  };
+  if (row < rows) {
+    int t = w;
+    for (; t + 24 < tiles; t += 32) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = part[(long long)(t + 8 * u) * rows + row];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) add(v[u]);
+    }
+    for (; t < tiles; t += 8) add(part[(long long)t * rows + row]);
+  }
+  sh[w][lane] = make_float2(m, s);
+  __syncthreads();
+  if (w == 0 && row < rows) {
+    for (int k = 1; k < 8; ++k) add(sh[k][lane]);
+    const float l = m + log2f(s);
+    lse[row] = l;
+    const long long target = ce_target(c, int(row));
+    loss[row] = target >= 0 && target < c.vocab ? (l - target_score[row]) * CE_LN2 : 0.f;
+  }
+}
+
+// operands and tiles of a product x [N, D] w [V, D]^T on 2-CTA tiles; 0 on success
+static int ce_operands(const ArbLinearCE* a, GemmArgs& g, CUtensorMap& ta, CUtensorMap& tb) {
+  if (!a || !a->x || !a->w || !a->targets || a->rows <= 0 || a->cols <= 0 || a->dim <= 0 || a->vocab <= 0 || a->col0 < 0) return -3;
+  if (a->rows > 0x7fffff00ll || a->vocab > 0x7fffff00ll || a->dim > 0x7fffff00ll || a->cols > a->vocab - a->col0) return -3;
+  if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->w)) & 15) return -4;
+  if ((a->ldx % 8) || (a->ldw % 8) || a->ldx < a->dim || a->ldw < a->dim) return -4;
+  if (!(a->softcap >= 0.0)) return -3;
+  if (g_num_sms == 0) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&g_num_sms, cudaDevAttrMultiProcessorCount, dev);
+  }
+  std::memset(&g, 0, sizeof g);
+  g.M = int(a->rows); g.N = int(a->cols); g.K = int(a->dim); g.batch = 1;
+  g.m_tiles = (g.M + 255) / 256; g.n_tiles = (g.N + 255) / 256;
+  if ((long long)g.m_tiles * g.n_tiles > 0x3fffffffll) return -3;
+  g.kb_total = g.kb_per_split = (g.K + BK - 1) / BK;
+  g.splitk = 1; g.b_div = 1; g.k_seg_kb = 1; g.k_nseg = 1;
+  g.ce.targets = a->targets; g.ce.wide = a->targets_64 ? 1 : 0; g.ce.col0 = int(a->col0); g.ce.vocab = int(a->vocab);
+  g.ce.cap = float(a->softcap);
+  const uint32_t box[3] = {BK, 128, 1};
+  uint64_t da[3] = {uint64_t(g.K), uint64_t(g.M), 1}, sa[2] = {uint64_t(a->ldx) * 2, uint64_t(a->ldx) * 2 * uint64_t(g.M)};
+  uint64_t db[3] = {uint64_t(g.K), uint64_t(g.N), 1}, sb[2] = {uint64_t(a->ldw) * 2, uint64_t(a->ldw) * 2 * uint64_t(g.N)};
+  if (int r = make_tmap_bf16(&ta, a->x, 3, da, sa, box)) return 1000 + r;
+  if (int r = make_tmap_bf16(&tb, a->w, 3, db, sb, box)) return 2000 + r;
+  return 0;
+}
+
+extern "C" int arb_linear_ce_fwd(const ArbLinearCE* a, int* err_flag, cudaStream_t stream) {
+  GemmArgs g;
+  CUtensorMap ta, tb;
+  if (int r = ce_operands(a, g, ta, tb)) return r;
+  if (!a->part || !a->target_score || !a->lse || !a->loss || a->cols != a->vocab) return -3;
+  g.err = err_flag;
+  g.ce.part = reinterpret_cast<float2*>(a->part); g.ce.target_score = a->target_score;
+  if (int r = launch_pair<false, false, EPI_CE_STATS>(ta, tb, g, stream)) return r;
+  return launch_dependent(true, ce_join_k, unsigned((g.M + 31) / 32), 256, 0, stream, g.ce.part, a->target_score, g.ce, a->lse, a->loss, g.M,
+                          g.n_tiles);
+}
+
+extern "C" int arb_linear_ce_grad(const ArbLinearCE* a, int* err_flag, cudaStream_t stream) {
+  GemmArgs g;
+  CUtensorMap ta, tb;
+  if (int r = ce_operands(a, g, ta, tb)) return r;
+  if (!a->lse || !a->weight || !a->d_logits || (reinterpret_cast<uintptr_t>(a->d_logits) & 15) || (a->ldd % 8) || a->ldd < a->cols) return -4;
+  g.err = err_flag;
+  g.ce.lse = a->lse; g.ce.weight = a->weight;
+  g.C = a->d_logits; g.ldc = a->ldd;
+  return launch_pair<false, false, EPI_CE_GRAD>(ta, tb, g, stream);
 }
 
 extern "C" int arb_gemm_dw_group(const void* const* dy, const void* const* x, float* const* c, const int* M, const int* N, int n, int K,
@@ -1342,6 +1557,7 @@ extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const
   a.k_seg_kb = k_valid ? k_seg_rows / BK : 1;
   a.k_nseg = k_valid ? K / k_seg_rows : 1;
   std::memset(&a.qp, 0, sizeof a.qp);
+  std::memset(&a.ce, 0, sizeof a.ce);
   if (epi == EPI_QKV_POST) {
     const bool have = g_qkv_post_set;
     g_qkv_post_set = false;

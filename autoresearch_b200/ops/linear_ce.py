@@ -1,0 +1,135 @@
+"""Cross entropy of a linear head over a vocabulary of any size, without its logits in memory (csrc/gemm_sm100.cu).
+
+    s = softcap tanh(x w^T / softcap)         (softcap 0: s = x w^T)
+    loss[n] = log sum_v exp s[n, v] - s[n, target[n]]
+
+The forward product hands out the maximum and the exponential sum of every row and tile of 256 ids, which one small kernel
+joins; no logit is written.  The backward pass multiplies again, a piece of the vocabulary at a time: the epilogue turns a
+piece of logits into d = g[n] (softmax(s) - [v = target]) ds/dx (bf16, at most ``PIECE_BYTES``), which the two gradient
+products dx += d w and dw = d^T x read.  What is kept between the passes is one fp32 number per row.
+
+Beside ``LMHeadCEFn`` (ops/sm100.py), which keeps whole rows of logits for a chunk of tokens and makes the gradients in its
+forward pass, this form returns per-token losses with any later weighting and needs no memory that grows with the vocabulary.
+"""
+from __future__ import annotations
+
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import kernels as K
+
+_ARGS = struct.Struct("=9q9qd")         # ArbLinearCE of csrc/api.h: 9 pointers, 9 sizes, the soft cap
+PIECE_BYTES = 1 << 29                   # bf16 gradient of a piece of logits
+TILE = 256
+
+
+def piece_columns(rows: int, vocab: int) -> int:
+    """Ids per piece of the backward pass: whole tiles, pieces of about the same size."""
+    most = max(TILE, PIECE_BYTES // (2 * max(rows, 1)) // TILE * TILE)
+    pieces = -(-vocab // most)
+    return -(-(-(-vocab // pieces)) // TILE) * TILE if pieces > 1 else vocab
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where the copy engine can read its rows, else a contiguous copy."""
+    if t.stride(1) == 1 and (t.shape[0] == 1 or (t.stride(0) >= t.shape[1] and not t.stride(0) & 7)) and not t.data_ptr() & 15:
+        return t
+    return t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _call(entry, x, w, targets, vocab, col0, softcap, part=0, target_score=0, lse=0, loss=0, weight=0, d_logits=None):
+    args = _ARGS.pack(x.data_ptr(), w.data_ptr(), targets.data_ptr(), part, target_score, lse, loss, weight,
+                      d_logits.data_ptr() if d_logits is not None else 0, x.shape[0], w.shape[0], x.shape[1], vocab, col0,
+                      int(targets.dtype is torch.int64), _ld(x), _ld(w), d_logits.stride(0) if d_logits is not None else 0, softcap)
+    K._check(getattr(K.lib(), entry)(args, K.err_flag(x.device).data_ptr(), K._stream()), entry)
+
+
+class LinearCEFn(torch.autograd.Function):
+    """Per-row losses [N] fp32.  A weight with a ``main_grad`` takes its gradient up there, as in the other products."""
+
+    @staticmethod
+    def forward(ctx, x, w, targets, softcap):
+        N, V = x.shape[0], w.shape[0]
+        loss = torch.empty(N, dtype=torch.float32, device=x.device)
+        lse = torch.empty(N, dtype=torch.float32, device=x.device)
+        xr, wr = _rows(x), _rows(w)
+        if N:
+            with K.on_device(x.device):
+                if K.pending_pulls:
+                    K.flush_pending_pulls()
+                tiles = -(-V // TILE)
+                scratch = torch.empty((2 * tiles + 1) * N, dtype=torch.float32, device=x.device)
+                part = scratch.data_ptr()
+                _call("arb_linear_ce_fwd", xr, wr, targets, V, 0, softcap, part, part + 8 * tiles * N, lse.data_ptr(), loss.data_ptr())
+                K.count_launch()                                     # the product and the join
+        ctx.save_for_backward(x, w, targets, lse)
+        ctx.softcap = softcap
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, targets, lse = ctx.saved_tensors
+        with K.on_device(x.device):
+            return (*_gradients(x, w, targets, lse, g.contiguous(), ctx.softcap, *ctx.needs_input_grad[:2]), None, None)
+
+
+def _gradients(x, w, targets, lse, g, softcap, need_x, need_w):
+    N, D = x.shape
+    V = w.shape[0]
+    dev = x.device
+    mg = getattr(w, "main_grad", None)
+    if not N:
+        return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w and mg is None else None)
+    if K.pending_pulls:
+        K.flush_pending_pulls()
+    xr, wr = _rows(x), _rows(w)
+    cols = piece_columns(N, V)
+    d = torch.empty(N, -(-cols // 8) * 8, dtype=torch.bfloat16, device=dev)
+    dx = torch.empty(N, D, dtype=torch.bfloat16, device=dev) if need_x else None
+    dw = torch.empty(V, D, dtype=torch.bfloat16, device=dev) if need_w and mg is None else None
+    # several pieces meet in fp32, in the order of the vocabulary
+    acc = torch.zeros(N, D, dtype=torch.float32, device=dev) if need_x and cols < V else None
+    for a in range(0, V, cols):
+        b = min(V, a + cols)
+        wp, dp = wr[a:b], d[:, :b - a]
+        _call("arb_linear_ce_grad", xr, wp, targets, V, a, softcap, lse=lse.data_ptr(), weight=g.data_ptr(), d_logits=d)
+        if acc is not None:
+            K.gemm(dp, wp, trans_b=False, out=acc, epi=K.EPI_ATOMIC_F32, splitk=1)
+        elif need_x:
+            K.gemm(dp, wp, trans_b=False, out=dx)
+        if need_w and mg is not None:
+            K.gemm(dp, xr, trans_a=True, trans_b=False, out=mg[a:b], epi=K.EPI_ATOMIC_F32)
+        elif need_w:
+            K.gemm(dp, xr, trans_a=True, trans_b=False, out=dw[a:b])
+    if acc is not None:
+        K.cast_f32_to_bf16(acc, dx)
+    return dx, dw
+
+
+def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, softcap: float = 0.0) -> torch.Tensor:
+    """Per-token losses [N] (fp32) of the head ``w`` [V, D] on ``x`` [N, D], both bf16, D a multiple of 8; differentiable in both.
+
+    ``targets`` [N], int32 or int64: a value outside of [0, V) marks a token that does not count (loss 0, no gradient).
+    ``softcap`` > 0: the logits are softcap * tanh(. / softcap).  Every row of ``x`` has to be finite, those that do not count
+    too: the gradient of ``w`` sums over all of them."""
+    K._bf16(x, "x")
+    K._bf16(w, "w")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x must be [N, D] and w [V, D], got {tuple(x.shape)} and {tuple(w.shape)}")
+    N, D = x.shape
+    if D < 8 or D % 8 or w.shape[0] < 1:
+        raise ValueError(f"D must be a positive multiple of 8 and w not empty, got {tuple(w.shape)}")
+    if targets.dtype not in (torch.int32, torch.int64) or targets.shape != (N,):
+        raise ValueError(f"targets must be int32 or int64 [{N}], got {targets.dtype} {tuple(targets.shape)}")
+    if w.device != x.device or targets.device != x.device:
+        raise ValueError("x, w and targets must be on one device")
+    if not 0.0 <= softcap < float("inf"):
+        raise ValueError(f"softcap must be finite and not negative, got {softcap}")
+    return LinearCEFn.apply(x, w, targets.contiguous(), float(softcap))
