@@ -119,6 +119,21 @@ typedef struct ArbLinearCE {
 int arb_linear_ce_fwd(const ArbLinearCE* a, int* err_flag, cudaStream_t stream);
 int arb_linear_ce_grad(const ArbLinearCE* a, int* err_flag, cudaStream_t stream);
 
+// ---- global gradient norm and clipping (clip.cu) --------------------------------------------------------------
+// Types: 0 fp32, 1 bf16, 2 fp16.  At most 1024 tensors a call; longer lists go in parts, each with `blocks` partial sums of its own.
+// squares: partial[0 .. blocks) = sums of squares that add up to the squared norm of these tensors.
+// scale: norm (may be null) = sqrt of the sum of all partials; max_norm >= 0: out = in * min(1, max_norm / norm), out = in left
+// alone where that is 1 or the norm is not finite (another out is then a copy); max_norm < 0: the norm alone.
+typedef struct ArbGrad {
+  const void* in;
+  void* out;
+  long long n;
+  int type, out_type;
+} ArbGrad;
+int arb_grad_squares(const ArbGrad* g, int n, double* partial, int blocks, cudaStream_t stream);
+int arb_grad_scale(const ArbGrad* g, int n, const double* partial, int partials, float max_norm, float* norm, int blocks,
+                   cudaStream_t stream);
+
 // ---- flash attention (attn_sm100.cu) ----------------------------------------------------------
 // q, k, v, o: [B, T, H, hd=128] bf16 with token stride `ld*` elements (head h at column
 // h*128); lse: [B, H, T] fp32.  window >= T means plain causal; key j is visible to query i

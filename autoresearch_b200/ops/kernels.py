@@ -73,6 +73,8 @@ def _signatures() -> dict:
         "arb_attn_bwd": [vp] * 11 + [i32, i32, i32] + [i64] * 8 + [i32, f32, vp, vp],
         "arb_linear_ce_fwd": [vp, vp, vp],
         "arb_linear_ce_grad": [vp, vp, vp],
+        "arb_grad_squares": [vp, i32, vp, i32, vp],
+        "arb_grad_scale": [vp, i32, vp, i32, f32, vp, i32, vp],
         "arb_packed_plan": [vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, vp],
         "arb_packed_attn_fwd": [vp, vp, vp],
         "arb_packed_attn_bwd": [vp, vp, vp],
