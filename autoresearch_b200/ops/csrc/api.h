@@ -107,17 +107,20 @@ int arb_gemm_bf16_ex(const void* A, const void* B, void* C, const void* aux, int
 // [0, vocab) marks a row that does not count: loss 0, zero gradient.
 // fwd: all ids (cols = vocab, col0 = 0).  part: scratch of ceil(vocab / 256) x rows float pairs; lse: what the backward pass needs of a
 // row, log2 sum_v exp s.
-// grad: w holds the rows of the ids [col0, col0 + cols); d_logits[n, v] = weight[n] (softmax(s)[n, v] - [v = target]) ds/dx.
+// bwd: `piece` ids at a time (a multiple of 256, or all), d_logits[n, v] = weight[n] (softmax(s)[n, v] - [v = target]) ds/dx in bf16
+// (scratch of rows x ldd), then dx (+)= d_logits w and dw = d_logits^T x.  dx: [rows, dim] bf16 or null; acc: fp32 scratch of its size
+// where there are several pieces.  dw: [vocab, dim] bf16, or main: fp32 rows ld_main apart that the gradient is added to, or both null.
 typedef struct ArbLinearCE {
   const void *x, *w, *targets;       // [rows, dim] bf16, [cols, dim] bf16, [rows] int32 or int64
   float *part, *target_score, *lse, *loss;
   const float* weight;
   void* d_logits;                    // [rows, ldd] bf16
-  long long rows, cols, dim, vocab, col0, targets_64, ldx, ldw, ldd;
+  long long rows, cols, dim, vocab, col0, targets_64, ldx, ldw, ldd;       // w: the rows of the ids [col0, col0 + cols)
   double softcap;
 } ArbLinearCE;
 int arb_linear_ce_fwd(const ArbLinearCE* a, int* err_flag, cudaStream_t stream);
-int arb_linear_ce_grad(const ArbLinearCE* a, int* err_flag, cudaStream_t stream);
+int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx, float* acc, void* dw, float* main, long long ld_main, int* err_flag,
+                      cudaStream_t stream);
 
 // ---- global gradient norm and clipping (clip.cu) --------------------------------------------------------------
 // Types: 0 fp32, 1 bf16, 2 fp16.  At most 1024 tensors a call; longer lists go in parts, each with `blocks` partial sums of its own.

@@ -1407,15 +1407,52 @@ extern "C" int arb_linear_ce_fwd(const ArbLinearCE* a, int* err_flag, cudaStream
                           g.n_tiles);
 }
 
-extern "C" int arb_linear_ce_grad(const ArbLinearCE* a, int* err_flag, cudaStream_t stream) {
+// the gradient of a piece of logits
+static int ce_grad(const ArbLinearCE& a, int* err_flag, cudaStream_t stream) {
   GemmArgs g;
   CUtensorMap ta, tb;
-  if (int r = ce_operands(a, g, ta, tb)) return r;
-  if (!a->lse || !a->weight || !a->d_logits || (reinterpret_cast<uintptr_t>(a->d_logits) & 15) || (a->ldd % 8) || a->ldd < a->cols) return -4;
+  if (int r = ce_operands(&a, g, ta, tb)) return r;
   g.err = err_flag;
-  g.ce.lse = a->lse; g.ce.weight = a->weight;
-  g.C = a->d_logits; g.ldc = a->ldd;
+  g.ce.lse = a.lse; g.ce.weight = a.weight;
+  g.C = a.d_logits; g.ldc = a.ldd;
   return launch_pair<false, false, EPI_CE_GRAD>(ta, tb, g, stream);
+}
+
+extern "C" int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx, float* acc, void* dw, float* main, long long ld_main,
+                                 int* err_flag, cudaStream_t stream) {
+  if (!a || a->col0 != 0 || a->cols != a->vocab || piece <= 0 || (piece < a->vocab && (piece % 256 || (dx && !acc)))) return -3;
+  if (!a->lse || !a->weight || !a->d_logits || (dw && main)) return -3;
+  if (((reinterpret_cast<uintptr_t>(a->d_logits) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(acc) |
+        reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(main)) & 15) || (a->ldd % 8) || a->ldd < (piece < a->vocab ? piece : a->vocab))
+    return -4;
+  if (main && ((ld_main % 4) || ld_main < a->dim)) return -4;
+  const int N = int(a->rows), D = int(a->dim);
+  const bool one = piece >= a->vocab;
+  for (long long c = 0; c < a->vocab; c += piece) {
+    ArbLinearCE b = *a;
+    b.w = reinterpret_cast<const __nv_bfloat16*>(a->w) + c * a->ldw;
+    b.col0 = c;
+    b.cols = piece < a->vocab - c ? piece : a->vocab - c;
+    if (int r = ce_grad(b, err_flag, stream)) return r;
+    if (dx) {
+      // several pieces meet in fp32, one after the other and without a split of the summed dimension: the same bits every time
+      const int epi = one ? EPI_STORE_BF16 : c == 0 ? EPI_STORE_F32 : EPI_ATOMIC_F32;
+      if (int r = arb_gemm_bf16(a->d_logits, b.w, one ? dx : acc, nullptr, N, D, int(b.cols), 1, a->ldd, a->ldw, D, 0, 0, 0, 0, 1, epi, 1, 0.f,
+                                0.f, 1.f, err_flag, stream))
+        return r;
+    }
+    if (main) {
+      if (int r = arb_gemm_bf16(a->d_logits, a->x, main + c * ld_main, nullptr, int(b.cols), D, N, 1, a->ldd, a->ldx, ld_main, 0, 0, 0, 1, 1,
+                                EPI_ATOMIC_F32, 0, 0.f, 0.f, 1.f, err_flag, stream))
+        return r;
+    } else if (dw) {
+      if (int r = arb_gemm_bf16(a->d_logits, a->x, reinterpret_cast<__nv_bfloat16*>(dw) + c * D, nullptr, int(b.cols), D, N, 1, a->ldd, a->ldx, D,
+                                0, 0, 0, 1, 1, EPI_STORE_BF16, 1, 0.f, 0.f, 1.f, err_flag, stream))
+        return r;
+    }
+  }
+  if (dx && !one) return arb_cast_f32_to_bf16(acc, dx, (long long)N * D, 1.f, stream);
+  return 0;
 }
 
 extern "C" int arb_gemm_dw_group(const void* const* dy, const void* const* x, float* const* c, const int* M, const int* N, int n, int K,

@@ -72,7 +72,7 @@ def _signatures() -> dict:
         "arb_attn_fwd": [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, i32, f32, vp, vp],
         "arb_attn_bwd": [vp] * 11 + [i32, i32, i32] + [i64] * 8 + [i32, f32, vp, vp],
         "arb_linear_ce_fwd": [vp, vp, vp],
-        "arb_linear_ce_grad": [vp, vp, vp],
+        "arb_linear_ce_bwd": [vp, i64, vp, vp, vp, vp, i64, vp, vp],
         "arb_grad_squares": [vp, i32, vp, i32, vp],
         "arb_grad_scale": [vp, i32, vp, i32, f32, vp, i32, vp],
         "arb_packed_plan": [vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, vp],
@@ -136,7 +136,8 @@ def available() -> bool:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # what torch.cuda.current_stream().cuda_stream says, without the Stream object (3.3 us -> 0.2 us a launch)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 _SAME_DEVICE = contextlib.nullcontext()
@@ -144,7 +145,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """Context in which ``device`` is the current one, so that a launch goes to that device and its current stream."""
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _SAME_DEVICE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def count_launch(n: int = 1) -> None:

@@ -36,18 +36,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself where the copy engine can read its rows, else a contiguous copy."""
     if t.stride(1) == 1 and (t.shape[0] == 1 or (t.stride(0) >= t.shape[1] and not t.stride(0) & 7)) and not t.data_ptr() & 15:
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _call(entry, x, w, targets, vocab, col0, softcap, part=0, target_score=0, lse=0, loss=0, weight=0, d_logits=None):
-    args = _ARGS.pack(x.data_ptr(), w.data_ptr(), targets.data_ptr(), part, target_score, lse, loss, weight,
-                      d_logits.data_ptr() if d_logits is not None else 0, x.shape[0], w.shape[0], x.shape[1], vocab, col0,
-                      int(targets.dtype is torch.int64), _ld(x), _ld(w), d_logits.stride(0) if d_logits is not None else 0, softcap)
-    K._check(getattr(K.lib(), entry)(args, K.err_flag(x.device).data_ptr(), K._stream()), entry)
+def _args(x, w, targets, softcap, part=0, target_score=0, lse=0, loss=0, weight=0, d_logits=0, ldd=0):
+    return _ARGS.pack(x.data_ptr(), w.data_ptr(), targets.data_ptr(), part, target_score, lse, loss, weight, d_logits, x.shape[0],
+                      w.shape[0], x.shape[1], w.shape[0], 0, int(targets.dtype is torch.int64), _ld(x), _ld(w), ldd, softcap)
 
 
 class LinearCEFn(torch.autograd.Function):
@@ -56,17 +54,18 @@ class LinearCEFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, softcap):
         N, V = x.shape[0], w.shape[0]
-        loss = torch.empty(N, dtype=torch.float32, device=x.device)
-        lse = torch.empty(N, dtype=torch.float32, device=x.device)
-        xr, wr = _rows(x), _rows(w)
+        loss = x.new_empty(N, dtype=torch.float32)
+        lse = x.new_empty(N, dtype=torch.float32)
         if N:
+            xr, wr = _rows(x), _rows(w)
             with K.on_device(x.device):
                 if K.pending_pulls:
                     K.flush_pending_pulls()
                 tiles = -(-V // TILE)
-                scratch = torch.empty((2 * tiles + 1) * N, dtype=torch.float32, device=x.device)
+                scratch = x.new_empty((2 * tiles + 1) * N, dtype=torch.float32)
                 part = scratch.data_ptr()
-                _call("arb_linear_ce_fwd", xr, wr, targets, V, 0, softcap, part, part + 8 * tiles * N, lse.data_ptr(), loss.data_ptr())
+                K._check(K.lib().arb_linear_ce_fwd(_args(xr, wr, targets, softcap, part, part + 8 * tiles * N, lse.data_ptr(), loss.data_ptr()),
+                                                   K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_fwd")
                 K.count_launch()                                     # the product and the join
         ctx.save_for_backward(x, w, targets, lse)
         ctx.softcap = softcap
@@ -81,35 +80,31 @@ class LinearCEFn(torch.autograd.Function):
 
 
 def _gradients(x, w, targets, lse, g, softcap, need_x, need_w):
+    """(dx, dw); dw is None where the main gradient of w has taken it up."""
     N, D = x.shape
     V = w.shape[0]
-    dev = x.device
-    mg = getattr(w, "main_grad", None)
+    main = getattr(w, "main_grad", None) if need_w else None
+    if main is not None and (main.dtype is not torch.float32 or main.shape != w.shape or main.device != w.device or main.stride(1) != 1
+                             or main.stride(0) % 4 or main.data_ptr() & 15):
+        raise ValueError(f"main_grad of a {tuple(w.shape)} weight must be fp32 of that shape with unit inner stride and 16-byte aligned rows")
     if not N:
-        return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w and mg is None else None)
+        return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w and main is None else None)
     if K.pending_pulls:
         K.flush_pending_pulls()
     xr, wr = _rows(x), _rows(w)
     cols = piece_columns(N, V)
-    d = torch.empty(N, -(-cols // 8) * 8, dtype=torch.bfloat16, device=dev)
-    dx = torch.empty(N, D, dtype=torch.bfloat16, device=dev) if need_x else None
-    dw = torch.empty(V, D, dtype=torch.bfloat16, device=dev) if need_w and mg is None else None
+    ldd = -(-cols // 8) * 8
+    d = x.new_empty(N * ldd)
+    dx = x.new_empty((N, D)) if need_x else None
+    dw = w.new_empty((V, D)) if need_w and main is None else None
     # several pieces meet in fp32, in the order of the vocabulary
-    acc = torch.zeros(N, D, dtype=torch.float32, device=dev) if need_x and cols < V else None
-    for a in range(0, V, cols):
-        b = min(V, a + cols)
-        wp, dp = wr[a:b], d[:, :b - a]
-        _call("arb_linear_ce_grad", xr, wp, targets, V, a, softcap, lse=lse.data_ptr(), weight=g.data_ptr(), d_logits=d)
-        if acc is not None:
-            K.gemm(dp, wp, trans_b=False, out=acc, epi=K.EPI_ATOMIC_F32, splitk=1)
-        elif need_x:
-            K.gemm(dp, wp, trans_b=False, out=dx)
-        if need_w and mg is not None:
-            K.gemm(dp, xr, trans_a=True, trans_b=False, out=mg[a:b], epi=K.EPI_ATOMIC_F32)
-        elif need_w:
-            K.gemm(dp, xr, trans_a=True, trans_b=False, out=dw[a:b])
-    if acc is not None:
-        K.cast_f32_to_bf16(acc, dx)
+    acc = x.new_empty((N, D), dtype=torch.float32) if need_x and cols < V else None
+    ptr = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
+    args = _args(xr, wr, targets, softcap, lse=lse.data_ptr(), weight=g.data_ptr(), d_logits=d.data_ptr(), ldd=ldd)
+    K._check(K.lib().arb_linear_ce_bwd(args, cols, ptr(dx), ptr(acc), ptr(dw), ptr(main), main.stride(0) if main is not None else 0,
+                                       K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_bwd")
+    pieces = -(-V // cols)
+    K.count_launch(pieces * (1 + need_x + need_w) - 1 + (acc is not None))
     return dx, dw
 
 

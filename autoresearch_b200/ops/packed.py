@@ -68,61 +68,61 @@ class PackedSequences:
         self.cap_q = rows // (128 // self.group) + self.n_seq + 2
         self.cap_k = rows // 128 + self.n_seq + 2
         self.device = cu_seqlens.device
+        self._err = K.err_flag(self.device)
         if (self.cap_q + self.cap_k) * n_kv_head >= 1 << 31:
             raise ValueError("too many tiles for one launch")
         items = 4 * (self.cap_q + self.cap_k)
         self.items = torch.empty(items + 4 * (self.n_seq + 3), dtype=torch.int32, device=self.device)
+        self._items_ptr, self._err_ptr = self.items.data_ptr(), self._err.data_ptr()
         if rows:
             span = max(128, L2_SPAN_BYTES // (512 * min(n_kv_head, 8)))
             with K.on_device(self.device):
                 K._check(K.lib().arb_packed_plan(self.cu_seqlens.data_ptr(), self.n_seq, rows, self.group, span, self.items.data_ptr(),
                                                  self.cap_q, self.cap_k, self.items.data_ptr() + 4 * items,
-                                                 K.err_flag(self.device).data_ptr(), K._stream()), "packed_plan")
+                                                 self._err.data_ptr(), K._stream()), "packed_plan")
 
 
-def _strided(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself where the kernels can read it: unit inner stride, the others positive multiples of 8 elements, 16-byte
-    aligned; else a contiguous copy."""
+def _layout(t: torch.Tensor):
+    """(tensor, row stride, head stride): ``t`` itself where the kernels can read it - unit inner stride, the others positive
+    multiples of 8 elements, 16-byte aligned - else a dense copy.  The stride of a dimension of size 1 is never used and
+    may be anything; it is given as that of dense storage."""
     s0, s1, s2 = t.stride()
-    n0, n1, _ = t.shape
-    if s2 == 1 and (n0 == 1 or (s0 > 0 and not s0 & 7)) and (n1 == 1 or (s1 > 0 and not s1 & 7)) and not t.data_ptr() & 15:
-        return t
-    return t.contiguous()
+    n0, n1, d = t.shape
+    if n1 == 1:
+        s1 = d
+    if n0 == 1:
+        s0 = n1 * d
+    if s2 == 1 and s0 > 0 and s1 > 0 and not (s0 | s1) & 7 and not t.data_ptr() & 15:
+        return t, s0, s1
+    return t.clone(memory_format=torch.contiguous_format), n1 * d, d
 
 
-def _strides(t: torch.Tensor):
-    """(row, head) stride; that of a dimension of size 1 is never used and may be anything."""
-    d = t.shape[2]
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * d), (t.stride(1) if t.shape[1] > 1 else d)
-
-
-def _call(entry: str, q, k, v, out, lse, seqs, window, scale, d_out=None, delta=None, dq=None, dk=None, dv=None) -> None:
-    strides = _strides(q) + _strides(k) + _strides(v) + (_strides(out)[0],)
-    if d_out is None:
-        ptrs, strides = (0, 0, 0, 0, 0), strides + (0, 0, 0, 0, 0)
-    else:
-        ptrs = (d_out.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
-        strides += _strides(d_out) + (_strides(dq)[0], _strides(dk)[0], _strides(dv)[0])
-    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *ptrs, seqs.items.data_ptr(),
-                      seqs.rows, seqs.n_kv_head, seqs.group, q.shape[2], window, seqs.cap_q, seqs.cap_k, *strides, scale)
-    with K.on_device(q.device):
-        K._check(getattr(K.lib(), entry)(args, K.err_flag(q.device).data_ptr(), K._stream()), entry)
-
-
-def _forward(q, k, v, seqs, window, scale):
+def _forward(q, k, v, strides, seqs, window, scale):
+    """(O, lse).  ``strides``: row and head stride of q, k and v."""
     rows, H, d = q.shape
-    out = torch.empty(rows, H, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(rows, H, dtype=torch.float32, device=q.device)
+    out = q.new_empty((rows, H, d))
+    lse = q.new_empty((rows, H), dtype=torch.float32)
     if rows:
-        _call("arb_packed_attn_fwd", q, k, v, out, lse, seqs, window, scale)
+        args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, seqs._items_ptr, rows,
+                          seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k, *strides, H * d, 0, 0, 0, 0, 0, scale)
+        with K.on_device(seqs.device):
+            K._check(K.lib().arb_packed_attn_fwd(args, seqs._err_ptr, K._stream()), "packed_attn_fwd")
     return out, lse
 
 
-def _backward(q, k, v, out, lse, d_out, dq, dk, dv, seqs, window, scale):
-    if q.shape[0]:
-        d_out = _strided(d_out)
-        _call("arb_packed_attn_bwd", q, k, v, out, lse, seqs, window, scale, d_out, torch.empty_like(lse), dq, dk, dv)
-        K.count_launch()                 # the row sums of dO o O and the gradient grid
+def _backward(q, k, v, out, lse, d_out, dq, dk, dv, strides, row_strides, seqs, window, scale):
+    """``row_strides``: those of dq, dk and dv, whose heads are d apart."""
+    rows, H, d = q.shape
+    if not rows:
+        return
+    d_out, do_row, do_head = _layout(d_out)
+    delta = lse.new_empty(lse.shape)
+    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), d_out.data_ptr(), delta.data_ptr(),
+                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), seqs._items_ptr, rows, seqs.n_kv_head, seqs.group, d, window,
+                      seqs.cap_q, seqs.cap_k, *strides, H * d, do_row, do_head, *row_strides, scale)
+    with K.on_device(seqs.device):
+        K._check(K.lib().arb_packed_attn_bwd(args, seqs._err_ptr, K._stream()), "packed_attn_bwd")
+    K.count_launch()                     # the row sums of dO o O and the gradient grid
 
 
 class PackedAttentionFn(torch.autograd.Function):
@@ -130,20 +130,22 @@ class PackedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, seqs, window, scale):
-        q, k, v = _strided(q), _strided(k), _strided(v)
-        out, lse = _forward(q, k, v, seqs, window, scale)
+        (q, q0, q1), (k, k0, k1), (v, v0, v1) = _layout(q), _layout(k), _layout(v)
+        strides = (q0, q1, k0, k1, v0, v1)
+        out, lse = _forward(q, k, v, strides, seqs, window, scale)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.args = (seqs, window, scale)
+        ctx.strides = strides
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
         q, k, v, out, lse = ctx.saved_tensors
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        _backward(q, k, v, out, lse, d_out, dq, dk, dv, *ctx.args)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
+        d = q.shape[2]
+        rows = (q.shape[1] * d, k.shape[1] * d, k.shape[1] * d)
+        _backward(q, k, v, out, lse, d_out, dq, dk, dv, ctx.strides, rows, *ctx.args)
         return dq, dk, dv, None, None, None
 
 
@@ -152,8 +154,9 @@ class PackedQKVAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, seqs, window, scale, d):
-        ctx.args, ctx.d = (seqs, window, scale), d
-        out, lse = _forward(*_blocks(qkv, seqs, d), seqs, window, scale)
+        ld = qkv.shape[1]
+        ctx.args, ctx.d, ctx.strides = (seqs, window, scale), d, (ld, d) * 3
+        out, lse = _forward(*_blocks(qkv, seqs, d), ctx.strides, seqs, window, scale)
         ctx.save_for_backward(qkv, out, lse)
         return out.view(qkv.shape[0], -1)
 
@@ -162,8 +165,9 @@ class PackedQKVAttentionFn(torch.autograd.Function):
     def backward(ctx, d_out):
         qkv, out, lse = ctx.saved_tensors
         seqs = ctx.args[0]
-        d_qkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _backward(*_blocks(qkv, seqs, ctx.d), out, lse, d_out.contiguous().view(out.shape), *_blocks(d_qkv, seqs, ctx.d), *ctx.args)
+        d_qkv = qkv.new_empty(qkv.shape)
+        _backward(*_blocks(qkv, seqs, ctx.d), out, lse, d_out.contiguous().view(out.shape), *_blocks(d_qkv, seqs, ctx.d), ctx.strides,
+                  (qkv.shape[1],) * 3, *ctx.args)
         return d_qkv, None, None, None, None
 
 
@@ -211,8 +215,8 @@ def packed_qkv_attention(qkv: torch.Tensor, seqs: PackedSequences, window: Optio
                          head_dim: int = 128) -> torch.Tensor:
     """The same on the contiguous packed projection output [rows, (H + 2 KV) head_dim] -> [rows, H head_dim]."""
     K._bf16(qkv, "qkv")
-    if qkv.dim() != 2 or not qkv.is_contiguous():
-        raise ValueError("qkv must be 2-D and contiguous")
+    if qkv.dim() != 2 or not qkv.is_contiguous() or qkv.data_ptr() & 15:
+        raise ValueError("qkv must be 2-D, contiguous and 16-byte aligned")
     rows = qkv.shape[0]
     window, scale = _common(qkv.device, rows, head_dim, seqs, window, scale)
     if qkv.shape[1] != (seqs.n_head + 2 * seqs.n_kv_head) * head_dim:

@@ -123,7 +123,7 @@ def test_strides():
     x, w, t, weight = _inputs(200, 64, 301)
     want = _run(x, w, t, weight, 0.0)
     forms = [torch.zeros(200, 136, dtype=x.dtype, device="cuda")[:, 8:72], torch.zeros(200, 67, dtype=x.dtype, device="cuda")[:, 1:65],
-             torch.zeros(64, 200, dtype=x.dtype, device="cuda").t()]
+             torch.zeros(64, 200, dtype=x.dtype, device="cuda").t(), torch.zeros(200 * 64 + 1, dtype=x.dtype, device="cuda")[1:].view(200, 64)]
     for f in forms:
         for p, q in zip(_run(f.copy_(x), w, t, weight, 0.0), want):
             assert torch.equal(p, q)

@@ -40,13 +40,17 @@ def test_cpu_tensors_are_refused():
 
 def test_strides_that_the_copy_engine_can_read():
     t = torch.zeros(6, 3, 64, dtype=torch.bfloat16)
-    assert P._strided(t) is t and P._strides(t) == (192, 64)
+    same, row, head = P._layout(t)
+    assert same is t and (row, head) == (192, 64)
     v = t.transpose(0, 1)
-    assert P._strided(v) is v
+    same, row, head = P._layout(v)
+    assert same is v and (row, head) == (64, 192)
     for bad in (t[:, :, ::2], t[:, :1].expand(6, 3, 64), t.view(-1)[:6 * 3 * 60].view(6, 3, 60)[:, :, :32]):
-        assert P._strided(bad).is_contiguous() and P._strided(bad) is not bad
+        dense, row, head = P._layout(bad)
+        assert dense.is_contiguous() and dense is not bad and (row, head) == (3 * bad.shape[2], bad.shape[2])
     one = torch.zeros(1, 1, 67, dtype=torch.bfloat16)[:, :, :64]
-    assert P._strides(one) == (64, 64)
+    same, row, head = P._layout(one)
+    assert same is one and (row, head) == (64, 64)
 
 
 def test_argument_block_matches_the_header():

@@ -206,6 +206,7 @@ def test_strides_and_alignment():
         buf = torch.empty(t.numel() + t.shape[0] * t.shape[1] + 1, dtype=t.dtype, device=t.device)
         return buf[1:1 + t.shape[0] * t.shape[1] * (d + 1)].view(t.shape[0], t.shape[1], d + 1)[..., :d].copy_(t)
     forms.append(tuple(odd(t) for t in (q, k, v, g)))
+    forms.append(tuple(torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape) for t in (q, k, v, g)))
     for f in forms:
         for x, y in zip(_run(*f, seqs), want):
             assert torch.equal(x, y)
