@@ -488,8 +488,7 @@ __device__ __forceinline__ void qkv_post_head(float (&f)[128], const QkvPostArgs
 }
 
 // ---- cross entropy of a linear head -----------------------------------------------------------------------------------------
-// s = cap tanh(x / cap) = cap (1 - 2 r), r = 1 / (1 + e), e = exp(2 x / cap); ds/dx = 4 e r^2.  Two instructions of the special
-// function unit for the cap and one for the softmax; tanhf under fast math is one instruction with an error of 2^-11, 0.007 in a
+// s = cap tanh(x / cap) = cap (1 - 2 r), r = 1 / (1 + e), e = exp(2 x / cap); ds/dx = 4 e r^2.  tanhf under fast math is one instruction with an error of 2^-11, 0.007 in a
 // logit at cap 15, which would go into the loss.  Scores, and what is kept of a row between the passes, are in units of log 2: a
 // probability is then one subtraction and one exponential away, without a rounding in between.
 constexpr float CE_LOG2E = 1.4426950408889634f, CE_LN2 = 0.6931471805599453f;
@@ -505,14 +504,30 @@ __device__ __forceinline__ float ce_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float ce_min(float x, float y) {      // a NaN stays one
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
 struct CeCap {
   float k1, k2;                 // 2 log2(e) / cap, cap log2(e)
   __device__ __forceinline__ explicit CeCap(float cap) : k1(cap > 0.f ? 2.f * CE_LOG2E / cap : 0.f), k2(cap * CE_LOG2E) {}
-  // e stays below 2^80, where r is zero to fp32 and e r still one
-  __device__ __forceinline__ float score(float x, float& e, float& r) const {
-    e = ce_ex2(fminf(x * k1, 80.f));
-    r = ce_rcp(1.f + e);
-    return fmaf(-2.f * k2, r, k2);
+  // r of four logits with one reciprocal of the product of their four denominators: products in place of three operations of the
+  // special function unit, which bounds these epilogues.  e stays below 2^30, where the score is the cap to fp32 and the product
+  // of four still has a normal reciprocal.
+  __device__ __forceinline__ void four(const uint32_t* u, unsigned long long& r01, unsigned long long& r23) const {
+    const unsigned long long kk = pk2(k1, k1), one = pk2(1.f, 1.f);
+    float x[4], p, q;
+    unpk2(mul2(pk2(__uint_as_float(u[0]), __uint_as_float(u[1])), kk), x[0], x[1]);
+    unpk2(mul2(pk2(__uint_as_float(u[2]), __uint_as_float(u[3])), kk), x[2], x[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = ce_ex2(ce_min(x[i], 30.f));
+    const unsigned long long a01 = add2(pk2(x[0], x[1]), one), a23 = add2(pk2(x[2], x[3]), one);
+    unpk2(mul2(a01, a23), p, q);                          // a0 a2, a1 a3
+    const float i4 = ce_rcp(p * q);
+    const unsigned long long i2 = pk2(i4 * q, i4 * p);    // 1 / (a0 a2), 1 / (a1 a3)
+    r01 = mul2(i2, a23);
+    r23 = mul2(i2, a01);
   }
 };
 __device__ __forceinline__ long long ce_target(const CeArgs& c, int row) {
@@ -540,10 +555,20 @@ __host__ __device__ constexpr bool epi_is_sym(int epi) { return epi == EPI_SYM_S
 // Work item -> output tile.  A symmetric product (Gram matrix, its square) computes the tiles on and above the diagonal only and
 // its epilogue also writes the transpose: 10 of 16 tiles at 1024, 36 of 64 at 2048.
 struct TileXY { int mt, nt, ks, b; };
-template <bool SYM>
+constexpr int CE_GROUP = 16;
+template <bool SYM, bool GROUPED = false>
 __host__ __device__ __forceinline__ TileXY tile_of(const GemmArgs& p, int w) {
   TileXY t;
-  if (SYM) {
+  if (GROUPED) {
+    // CE_GROUP rows of tiles together, column by column: the weight matrix of a large vocabulary outgrows L2, and row by row it would
+    // be read from HBM once for every 256 tokens (16384 x 1024 x 131072, forward: 4.88 ms row by row with four warps, 4.25 in groups
+    // of 8 and 3.79 in groups of 16 with eight; boxes under their power cap differ by 10 %)
+    const int per = CE_GROUP * p.n_tiles, g = w / per, i = w - g * per;
+    const int rows = p.m_tiles - g * CE_GROUP < CE_GROUP ? p.m_tiles - g * CE_GROUP : CE_GROUP;
+    t.nt = i / rows;
+    t.mt = g * CE_GROUP + i - t.nt * rows;
+    t.ks = t.b = 0;
+  } else if (SYM) {
     const int per = p.n_tiles * (p.n_tiles + 1) / 2;
     t.b = w / per;
     int i = w - t.b * per;
@@ -564,24 +589,31 @@ __host__ __device__ __forceinline__ int tile_count(const GemmArgs& p) {
   return SYM ? p.batch * (p.n_tiles * (p.n_tiles + 1) / 2) : p.batch * p.m_tiles * p.n_tiles * p.splitk;
 }
 
+// The cross-entropy epilogues do three to ten times the work of the others per element (exponentials, a reciprocal): eight warps
+// instead of four, each for half of a tile's columns, so that two of them share a scheduler and one computes while the other waits
+// (16384 x 512 x 65536 with a soft cap: forward 2.12 -> 1.13 ms, gradient 1.91 -> 1.29 ms, together with the packed arithmetic above).
+__host__ __device__ constexpr bool epi_is_ce(int epi) { return epi == EPI_CE_STATS || epi == EPI_CE_GRAD; }
+__host__ __device__ constexpr int pair_threads(int epi) { return epi_is_ce(epi) ? GEMM_THREADS + 128 : GEMM_THREADS; }
+
 // bf16 outputs leave through a swizzled smem staging slab (128 rows x 64 columns, double buffered)
 // and TMA stores, so every request to L2 is a full line; aux operands arrive the same way.
 template <int EPI>
 struct Smem2 {
   static constexpr bool STAGED = true;      // fp32 outputs are staged as 128 x 32 slabs (TMA store / reduce-add)
   static constexpr bool AUX = epi_has_aux(EPI);
-  static constexpr int STAGES = AUX ? 5 : 6;
+  static constexpr bool WIDE = EPI == EPI_CE_GRAD;                           // a pair of slabs for each of the two groups of warps
+  static constexpr int STAGES = AUX || WIDE ? 5 : 6;
   static constexpr int A_BYTES = 128 * BK * 2;
   static constexpr int B_BYTES = 128 * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int C_STAGE = STAGES * STAGE_BYTES;                       // 2 x 16 KB
   static constexpr int X_STAGE = C_STAGE + (STAGED ? 32768 : 0);             // 2 x 16 KB
-  static constexpr int BAR_OFFSET = X_STAGE + (AUX ? 32768 : 0);
+  static constexpr int BAR_OFFSET = X_STAGE + (AUX || WIDE ? 32768 : 0);
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
 };
 
 template <bool A_MN, bool B_MN, int EPI>
-__global__ void __launch_bounds__(GEMM_THREADS, 1)
+__global__ void __launch_bounds__(pair_threads(EPI), 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmX, const GemmArgs p) {
   using L = Smem2<EPI>;
@@ -604,11 +636,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const int cluster_id = blockIdx.x >> 1;
   const int n_clusters = gridDim.x >> 1;
   constexpr bool SYM = epi_is_sym(EPI);
+  constexpr int EPI_WARPS = epi_is_ce(EPI) ? 8 : 4;
   const int items = tile_count<SYM>(p);                            // m_tiles counted in 256-row tiles
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], 8); mbar_init(&xfull_bar[a], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], 2 * EPI_WARPS); mbar_init(&xfull_bar[a], 1); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -627,7 +660,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       uint32_t it = 0;
       bool ok = true;
       for (int w = cluster_id; w < items && ok; w += n_clusters) {
-        const TileXY tile = tile_of<SYM>(p, w);
+        const TileXY tile = tile_of<SYM, epi_is_ce(EPI)>(p, w);
         const int nt = tile.nt, mt = tile.mt, ks = tile.ks, b = tile.b;
         const int kb0 = ks * p.kb_per_split;
         const int kb1 = min(p.kb_total, kb0 + p.kb_per_split);
@@ -668,7 +701,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       uint32_t it = 0, tile_it = 0;
       bool ok = true;
       for (int w = cluster_id; w < items && ok; w += n_clusters) {
-        const TileXY tile = tile_of<SYM>(p, w);
+        const TileXY tile = tile_of<SYM, epi_is_ce(EPI)>(p, w);
         const int mt = tile.mt, ks = tile.ks, b = tile.b;
         const int kb0 = ks * p.kb_per_split;
         const int kb1 = min(p.kb_total, kb0 + p.kb_per_split);
@@ -711,10 +744,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     pull_ahead(p, lane);
   } else {
     const int q = warp & 3;
+    const int half = EPI_WARPS == 8 && warp > 6 ? 1 : 0;   // which half of the columns, with eight warps
     uint32_t tile_it = 0, slab_it = 0;
     bool ok = true;
     for (int w = cluster_id; w < items; w += n_clusters) {
-      const TileXY tile = tile_of<SYM>(p, w);
+      const TileXY tile = tile_of<SYM, epi_is_ce(EPI)>(p, w);
       const int nt = tile.nt, mt = tile.mt, ks = tile.ks, b = tile.b;
       {
         const int kb0 = ks * p.kb_per_split;
@@ -731,57 +765,84 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const bool row_ok = row < p.M;
       const long long row_off = (long long)b * p.stride_c + (long long)row * p.ldc;
       if constexpr (EPI == EPI_CE_STATS) {
-        // a thread holds a row of the tile: running maximum and sum over its 256 scores, 32 at a time, the next 32 being fetched
+        // a thread holds half a row of the tile: running maximum and sum over its 128 scores, 32 at a time while the next 32 are
+        // fetched; the two halves of a row meet in shared memory
         const CeCap cap(p.ce.cap);
         const bool capped = p.ce.cap > 0.f, fixed = capped && p.ce.cap <= CE_FIXED_MAX;
         const long long target = row_ok ? ce_target(p.ce, row) : -1;
-        const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN2);
+        const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(acc * BN2 + half * 128);
+        const int col_h = nt * BN2 + half * 128;
         float mx = fixed ? cap.k2 : -INFINITY, sum = 0.f;
-        uint32_t v[2][32];
-        tmem_ld32(taddr, v[0]);
-#pragma unroll
-        for (int c = 0; c < BN2 / 32; ++c) {
-          uint32_t (&u)[32] = v[c & 1];
-          tmem_wait_ld();
-          if (c + 1 < BN2 / 32) tmem_ld32(taddr + uint32_t((c + 1) * 32), v[(c + 1) & 1]);
-          const int col = nt * BN2 + c * 32;
-          if (col >= p.N) continue;
-          float f[32];
+        const unsigned long long m2k = pk2(-2.f * cap.k2, -2.f * cap.k2), add = fixed ? pk2(0.f, 0.f) : pk2(cap.k2, cap.k2);
+        const float unit = capped ? 1.f : CE_LOG2E;          // of z below
+        auto take = [&](const uint32_t (&u)[32], int col) {
+          if (col >= p.N) return;
+          float z[32];                                       // score minus the fixed maximum; score; logit
           if (capped) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) { float e, r; f[j] = cap.score(__uint_as_float(u[j]), e, r); }
+            for (int j = 0; j < 32; j += 4) {
+              unsigned long long r01, r23;
+              cap.four(&u[j], r01, r23);
+              unpk2(fma2(r01, m2k, add), z[j], z[j + 1]);
+              unpk2(fma2(r23, m2k, add), z[j + 2], z[j + 3]);
+            }
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(u[j]) * CE_LOG2E;
+            for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(u[j]);
           }
           const int tc = ce_column(target, (long long)p.ce.col0 + col, min(32, p.N - col));
           if (tc >= 0) {
             float s = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s = j == tc ? f[j] : s;
-            p.ce.target_score[row] = s;
+            for (int j = 0; j < 32; ++j) s = j == tc ? z[j] : s;
+            p.ce.target_score[row] = fixed ? s + cap.k2 : s * unit;
           }
           if (col + 32 > p.N) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = col + j < p.N ? f[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) z[j] = col + j < p.N ? z[j] : -INFINITY;
           }
           if (!fixed) {
-            float a = mx, b2 = mx;
+            float a = -INFINITY, b2 = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) { a = fmaxf(a, fmaxf(f[j], f[j + 1])); b2 = fmaxf(b2, fmaxf(f[j + 2], f[j + 3])); }
-            const float m = fmaxf(a, b2);
+            for (int j = 0; j < 32; j += 4) { a = fmaxf(a, fmaxf(z[j], z[j + 1])); b2 = fmaxf(b2, fmaxf(z[j + 2], z[j + 3])); }
+            const float m = fmaxf(a, b2) * unit;
             if (m > mx) { sum *= ce_ex2(mx - m); mx = m; }
+            const float off = mx == -INFINITY ? 0.f : mx;
+            const unsigned long long un = pk2(unit, unit), no = pk2(-off, -off);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) unpk2(fma2(pk2(z[j], z[j + 1]), un, no), z[j], z[j + 1]);
           }
-          const float off = mx == -INFINITY ? 0.f : mx;
-          float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
+          unsigned long long t0 = pk2(0.f, 0.f), t1 = t0;
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            t0 += ce_ex2(f[j] - off); t1 += ce_ex2(f[j + 1] - off); t2 += ce_ex2(f[j + 2] - off); t3 += ce_ex2(f[j + 3] - off);
+            t0 = add2(t0, pk2(ce_ex2(z[j]), ce_ex2(z[j + 1])));
+            t1 = add2(t1, pk2(ce_ex2(z[j + 2]), ce_ex2(z[j + 3])));
           }
-          sum += (t0 + t1) + (t2 + t3);
+          float lo, hi;
+          unpk2(add2(t0, t1), lo, hi);
+          sum += lo + hi;
+        };
+        uint32_t v0[32], v1[32];
+        tmem_ld32(taddr, v0);
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          tmem_wait_ld();
+          tmem_ld32(taddr + uint32_t(c + 32), v1);
+          take(v0, col_h + c);
+          tmem_wait_ld();
+          if (c == 0) tmem_ld32(taddr + 64u, v0);
+          take(v1, col_h + c + 32);
         }
-        tmem_wait_ld();
-        if (row_ok) p.ce.part[(long long)nt * p.M + row] = make_float2(mx, sum);
+        float2* meet = reinterpret_cast<float2*>(smem + L::C_STAGE) + (tile_it & 1) * 128 + q * 32 + lane;     // two tiles in turn
+        if (half) *meet = make_float2(mx, sum);
+        named_barrier(2, 256);
+        if (!half && row_ok) {
+          const float2 o = *meet;
+          const float m = fmaxf(mx, o.x);
+          if (m > -INFINITY) sum = sum * ce_ex2(mx - m) + o.y * ce_ex2(o.x - m);
+          else sum += o.y;
+          p.ce.part[(long long)nt * p.M + row] = make_float2(m, sum);
+        }
       } else if (!L::STAGED) {
 #pragma unroll 1
         for (int c = 0; c < BN2 / 32; ++c) {
@@ -793,7 +854,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           epilogue_chunk<EPI>(v, p, row, row_off, col0);
         }
       } else {
-        const bool t0 = (threadIdx.x == 64);              // the thread that drives the TMA copies
+        const bool t0 = (threadIdx.x == (half ? 224 : 64));      // the thread that drives the TMA copies (of its half)
         const int r_local = q * 32 + lane;
         const int row0 = mt * 256 + int(rank) * 128;
         [[maybe_unused]] const CeCap cap(EPI == EPI_CE_GRAD ? p.ce.cap : 0.f);
@@ -877,24 +938,25 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           }
         } else {
 #pragma unroll 1
-        for (int sl = 0; sl < (epi_is_bf16(EPI) ? 4 : 0); ++sl, ++slab_it) {
+        for (int sl = 2 * half; sl < (!epi_is_bf16(EPI) ? 0 : EPI_WARPS == 8 ? 2 * half + 2 : 4); ++sl, ++slab_it) {
           const int buf = slab_it & 1;
           const int col_s = nt * BN2 + sl * 64;
+          uint8_t* stage = smem + L::C_STAGE + half * 32768 + buf * 16384;
           if (t0) tma_store_wait_read_1();                // the store issued two slabs ago has read its buffer
-          named_barrier(2, 128);
+          named_barrier(2 + 2 * half, 128);
           if (L::AUX) {
             if (t0) {                                      // prefetch the next aux slab (this tile or the next one)
               int nsl = sl + 1, nw = w;
               if (nsl == 4) {                              // the next item of this cluster that is not skipped
                 nsl = 0;
                 for (nw = w + n_clusters; nw < items; nw += n_clusters) {
-                  const TileXY nx = tile_of<SYM>(p, nw);
+                  const TileXY nx = tile_of<SYM, epi_is_ce(EPI)>(p, nw);
                   const int nkb0 = nx.ks * p.kb_per_split;
                   if (item_live(p, nx.b, nx.mt * 256, nkb0, min(p.kb_total, nkb0 + p.kb_per_split))) break;
                 }
               }
               if (nw < items) {
-                const TileXY nx = tile_of<SYM>(p, nw);
+                const TileXY nx = tile_of<SYM, epi_is_ce(EPI)>(p, nw);
                 const int nnt = nx.nt, nmt = nx.mt, nb = nx.b;
                 mbar_expect_tx(&xfull_bar[buf ^ 1], 16384);
                 tma_load_3d(smem + L::X_STAGE + (buf ^ 1) * 16384, &tmX, &xfull_bar[buf ^ 1], nnt * BN2 + nsl * 64,
@@ -903,7 +965,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
             if (!mbar_wait(&xfull_bar[buf], (slab_it >> 1) & 1, abort_flag)) { ok = false; }
           }
-          const uint32_t cbase = smem_u32(smem + L::C_STAGE + buf * 16384);
+          const uint32_t cbase = smem_u32(stage);
           const uint32_t xbase = smem_u32(smem + L::X_STAGE + buf * 16384);
 #pragma unroll
           for (int hc = 0; hc < 2; ++hc) {
@@ -918,22 +980,44 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               for (int j = 0; j < 32; ++j) { const float r = fmaxf(f[j], 0.f); f[j] = r * r; }
             }
             if constexpr (EPI == EPI_CE_GRAD) {
-              // weight (softmax - [target]) ds/dx, rounded to bf16 as the operand of the two gradient products
-              const int tc = ce_column(target, (long long)p.ce.col0 + col_s + hc * 32, 32);
+              // weight (softmax - [target]) ds/dx, rounded to bf16 as the operand of the two gradient products;
+              // ds/dx = 4 e r^2 = 4 (r - r^2)
               if (p.ce.cap > 0.f) {
+                const unsigned long long m2k = pk2(-2.f * cap.k2, -2.f * cap.k2), off = pk2(cap.k2 - lse2, cap.k2 - lse2);
+                const unsigned long long w4 = pk2(4.f * weight, 4.f * weight), neg = pk2(-1.f, -1.f);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  float e, r;
-                  const float s = cap.score(f[j], e, r);
-                  const float pr = ce_ex2(s - lse2) - (j == tc ? 1.f : 0.f);
-                  f[j] = pr * (weight * (4.f * (e * r) * r));
+                for (int j = 0; j < 32; j += 4) {
+                  unsigned long long r[2];
+                  cap.four(&v[j], r[0], r[1]);
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    float s0, s1;
+                    unpk2(fma2(r[i], m2k, off), s0, s1);
+                    const unsigned long long slope = fma2(mul2(r[i], neg), r[i], r[i]);
+                    unpk2(mul2(mul2(pk2(ce_ex2(s0), ce_ex2(s1)), w4), slope), f[j + 2 * i], f[j + 2 * i + 1]);
+                  }
                 }
               } else {
+                const unsigned long long un = pk2(CE_LOG2E, CE_LOG2E), off = pk2(-lse2, -lse2), wt = pk2(weight, weight);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  const float pr = ce_ex2(fmaf(f[j], CE_LOG2E, -lse2)) - (j == tc ? 1.f : 0.f);
-                  f[j] = pr * weight;
+                for (int j = 0; j < 32; j += 2) {
+                  float s0, s1;
+                  unpk2(fma2(pk2(f[j], f[j + 1]), un, off), s0, s1);
+                  unpk2(mul2(pk2(ce_ex2(s0), ce_ex2(s1)), wt), f[j], f[j + 1]);
                 }
+              }
+              const int tc = ce_column(target, (long long)p.ce.col0 + col_s + hc * 32, 32);
+              if (tc >= 0) {                              // one in V / 32 times the rows of a warp
+                float x = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x = j == tc ? __uint_as_float(v[j]) : x;
+                float one = weight;
+                if (p.ce.cap > 0.f) {
+                  const float r = ce_rcp(1.f + ce_ex2(ce_min(x * cap.k1, 30.f)));
+                  one *= 4.f * fmaf(-r, r, r);
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[j] -= j == tc ? one : 0.f;
               }
             }
             if (L::AUX) {
@@ -974,9 +1058,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
           fence_proxy_async_smem();
-          named_barrier(3, 128);
+          named_barrier(3 + 2 * half, 128);
           if (t0 && col_s < p.N && row0 < p.M) {
-            tma_store_3d(&tmC, smem + L::C_STAGE + buf * 16384, col_s, row0, b);
+            tma_store_3d(&tmC, stage, col_s, row0, b);
             tma_store_commit();
           } else if (t0) {
             tma_store_commit();                           // keep the group count in step with the slab count
@@ -991,7 +1075,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         else mbar_arrive_remote(mapa_u32(smem_u32(&tempty_bar[acc]), 0));
       }
     }
-    if (L::STAGED && threadIdx.x == 64) tma_store_wait_all();   // staged tiles are on their way before smem goes away
+    if (L::STAGED && (threadIdx.x == 64 || (EPI_WARPS == 8 && threadIdx.x == 224))) tma_store_wait_all();   // staged tiles are on their way before smem goes away
   }
 
   tc_fence_before();
@@ -1219,9 +1303,10 @@ static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmArgs& 
   return launch_dependent(true, kern, grid, GEMM_THREADS, L::TOTAL, st, ta, tb, args);
 }
 
-static void pair_launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int clusters, int smem, cudaStream_t st) {
+static void pair_launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int clusters, int smem, cudaStream_t st,
+                               int threads = GEMM_THREADS) {
   cfg.gridDim = dim3(unsigned(clusters * 2));
-  cfg.blockDim = dim3(GEMM_THREADS);
+  cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1263,7 +1348,7 @@ static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmA
   if (items < clusters) clusters = items;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  pair_launch_config(cfg, attr, clusters, Smem2<EPI>::TOTAL, st);
+  pair_launch_config(cfg, attr, clusters, Smem2<EPI>::TOTAL, st, pair_threads(EPI));
   GemmArgs args = a;
   if (int r = arm_pull(args, clusters * 2)) return r;
   return launch_status(cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, tx, args));

@@ -210,3 +210,16 @@ def test_no_tokens():
     x, w, t, weight = _inputs(0, 64, 300)
     loss, dx, dw = _run(x, w, t, weight, 0.0)
     assert loss.shape == (0,) and dx.shape == (0, 64) and bool((dw == 0).all())
+
+
+@pytest.mark.parametrize("cap", [0.0, 15.0, 50.0])
+def test_values_that_are_not_finite_show_in_their_row_and_in_no_other(cap):
+    from autoresearch_b200.ops.linear_ce import linear_cross_entropy
+    x, w, t, weight = _inputs(300, 64, 1000)
+    want = linear_cross_entropy(x, w, t, softcap=cap)
+    x[7, 3], x[131, 0] = float("nan"), float("inf")
+    got = linear_cross_entropy(x, w, t, softcap=cap)
+    assert bool(torch.isnan(got[7]))
+    assert not bool(torch.isfinite(got[131])) or cap > 0          # a capped logit of an infinity is the cap
+    rest = [i for i in range(300) if i not in (7, 131)]
+    assert torch.equal(got[rest], want[rest])
