@@ -3,8 +3,10 @@
 //   norm = sqrt(sum over all tensors and elements g^2);   out = g * min(1, max_norm / norm)
 //
 // Two launches, both bound by memory: one pass that leaves a sum per block, one that joins them (every block by itself, in one
-// fixed order) and scales.  The list travels as a kernel argument, so nothing is copied to the device and a captured graph
-// holds it.  Work items are 8192 elements of one tensor.
+// fixed order) and scales, from the last item to the first: what the first pass read last is still in L2.  The list travels as
+// a kernel argument, so nothing is copied to the device and a captured graph holds it.  Work items are 16384 elements of one
+// tensor; a thread has four loads of 16 bytes in flight and few enough registers for five blocks an SM (with all of an item's
+// loads in flight at once, 120 and 242 registers a thread: 2.9 TB/s).
 //
 // Sums: a thread squares and adds up to 32 elements in fp32, then adds to a 64-bit sum.  Where the 32 leave the range in which
 // fp32 squares are exact enough (elements around 1e-15 and below or 1e15 and above), they are squared again in 64 bits, from
@@ -17,7 +19,7 @@
 namespace arb {
 
 constexpr int CLIP_THREADS = 256;
-constexpr int CLIP_ITEM = 8192;                  // elements: 32 per thread
+constexpr int CLIP_ITEM = 16384;                 // elements: 64 per thread
 constexpr int CLIP_SMALL = 128, CLIP_LARGE = 1024;
 
 template <int CAP>
@@ -61,11 +63,11 @@ __device__ __forceinline__ float narrow(double x) {
 template <typename T, int W>
 struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Vec { T v[W]; };
 
-// elements from `p` on that one access may take, up to 8
+// elements from `p` on that one access of at most 16 bytes may take
 template <typename T>
 __device__ __forceinline__ int grad_width(const void* p) {
   const unsigned a = unsigned(reinterpret_cast<uintptr_t>(p));
-  if ((a & 15u) == 0) return 8;
+  if (sizeof(T) == 2 && (a & 15u) == 0) return 8;
   if ((a & (4u * sizeof(T) - 1)) == 0) return 4;
   return (a & (2u * sizeof(T) - 1)) == 0 ? 2 : 1;
 }
@@ -93,24 +95,12 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
   return v;
 }
 
-// sum of squares of the thread's share of `n` <= CLIP_ITEM elements
-template <typename T, int W>
-__device__ __forceinline__ double item_squares(const T* p, int n) {
-  constexpr int STEPS = CLIP_ITEM / CLIP_THREADS / W;
-  Vec<T, W> v[STEPS];
-#pragma unroll
-  for (int k = 0; k < STEPS; ++k) {
-    const int i = (k * CLIP_THREADS + int(threadIdx.x)) * W;
-    if (i + W <= n) {
-      v[k] = *reinterpret_cast<const Vec<T, W>*>(p + i);
-    } else {
-#pragma unroll
-      for (int e = 0; e < W; ++e) { if (i + e < n) v[k].v[e] = p[i + e]; else from_f32(0.f, v[k].v[e]); }
-    }
-  }
+// squares of N values, in 64 bits where fp32 would lose them
+template <int N, typename T, int W>
+__device__ __forceinline__ double batch_squares(const Vec<T, W> (&v)[N]) {
   float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < STEPS; ++k)
+  for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       const float x = to_f32(v[k].v[e]);
@@ -121,7 +111,7 @@ __device__ __forceinline__ double item_squares(const T* p, int n) {
   if (sum > 1e-28f && sum < 1e30f) return double(sum);
   double d = 0.0;
 #pragma unroll
-  for (int k = 0; k < STEPS; ++k)
+  for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       const double x = widen(to_f32(v[k].v[e]));
@@ -130,11 +120,33 @@ __device__ __forceinline__ double item_squares(const T* p, int n) {
   return d;
 }
 
+// sum of squares of the thread's share of `n` <= CLIP_ITEM elements: four accesses at a time, then what is left one by one
+template <typename T, int W>
+__device__ __forceinline__ double item_squares(const T* p, int n) {
+  double acc = 0.0;
+  constexpr int STEP = CLIP_THREADS * W * 4;
+  int at = 0;
+#pragma unroll 1
+  for (; at + STEP <= n; at += STEP) {
+    Vec<T, W> v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const Vec<T, W>*>(p + at + (k * CLIP_THREADS + int(threadIdx.x)) * W);
+    acc += batch_squares<4>(v);
+  }
+#pragma unroll 1
+  for (int i = at + int(threadIdx.x); i < n; i += CLIP_THREADS) {
+    Vec<T, 1> v[1];
+    v[0].v[0] = p[i];
+    acc += batch_squares<1>(v);
+  }
+  return acc;
+}
+
 template <typename T>
 __device__ __forceinline__ double tensor_squares(const void* p, long long from, int n) {
   const T* q = reinterpret_cast<const T*>(p) + from;
   switch (grad_width<T>(q)) {
-    case 8: return item_squares<T, 8>(q, n);
+    case 8: if constexpr (sizeof(T) == 2) return item_squares<T, 8>(q, n);
     case 4: return item_squares<T, 4>(q, n);
     case 2: return item_squares<T, 2>(q, n);
     default: return item_squares<T, 1>(q, n);
@@ -142,7 +154,7 @@ __device__ __forceinline__ double tensor_squares(const void* p, long long from, 
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(CLIP_THREADS) grad_squares_k(const __grid_constant__ GradTable<CAP> t, double* partial) {
+__global__ void __launch_bounds__(CLIP_THREADS, 5) grad_squares_k(const __grid_constant__ GradTable<CAP> t, double* partial) {
   __shared__ double sh[CLIP_THREADS / 32];
   grid_enter();
   double acc = 0.0;
@@ -162,31 +174,23 @@ __global__ void __launch_bounds__(CLIP_THREADS) grad_squares_k(const __grid_cons
 
 template <typename TI, typename TO, int W>
 __device__ __forceinline__ void item_scale(const TI* p, TO* q, int n, float c) {
-  constexpr int STEPS = CLIP_ITEM / CLIP_THREADS / W;
-  Vec<TI, W> v[STEPS];
+  constexpr int STEP = CLIP_THREADS * W * 4;
+  int at = 0;
+#pragma unroll 1
+  for (; at + STEP <= n; at += STEP) {
+    Vec<TI, W> v[4];
 #pragma unroll
-  for (int k = 0; k < STEPS; ++k) {
-    const int i = (k * CLIP_THREADS + int(threadIdx.x)) * W;
-    if (i + W <= n) {
-      v[k] = *reinterpret_cast<const Vec<TI, W>*>(p + i);
-    } else {
+    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const Vec<TI, W>*>(p + at + (k * CLIP_THREADS + int(threadIdx.x)) * W);
 #pragma unroll
-      for (int e = 0; e < W; ++e) { if (i + e < n) v[k].v[e] = p[i + e]; else from_f32(0.f, v[k].v[e]); }
+    for (int k = 0; k < 4; ++k) {
+      Vec<TO, W> o;
+#pragma unroll
+      for (int e = 0; e < W; ++e) from_f32(to_f32(v[k].v[e]) * c, o.v[e]);
+      *reinterpret_cast<Vec<TO, W>*>(q + at + (k * CLIP_THREADS + int(threadIdx.x)) * W) = o;
     }
   }
-#pragma unroll
-  for (int k = 0; k < STEPS; ++k) {
-    const int i = (k * CLIP_THREADS + int(threadIdx.x)) * W;
-    Vec<TO, W> o;
-#pragma unroll
-    for (int e = 0; e < W; ++e) from_f32(to_f32(v[k].v[e]) * c, o.v[e]);
-    if (i + W <= n) {
-      *reinterpret_cast<Vec<TO, W>*>(q + i) = o;
-    } else {
-#pragma unroll
-      for (int e = 0; e < W; ++e) if (i + e < n) q[i + e] = o.v[e];
-    }
-  }
+#pragma unroll 1
+  for (int i = at + int(threadIdx.x); i < n; i += CLIP_THREADS) from_f32(to_f32(p[i]) * c, q[i]);
 }
 
 template <typename TI, typename TO>
@@ -194,7 +198,7 @@ __device__ __forceinline__ void tensor_scale(const void* in, void* out, long lon
   const TI* p = reinterpret_cast<const TI*>(in) + from;
   TO* q = reinterpret_cast<TO*>(out) + from;
   switch (min(grad_width<TI>(p), grad_width<TO>(q))) {
-    case 8: item_scale<TI, TO, 8>(p, q, n, c); break;
+    case 8: if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) { item_scale<TI, TO, 8>(p, q, n, c); break; }
     case 4: item_scale<TI, TO, 4>(p, q, n, c); break;
     case 2: item_scale<TI, TO, 2>(p, q, n, c); break;
     default: item_scale<TI, TO, 1>(p, q, n, c); break;
@@ -211,7 +215,7 @@ __device__ __forceinline__ void tensor_scale_to(int to, const void* in, void* ou
 
 // max_norm < 0: the norm alone.  A norm that is not finite scales nothing.
 template <int CAP>
-__global__ void __launch_bounds__(CLIP_THREADS) grad_scale_k(const __grid_constant__ GradTable<CAP> t, const double* partial, int partials,
+__global__ void __launch_bounds__(CLIP_THREADS, 5) grad_scale_k(const __grid_constant__ GradTable<CAP> t, const double* partial, int partials,
                                                              double max_norm, float* norm_out) {
   __shared__ double sh[CLIP_THREADS / 32];
   grid_enter();
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(CLIP_THREADS) grad_scale_k(const __grid_consta
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) *norm_out = narrow(norm);
   if (max_norm < 0.f) return;
   const float c = norm > double(max_norm) && norm <= 1.7976931348623157e308 ? float(double(max_norm) / norm) : 1.f;
-  for (int i = blockIdx.x; i < t.first[t.count]; i += gridDim.x) {
+  for (int i = t.first[t.count] - 1 - int(blockIdx.x); i >= 0; i -= gridDim.x) {
     const int k = grad_tensor(t, i);
     if (c == 1.f && t.out[k] == t.in[k]) continue;          // in place and nothing to do
     const long long from = (long long)(i - t.first[k]) * CLIP_ITEM, left = t.n[k] - from;

@@ -20,7 +20,8 @@ from ..ops import kernels as K
 _ENTRY = struct.Struct("=3q2i")         # ArbGrad of csrc/api.h
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_TENSORS = 1024                      # per launch
-BLOCKS_PER_SM = 6
+BLOCKS_PER_SM = 5
+ITEM = 16384                            # elements of a work item
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -79,7 +80,7 @@ class GradSet:
         if rows:
             most = torch.cuda.get_device_properties(self.device).multi_processor_count * BLOCKS_PER_SM
             for a in range(0, len(rows), MAX_TENSORS):
-                items = sum(-(-t.numel() // 8192) for t, _ in live[a:a + MAX_TENSORS])
+                items = sum(-(-t.numel() // ITEM) for t, _ in live[a:a + MAX_TENSORS])
                 self._parts.append((b"".join(rows[a:a + MAX_TENSORS]), len(rows[a:a + MAX_TENSORS]), min(items, most)))
 
     def _run(self, max_norm: float) -> torch.Tensor:

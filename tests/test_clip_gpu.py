@@ -9,7 +9,7 @@ import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
-SIZES = [(1,), (7, 3), (8192,), (8193,), (8191, 1), (100, 333), (5, 0), (30,), (1 << 18,), (3,), (123457,), ()]
+SIZES = [(1,), (7, 3), (8192,), (8193,), (8191, 1), (16384,), (16385,), (49151,), (100, 333), (5, 0), (30,), (1 << 18,), (3,), (123457,), ()]
 
 
 def _grads(sizes, dtype, seed=0, scale=1e-2, back_to_back=False):
@@ -116,10 +116,10 @@ def test_neighbours_in_memory_stay_as_they_were():
     from autoresearch_b200.optim.clip import clip_grad_norm
     for dtype in (torch.float32, torch.bfloat16):
         for offset in range(1, 9):
-            buf = torch.full((8192 + 64,), 5.0, dtype=dtype, device="cuda")
-            clip_grad_norm([buf[offset:offset + 8192 + 13]], 1.0)
-            assert bool((buf[:offset] == 5).all()) and bool((buf[offset + 8192 + 13:] == 5).all())
-            assert bool((buf[offset:offset + 8192 + 13] < 1).all())
+            buf = torch.full((16384 + 64,), 5.0, dtype=dtype, device="cuda")
+            clip_grad_norm([buf[offset:offset + 16384 + 13]], 1.0)
+            assert bool((buf[:offset] == 5).all()) and bool((buf[offset + 16384 + 13:] == 5).all())
+            assert bool((buf[offset:offset + 16384 + 13] < 1).all())
 
 
 def test_memory_orders():
