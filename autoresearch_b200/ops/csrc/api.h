@@ -162,10 +162,10 @@ int arb_attn_bwd(const void* q, const void* k, const void* v, const void* o, con
 // together stay in L2.
 typedef struct ArbPacked {
   const void *q, *k, *v;
-  void* o;
+  void *o, *o_lo;                    // o_lo: what rounding left over of o, which the backward pass reads; null where none follows
   float* lse;
   const void* d_o;                   // backward, as everything down to dv
-  float* delta;                      // scratch
+  float* delta;                      // scratch of rows x KV x G + 2 words
   void *dq, *dk, *dv;
   const void* items;
   long long rows, KV, G, D, window, cap_q, cap_k;

@@ -10,13 +10,12 @@
 // fixed order and without atomics.  A TMA box {64, G, 1, P} over the [D, G, KV, rows] view of the queries lays that tile out.
 //
 // Tiles never span two sequences.  Which tiles there are depends on lengths that only the device knows, so a plan kernel writes
-// two work lists (query tiles, key tiles), longest first within a span of rows whose K and V stay in L2; the grids are sized by
-// the bound rows / P + sequences + 2 and a CTA without a tile returns.  What a tile loads beyond the end of its sequence (another
+// two work lists (query tiles, key tiles), longest first within a span of rows whose K and V stay in L2.  What a tile loads beyond the end of its sequence (another
 // sequence's rows, or rows behind the last one, with any values in them) is set to zero in shared memory before a product sums
 // over it, so the results of a sequence do not depend on what surrounds it, bit for bit.
 //
-// The pipelines are those of attn_fwd4_sm100.cu (forward: two CTAs per SM) and attn_wide_sm100.cu (backward: ten warps, two-phase
-// softmax, dK/dV and dQ in one grid); what is said there about the MMA order, the TMEM reuse and their bounds holds here too.
+// The inner pipelines are those of attn_fwd4_sm100.cu (forward: two CTAs per SM) and attn_wide_sm100.cu (backward: ten warps, two-phase
+// softmax); what is said there about the MMA order, the TMEM reuse and their bounds holds here too.
 #include "attn_common.cuh"
 
 namespace arb {
@@ -40,6 +39,8 @@ struct PackedArgs {
   float scale;
   __nv_bfloat16* o;                  // forward: O; backward: dQ.  Row stride in elements, heads D apart
   long long ldo;
+  __nv_bfloat16* o_lo;               // forward: what the rounding of O to bf16 left over, or null
+  int* next;                         // backward: [2] next tile of the key and of the query list
   float* lse;                        // [rows, H]
   const float* delta;                // [rows, H]
   __nv_bfloat16* dk;
@@ -204,6 +205,47 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedArgs& p, const Pac
   return t;
 }
 
+// A wait of a whole warp: all of its lanes go on, or none does, so that the warp stays together where a wait runs out.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+}
+
+// CTAs stay and take tile after tile: barriers, TMEM and the pipeline's start are paid once, and a tile's first loads run under the
+// previous tile's last products and epilogue (as one CTA per tile, sequences of 128 rows cost 10 us of an SM per backward tile).
+// The loading warp decides which tile is next and hands it to the other roles through two slots.
+struct PackedSlot { int start, len, tile, kv; };       // len = 0: no more tiles
+struct SlotRing {
+  uint64_t* full;                                       // [2] 1 arrival
+  uint64_t* empty;                                      // [2] one arrival per consumer
+  PackedSlot* slot;                                     // [2]
+  volatile int* abort_flag;
+  __device__ __forceinline__ void init(int consumers) {
+    for (int i = 0; i < 2; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], uint32_t(consumers)); }
+  }
+  // by one thread
+  __device__ __forceinline__ bool put(int n, const PackedTile& t) {
+    if (!mbar_wait(&empty[n & 1], (uint32_t(n >> 1) & 1u) ^ 1u, abort_flag)) return false;
+    slot[n & 1] = PackedSlot{t.it.start, t.it.len, t.it.tile, t.kv};
+    mbar_arrive(&full[n & 1]);
+    return true;
+  }
+  // by one thread
+  __device__ __forceinline__ PackedSlot take(int n) {
+    if (!mbar_wait(&full[n & 1], uint32_t(n >> 1) & 1u, abort_flag)) return PackedSlot{0, 0, 0, 0};
+    const PackedSlot s = slot[n & 1];
+    mbar_arrive(&empty[n & 1]);
+    return s;
+  }
+  // by a whole warp
+  __device__ __forceinline__ PackedSlot take_warp(int n, int lane) {
+    if (!wait_warp(&full[n & 1], uint32_t(n >> 1) & 1u, abort_flag)) return PackedSlot{0, 0, 0, 0};
+    const PackedSlot s = slot[n & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[n & 1]);
+    return s;
+  }
+};
+
 // Rows [from, to) of a 128-row tile of D columns, set to zero by the 32 lanes of a warp
 template <int D>
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int lane) {
@@ -246,10 +288,20 @@ __device__ __forceinline__ void store32(__nv_bfloat16* dst, const uint32_t (&v)[
     *reinterpret_cast<uint4*>(dst + j) = u;
   }
 }
-// `n` rows from `row` of `width` elements each, zero
-__device__ __forceinline__ void zero_out(__nv_bfloat16* dst, long long ld, int row, int n, int width) {
+// ... and what that rounding leaves over, rounded in turn
+__device__ __forceinline__ void store32_rest(__nv_bfloat16* dst, const uint32_t (&v)[32], float s) {
+  uint32_t rest[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float x = __uint_as_float(v[j]) * s;
+    rest[j] = __float_as_uint(x - __bfloat162float(__float2bfloat16(x)));
+  }
+  store32(dst, rest, 1.f);
+}
+// `n` rows from `row` of `width` elements each, zero, by a warp
+__device__ __forceinline__ void zero_out(__nv_bfloat16* dst, long long ld, int row, int n, int width, int lane) {
   const int per = width / 8;
-  for (int i = threadIdx.x; i < n * per; i += blockDim.x)
+  for (int i = lane; i < n * per; i += 32)
     *reinterpret_cast<uint4*>(dst + (long long)(row + i / per) * ld + (i % per) * 8) = make_uint4(0, 0, 0, 0);
 }
 
@@ -261,7 +313,20 @@ struct PackedFwdSmem {
   static constexpr int TILE = 128 * D * 2;
   static constexpr int Q = 0, K = TILE, V = 2 * TILE;
   static constexpr int BAR = 3 * TILE;
-  static constexpr int TOTAL = BAR + 128 + 1024;         // + alignment slack
+  static constexpr int TOTAL = BAR + 192 + 1024;         // + alignment slack
+};
+static_assert(2 * (PackedFwdSmem<128>::TOTAL + 1024) <= 233472, "two CTAs must fit the 228 KB of an SM");
+
+// positions and key tiles of a query tile
+struct QueryTile {
+  int m0, m_last, j_lo, n_tiles, live;                   // live: rows of the last key tile that belong to the sequence
+  __device__ __forceinline__ QueryTile(const PackedArgs& p, int len, int tile) {
+    m0 = tile * p.P;
+    m_last = min(m0 + p.P, len) - 1;
+    j_lo = max(0, m0 - p.window) / 128;
+    n_tiles = m_last / 128 - j_lo + 1;
+    live = min(128, len - (j_lo + n_tiles - 1) * 128);
+  }
 };
 
 template <int D>
@@ -272,20 +337,22 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
-  uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;
+  uint64_t* q_full = bars;            // Q of the n-th query tile
+  uint64_t* k_full = bars + 1;        // below, T counts the key tiles of all query tiles
   uint64_t* v_full = bars + 2;
-  uint64_t* s_full = bars + 3;        // S(t) complete: scores readable, K slot free
-  uint64_t* p_full = bars + 4;        // [2] P(t) of keys 64..127, then of keys 0..63, written (4 arrivals)
-  uint64_t* pv_done = bars + 6;       // P V(t) complete: V slot free, after the last one O is final
+  uint64_t* s_full = bars + 3;        // S(T) complete: scores readable, K slot free; Q's too behind the last one of a query tile
+  uint64_t* p_full = bars + 4;        // [2] P(T) of keys 64..127, then of keys 0..63, written (4 arrivals)
+  uint64_t* pv_done = bars + 6;       // P V(T) complete: V slot free, behind the last one O is final
   uint64_t* v_land = bars + 7;        // a V tile that has to be cleaned has landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  SlotRing ring{bars + 8, bars + 10, reinterpret_cast<PackedSlot*>(bars + 14), abort_flag};
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1); mbar_init(k_full, 1); mbar_init(v_full, 1);
     mbar_init(s_full, 1); mbar_init(&p_full[0], 4); mbar_init(&p_full[1], 4); mbar_init(pv_done, 1); mbar_init(v_land, 1);
+    ring.init(1 + 4);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -296,64 +363,88 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t tmem = *tmem_slot;
   grid_enter();                 // global memory is not touched above
   const uint32_t TM_S = tmem, TM_P = tmem + 64, TM_O = tmem + 128;
-
-  const PackedTile tile = packed_tile(p, p.items_q, p.n_q, int(blockIdx.x));
-  const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
   const int H = p.KV * p.G;
-  if (len > 0 && tile.it.tile < 0) {                     // rows of no sequence
-    zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D);
-    for (int i = threadIdx.x; i < len * p.G; i += blockDim.x)
-      p.lse[(long long)(start + i / p.G) * H + kv * p.G + i % p.G] = -INFINITY;
-  } else if (len > 0) {
-    const int m0 = tile.it.tile * p.P, m_last = min(m0 + p.P, len) - 1;       // first and last position of the tile
-    const int j_lo = max(0, m0 - p.window) / 128;
-    const int n_tiles = m_last / 128 - j_lo + 1;
-    const int live = len - (j_lo + n_tiles - 1) * 128;   // rows of the last key tile that belong to the sequence
-    const bool clean = live < 128;
-    if (warp == 0) {
+
+  if (warp == 0) {
+    if (lane == 0) { tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
+    const int total = p.n_q * p.KV, width = int(gridDim.x);
+    int T = 0, n = 0, cleaned = 0;
+    bool ok = true;
+    // rounds over the list in turn from either end of the grid, so that every CTA gets long and short tiles
+    for (int round = 0; ok; ++round) {
+      const int i = round * width + ((round & 1) ? width - 1 - int(blockIdx.x) : int(blockIdx.x));
+      if (round * width >= total) break;
+      if (i >= total) continue;
+      const PackedTile tile = packed_tile(p, p.items_q, p.n_q, i);
+      const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+      if (len == 0) continue;
+      if (tile.it.tile < 0) {                            // rows of no sequence
+        zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D, lane);
+        if (p.o_lo) zero_out(p.o_lo + (long long)kv * p.G * D, p.ldo, start, len, p.G * D, lane);
+        for (int e = lane; e < len * p.G; e += 32) p.lse[(long long)(start + e / p.G) * H + kv * p.G + e % p.G] = -INFINITY;
+        continue;
+      }
+      const QueryTile qt(p, len, tile.it.tile);
+      const bool clean = qt.live < 128;
       if (lane == 0) {
-        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
-        mbar_expect_tx(q_full, uint32_t(p.P * p.G * D * 2));          // rows past the end of the tensor are zero-filled
-        load_q<D>(smem + L::Q, &tmQ, q_full, kv, start + m0);
-        for (int t = 0; t < n_tiles; ++t) {
-          const int row = start + (j_lo + t) * 128;
-          if (t > 0 && !mbar_wait(s_full, uint32_t(t - 1) & 1u, abort_flag)) break;
+        ok = ring.put(n, tile);
+        for (int t = 0; ok && t < qt.n_tiles; ++t, ++T) {
+          const int row = start + (qt.j_lo + t) * 128;
+          if (T > 0 && !mbar_wait(s_full, uint32_t(T - 1) & 1u, abort_flag)) { ok = false; break; }
+          if (t == 0) {
+            mbar_expect_tx(q_full, uint32_t(p.P * p.G * D * 2));          // rows past the end of the tensor are zero-filled
+            load_q<D>(smem + L::Q, &tmQ, q_full, kv, start + qt.m0);
+          }
           mbar_expect_tx(k_full, L::TILE);
           load_kv<D>(smem + L::K, &tmK, k_full, kv, row);
-          if (t > 0 && !mbar_wait(pv_done, uint32_t(t - 1) & 1u, abort_flag)) break;
-          uint64_t* bar = (clean && t == n_tiles - 1) ? v_land : v_full;
+          if (T > 0 && !mbar_wait(pv_done, uint32_t(T - 1) & 1u, abort_flag)) { ok = false; break; }
+          uint64_t* bar = (clean && t == qt.n_tiles - 1) ? v_land : v_full;
           mbar_expect_tx(bar, L::TILE);
           load_kv<D>(smem + L::V, &tmV, bar, kv, row);
         }
       }
-      __syncwarp();
-      if (clean && mbar_wait(v_land, 0, abort_flag)) clean_tile<D>(smem + L::V, live, 128, v_full, lane);
-    } else if (warp == 1) {
-      if (lane == 0) {
-        constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
-        constexpr uint32_t idesc_o = make_idesc_bf16(128, D, false, true);
-        // descriptor words once; a K slice is a 32-bit add on the low word (start address >> 4)
-        const uint32_t hi_k = uint32_t(make_smem_desc(0, 0, 1024) >> 32), hi_v = uint32_t(make_smem_desc(0, 16384, 1024) >> 32);
-        const uint32_t q_lo = uint32_t(make_smem_desc(smem_u32(smem + L::Q), 0, 1024));
-        const uint32_t k_lo = uint32_t(make_smem_desc(smem_u32(smem + L::K), 0, 1024));
-        const uint32_t v_lo = uint32_t(make_smem_desc(smem_u32(smem + L::V), 16384, 1024));
-        bool ok = mbar_wait(q_full, 0, abort_flag);
-        auto issue_s = [&](int t) {
-          if (!mbar_wait(k_full, uint32_t(t) & 1u, abort_flag)) { ok = false; return; }
-          tc_fence_after();
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (clean && ok) {
+        ok = wait_warp(v_land, uint32_t(cleaned) & 1u, abort_flag);
+        ++cleaned;
+        if (ok) clean_tile<D>(smem + L::V, qt.live, 128, v_full, lane);
+      }
+      ++n;
+    }
+    if (ok && lane == 0) ring.put(n, PackedTile{PackedItem{0, 0, 0, 0}, 0});
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc_bf16(128, 128, false, false);
+      constexpr uint32_t idesc_o = make_idesc_bf16(128, D, false, true);
+      // descriptor words once; a K slice is a 32-bit add on the low word (start address >> 4)
+      const uint32_t hi_k = uint32_t(make_smem_desc(0, 0, 1024) >> 32), hi_v = uint32_t(make_smem_desc(0, 16384, 1024) >> 32);
+      const uint32_t q_lo = uint32_t(make_smem_desc(smem_u32(smem + L::Q), 0, 1024));
+      const uint32_t k_lo = uint32_t(make_smem_desc(smem_u32(smem + L::K), 0, 1024));
+      const uint32_t v_lo = uint32_t(make_smem_desc(smem_u32(smem + L::V), 16384, 1024));
+      bool ok = true;
+      int T = 0;
+      auto issue_s = [&](int tt) {
+        if (!mbar_wait(k_full, uint32_t(tt) & 1u, abort_flag)) { ok = false; return; }
+        tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = uint32_t(k >> 2) * 1024u + uint32_t(k & 3) * 2u;     // (16 KB half, 32 B slice) >> 4
-            tc_mma_ss_lh(TM_S, q_lo + off, hi_k, k_lo + off, hi_k, idesc_s, k > 0);
-          }
-          tc_commit(s_full);
-        };
-        if (ok) issue_s(0);
-        for (int t = 0; t < n_tiles && ok; ++t) {
-          if (!mbar_wait(v_full, uint32_t(t) & 1u, abort_flag)) { ok = false; break; }
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = uint32_t(k >> 2) * 1024u + uint32_t(k & 3) * 2u;     // (16 KB half, 32 B slice) >> 4
+          tc_mma_ss_lh(TM_S, q_lo + off, hi_k, k_lo + off, hi_k, idesc_s, k > 0);
+        }
+        tc_commit(s_full);
+      };
+      for (int n = 0; ok; ++n) {
+        const PackedSlot slot = ring.take(n);
+        if (slot.len == 0) break;
+        const int n_tiles = QueryTile(p, slot.len, slot.tile).n_tiles;
+        ok = mbar_wait(q_full, uint32_t(n) & 1u, abort_flag);
+        if (ok) issue_s(T);               // behind the previous query tile's last P V, which reads columns of the tile it overwrites
+        for (int t = 0; t < n_tiles && ok; ++t, ++T) {
+          if (!mbar_wait(v_full, uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {              // the upper keys' products run under the lower keys' exponentials
-            if (!mbar_wait(&p_full[hf], uint32_t(t) & 1u, abort_flag)) { ok = false; break; }
+            // t = 0: the four warps announce P behind their epilogue of the previous query tile, so O may be overwritten
+            if (!mbar_wait(&p_full[hf], uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
             tc_fence_after();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -363,25 +454,32 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           if (!ok) break;
           tc_commit(pv_done);
-          if (t + 1 < n_tiles) issue_s(t + 1);          // behind P V(t), which reads columns of the tile it overwrites
+          if (t + 1 < n_tiles) issue_s(T + 1);          // behind P V(T), which reads columns of the tile it overwrites
         }
       }
-    } else {
-      // ---------------- softmax / epilogue: thread <-> row of the tile = (position, head of the group) ----------------
-      const int q = warp & 3;
-      const int r = q * 32 + lane;
-      const int at = r / p.G, pos = m0 + at;
-      const bool live_row = at < p.P && pos < len;
-      const uint32_t lane_addr = uint32_t(q * 32) << 16;
-      const float c = p.scale * LOG2E;
+    }
+  } else {
+    // ---------------- softmax / epilogue: thread <-> row of the tile = (position, head of the group) ----------------
+    const int q = warp & 3;
+    const int r = q * 32 + lane;
+    const int at = r / p.G;
+    const uint32_t lane_addr = uint32_t(q * 32) << 16;
+    const float c = p.scale * LOG2E;
+    bool ok = true;
+    int T = 0;
+    for (int n = 0; ok; ++n) {
+      const PackedSlot slot = ring.take_warp(n, lane);
+      if (slot.len == 0) break;
+      const QueryTile qt(p, slot.len, slot.tile);
+      const int pos = qt.m0 + at;
+      const bool live_row = at < p.P && pos < slot.len;
       float m_used = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int t = 0; t < n_tiles; ++t) {
-        const int n0 = (j_lo + t) * 128;
-        if (!mbar_wait(s_full, uint32_t(t) & 1u, abort_flag)) { ok = false; break; }
+      for (int t = 0; t < qt.n_tiles; ++t, ++T) {
+        const int n0 = (qt.j_lo + t) * 128;
+        if (!wait_warp(s_full, uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        // rows without a query see nothing, in the unmasked tiles too only their own, unused results differ
-        const bool need_mask = (n0 + 127 > m0) || (n0 < m_last - p.window);
+        // in unmasked tiles rows without a query compute results of their own that nothing uses
+        const bool need_mask = (n0 + 127 > qt.m0) || (n0 < qt.m_last - p.window);
         // visible keys of this row inside the tile: column indices [mlo, mlo + span]
         const int mlo = live_row ? pos - p.window - n0 : 128;
         const unsigned span = live_row ? unsigned(p.window) : 0u;
@@ -459,20 +557,22 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[1]);
       }
-      if (ok && mbar_wait(pv_done, uint32_t(n_tiles - 1) & 1u, abort_flag)) {
-        tc_fence_after();
-        const float inv_l = (l > 0.f) ? 1.f / l : 0.f;
-        const int head = kv * p.G + (r - at * p.G);
-        __nv_bfloat16* orow = p.o + (long long)(start + pos) * p.ldo + (long long)head * D;
+      if (!ok || !wait_warp(pv_done, uint32_t(T - 1) & 1u, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      const float inv_l = (l > 0.f) ? 1.f / l : 0.f;
+      const int head = slot.kv * p.G + (r - at * p.G);
+      const long long row = (long long)(slot.start + pos) * p.ldo + (long long)head * D;
 #pragma unroll
-        for (int cc = 0; cc < D / 32; ++cc) {
-          uint32_t v[32];
-          tmem_ld32(TM_O + lane_addr + uint32_t(cc * 32), v);
-          tmem_wait_ld();
-          if (live_row) store32(orow + cc * 32, v, inv_l);
+      for (int cc = 0; cc < D / 32; ++cc) {
+        uint32_t v[32];
+        tmem_ld32(TM_O + lane_addr + uint32_t(cc * 32), v);
+        tmem_wait_ld();
+        if (live_row) {
+          store32(p.o + row + cc * 32, v, inv_l);
+          if (p.o_lo) store32_rest(p.o_lo + row + cc * 32, v, inv_l);
         }
-        if (live_row) p.lse[(long long)(start + pos) * H + head] = (l > 0.f) ? (m_used * p.scale + __logf(l)) : -INFINITY;
       }
+      if (live_row) p.lse[(long long)(slot.start + pos) * H + head] = (l > 0.f) ? (m_used * p.scale + __logf(l)) : -INFINITY;
     }
   }
   tc_fence_before();
@@ -484,7 +584,8 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 // -----------------------------------------------------------------------------------------------
 // backward
 // -----------------------------------------------------------------------------------------------
-// two resident tiles, a three-slot and a two-slot ring
+// Two resident tiles, a three-slot and a two-slot ring.  A CTA takes key tiles (dK, dV) until there are no more, then query tiles
+// (dQ): both lists are handed out by counters, so CTAs that got short tiles take more of them.
 template <int D>
 struct PackedBwdSmem {
   static constexpr int TILE = 128 * D * 2;
@@ -492,10 +593,26 @@ struct PackedBwdSmem {
   static constexpr int RING3 = 2 * TILE;
   static constexpr int RING2 = 5 * TILE;
   static constexpr int STAT = 7 * TILE;                  // lse2[2][128], delta[2][128] (dK/dV)
-  static constexpr int BAR = STAT + 4 * 128 * 4;
-  static constexpr int TOTAL = BAR + 512;
+  static constexpr int BAR = STAT + 4 * 128 * 4;         // dK/dV, dQ, then what both share
+  static constexpr int BAR_DQ = BAR + 256, COMMON = BAR_DQ + 256;
+  static constexpr int TOTAL = COMMON + 64;
 };
 static_assert(PackedBwdSmem<128>::TOTAL <= 232448, "exceeds the 227 KB shared memory of one CTA");
+
+struct BwdCta { uint8_t* smem; uint32_t tmem; volatile int* abort_flag; int warp, lane; };
+
+// the next tile of a list that is not empty, to the whole warp; len = 0: none
+__device__ __forceinline__ PackedTile next_tile(const PackedArgs& p, const PackedItem* items, int n, int* counter, int lane) {
+  const int total = n * p.KV;
+  for (;;) {
+    int i = 0;
+    if (lane == 0) i = atomicAdd(counter, 1);
+    i = __shfl_sync(0xffffffffu, i, 0);
+    if (i >= total) return PackedTile{PackedItem{0, 0, 0, 0}, 0};
+    const PackedTile t = packed_tile(p, items, n, i);
+    if (t.it.len > 0) return t;
+  }
+}
 
 // 128 x 128 product over the D columns of two K-major tiles
 template <int D>
@@ -521,156 +638,176 @@ __device__ __forceinline__ void mma_sum(uint32_t d_tmem, uint32_t a_lo, uint32_t
 
 // ---- dQ: query tile stationary -----------------------------------------------------------------
 template <int D>
-__device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
-                                              const CUtensorMap& tmDO, const PackedArgs& p, int block) {
-  using L = PackedBwdSmem<D>;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
-  uint64_t* q_full = bars;            // Q + dO resident
-  uint64_t* k_full = bars + 1;        // [3]
-  uint64_t* v_full = bars + 4;        // [2]
-  uint64_t* s_full = bars + 6;        // S(t) complete
-  uint64_t* a_done = bars + 7;        // phase A(t) has read S(t)            (8 arrivals)
-  uint64_t* dp_full = bars + 8;       // [2] dP(t) complete; also frees V(t)'s slot
-  uint64_t* ds_full = bars + 10;      // [2] phase B(t) wrote dS(t) and has read dP(t) (8 arrivals)
-  uint64_t* dq_done = bars + 12;      // [6] dQ(t) MMAs complete: frees K(t)'s slot and dS buffer t&1
-  uint64_t* done = bars + 18;         // all dQ MMAs complete
-  uint64_t* land = bars + 19;         // [2] K / V tile that has to be cleaned has landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int i = 0; i < 3; ++i) mbar_init(&k_full[i], 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&v_full[i], 1); mbar_init(&dp_full[i], 1); mbar_init(&ds_full[i], 8); mbar_init(&land[i], 1); }
-    mbar_init(s_full, 1); mbar_init(a_done, 8);
-    for (int i = 0; i < 6; ++i) mbar_init(&dq_done[i], 1);
-    mbar_init(done, 1);
-    *abort_flag = 0;
-    fence_barrier_init();
+struct DqBars {
+  uint64_t* b;
+  __device__ __forceinline__ uint64_t* q_full() const { return b; }             // Q + dO of the n-th query tile
+  __device__ __forceinline__ uint64_t* k_full(int T) const { return b + 1 + T % 3; }
+  __device__ __forceinline__ uint64_t* v_full(int T) const { return b + 4 + (T & 1); }
+  __device__ __forceinline__ uint64_t* s_full() const { return b + 6; }         // S(T) complete
+  __device__ __forceinline__ uint64_t* a_done() const { return b + 7; }         // phase A(T) has read S(T)            (8 arrivals)
+  __device__ __forceinline__ uint64_t* dp_full(int T) const { return b + 8 + (T & 1); }    // dP(T) complete; also frees V(T)'s slot
+  __device__ __forceinline__ uint64_t* ds_full(int T) const { return b + 10 + (T & 1); }   // phase B(T) wrote dS(T) and has read dP(T) (8)
+  __device__ __forceinline__ uint64_t* dq_done(int T) const { return b + 12 + T % 6; }     // dQ(T) complete: K(T)'s slot and dS buffer T & 1 free
+  __device__ __forceinline__ uint64_t* done() const { return b + 18; }          // dQ of the n-th query tile complete
+  __device__ __forceinline__ uint64_t* land(int i) const { return b + 19 + i; } // K / V tile that has to be cleaned has landed
+  __device__ __forceinline__ uint64_t* ring() const { return b + 21; }          // 4
+  static constexpr int COUNT = 25;
+  __device__ __forceinline__ void init() const {
+    for (int i = 0; i < 21; ++i) mbar_init(b + i, i == 7 || i == 10 || i == 11 ? 8 : 1);
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  grid_enter();                 // global memory is not touched above
-  const uint32_t TM_S = tmem, TM_DP = tmem + 128, TM_DQ = tmem + 256, TM_DS = tmem + 384;
+};
+static_assert(DqBars<64>::COUNT * 8 + 2 * sizeof(PackedSlot) <= 256, "barrier space");
 
-  const PackedTile tile = packed_tile(p, p.items_q, p.n_q, block);
-  const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+template <int D>
+__device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
+                                              const CUtensorMap& tmDO, const PackedArgs& p, const BwdCta& cta) {
+  using L = PackedBwdSmem<D>;
+  uint8_t* smem = cta.smem;
+  volatile int* abort_flag = cta.abort_flag;
+  const DqBars<D> bar{reinterpret_cast<uint64_t*>(smem + L::BAR_DQ)};
+  SlotRing ring{bar.ring(), bar.ring() + 2, reinterpret_cast<PackedSlot*>(smem + L::COMMON + 32), abort_flag};
+  const int warp = cta.warp, lane = cta.lane;
+  const uint32_t TM_S = cta.tmem, TM_DP = cta.tmem + 128, TM_DQ = cta.tmem + 256, TM_DS = cta.tmem + 384;
   const int H = p.KV * p.G;
-  if (len > 0 && tile.it.tile < 0) {                     // rows of no sequence
-    zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D);
-  } else if (len > 0) {
-    const int m0 = tile.it.tile * p.P, m_last = min(m0 + p.P, len) - 1;
-    const int j_lo = max(0, m0 - p.window) / 128;
-    const int n_tiles = m_last / 128 - j_lo + 1;
-    const int live = len - (j_lo + n_tiles - 1) * 128;   // rows of the last key tile that belong to the sequence
-    const bool clean = live < 128;
-    if (warp == 0) {
-      const uint32_t q_bytes = uint32_t(p.P * p.G * D * 2);
-      auto k_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
-      auto v_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
-      // K(t) is requested when dQ(t-3) has released its slot, V(t) when dP(t-2) has
-      auto load_k_tile = [&](int t, uint64_t* bar) -> bool {
-        if (t >= 3 && !mbar_wait(&dq_done[(t - 3) % 6], uint32_t((t - 3) / 6) & 1u, abort_flag)) return false;
-        mbar_expect_tx(bar, L::TILE);
-        load_kv<D>(k_slot(t), &tmK, bar, kv, start + (j_lo + t) * 128);
-        return true;
-      };
-      auto load_v_tile = [&](int t, uint64_t* bar) -> bool {
-        if (t >= 2 && !mbar_wait(&dp_full[t & 1], uint32_t((t - 2) >> 1) & 1u, abort_flag)) return false;
-        mbar_expect_tx(bar, L::TILE);
-        load_kv<D>(v_slot(t), &tmV, bar, kv, start + (j_lo + t) * 128);
-        return true;
-      };
-      const int last = n_tiles - 1;
-      if (lane == 0) {
-        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmDO);
-        mbar_expect_tx(q_full, 2 * q_bytes);
-        load_q<D>(smem + L::RES0, &tmQ, q_full, kv, start + m0);
-        load_q<D>(smem + L::RES1, &tmDO, q_full, kv, start + m0);
-        bool ok = true;
-        for (int t = 0; ok && t < n_tiles - (clean ? 1 : 0); ++t)
-          ok = load_k_tile(t, &k_full[t % 3]) && load_v_tile(t, &v_full[t & 1]);
-        if (clean && ok) ok = load_k_tile(last, &land[0]) && load_v_tile(last, &land[1]);
+
+  if (warp == 0) {
+    const uint32_t q_bytes = uint32_t(p.P * p.G * D * 2);
+    int T = 0, cleaned = 0;
+    bool ok = true;
+    auto k_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
+    auto v_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
+    for (int n = 0; ok;) {
+      const PackedTile tile = next_tile(p, p.items_q, p.n_q, p.next + 1, lane);
+      const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+      if (len == 0) { if (lane == 0) ring.put(n, tile); break; }
+      if (tile.it.tile < 0) {                            // rows of no sequence
+        zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D, lane);
+        continue;
       }
-      __syncwarp();
-      // both are summed over or multiplied with: rows of other sequences must not leave a NaN behind
-      if (clean && mbar_wait(&land[0], 0, abort_flag)) {
-        clean_tile<D>(k_slot(last), live, 128, &k_full[last % 3], lane);
-        if (mbar_wait(&land[1], 0, abort_flag)) clean_tile<D>(v_slot(last), live, 128, &v_full[last & 1], lane);
-      }
-    } else if (warp == 1) {
+      const QueryTile qt(p, len, tile.it.tile);
+      const bool clean = qt.live < 128;
+      const int last = T + qt.n_tiles - 1;
       if (lane == 0) {
-        const uint32_t sq = smem_u32(smem + L::RES0), sdo = smem_u32(smem + L::RES1);
-        const uint32_t sk0 = smem_u32(smem + L::RING3), sv0 = smem_u32(smem + L::RING2);
-        bool ok = mbar_wait(q_full, 0, abort_flag);
-        if (ok) ok = mbar_wait(&k_full[0], 0, abort_flag);
+        ok = ring.put(n, tile);
+        // Q and dO are free behind the last S and dP of the previous query tile
+        if (ok && T > 0) ok = mbar_wait(bar.dp_full(T - 1), uint32_t((T - 1) >> 1) & 1u, abort_flag);
         if (ok) {
-          tc_fence_after();
-          mma_scores<D>(TM_S, sq, sk0);
-          tc_commit(s_full);
-          ok = mbar_wait(&v_full[0], 0, abort_flag);
+          mbar_expect_tx(bar.q_full(), 2 * q_bytes);
+          load_q<D>(smem + L::RES0, &tmQ, bar.q_full(), kv, start + qt.m0);
+          load_q<D>(smem + L::RES1, &tmDO, bar.q_full(), kv, start + qt.m0);
         }
-        if (ok) {
-          tc_fence_after();
-          mma_scores<D>(TM_DP, sdo, sv0);
-          tc_commit(&dp_full[0]);
+        // K(T) is requested when dQ(T-3) has released its slot, V(T) when dP(T-2) has
+        for (int t = T; ok && t <= last; ++t) {
+          const int row = start + (qt.j_lo + t - T) * 128;
+          if (t >= 3 && !mbar_wait(bar.dq_done(t - 3), uint32_t((t - 3) / 6) & 1u, abort_flag)) { ok = false; break; }
+          uint64_t* kb = clean && t == last ? bar.land(0) : bar.k_full(t);
+          mbar_expect_tx(kb, L::TILE);
+          load_kv<D>(k_slot(t), &tmK, kb, kv, row);
+          if (t >= 2 && !mbar_wait(bar.dp_full(t), uint32_t((t - 2) >> 1) & 1u, abort_flag)) { ok = false; break; }
+          uint64_t* vb = clean && t == last ? bar.land(1) : bar.v_full(t);
+          mbar_expect_tx(vb, L::TILE);
+          load_kv<D>(v_slot(t), &tmV, vb, kv, row);
         }
-        for (int t = 0; t < n_tiles && ok; ++t) {
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (clean && ok) {
+        // both are summed over or multiplied with: rows of other sequences must not leave a NaN behind
+        ok = wait_warp(bar.land(0), uint32_t(cleaned) & 1u, abort_flag);
+        if (ok) clean_tile<D>(k_slot(last), qt.live, 128, bar.k_full(last), lane);
+        ok = ok && wait_warp(bar.land(1), uint32_t(cleaned) & 1u, abort_flag);
+        if (ok) clean_tile<D>(v_slot(last), qt.live, 128, bar.v_full(last), lane);
+        ++cleaned;
+      }
+      T = last + 1;
+      ++n;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t sq = smem_u32(smem + L::RES0), sdo = smem_u32(smem + L::RES1);
+      const uint32_t sk0 = smem_u32(smem + L::RING3), sv0 = smem_u32(smem + L::RING2);
+      bool ok = true;
+      auto issue_s = [&](int T) {
+        ok = ok && mbar_wait(bar.k_full(T), uint32_t(T / 3) & 1u, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+        mma_scores<D>(TM_S, sq, sk0 + uint32_t(T % 3) * L::TILE);
+        tc_commit(bar.s_full());
+      };
+      auto issue_dp = [&](int T) {
+        ok = ok && mbar_wait(bar.v_full(T), uint32_t(T >> 1) & 1u, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+        mma_scores<D>(TM_DP, sdo, sv0 + uint32_t(T & 1) * L::TILE);
+        tc_commit(bar.dp_full(T));
+      };
+      int T = 0;
+      for (int n = 0; ok; ++n) {
+        const PackedSlot slot = ring.take(n);
+        if (slot.len == 0) break;
+        const int n_tiles = QueryTile(p, slot.len, slot.tile).n_tiles;
+        ok = mbar_wait(bar.q_full(), uint32_t(n) & 1u, abort_flag);
+        // S and dP of the previous query tile's last key tile have been read: phase B announced its dS behind both
+        issue_s(T);
+        issue_dp(T);
+        for (int t = 0; t < n_tiles && ok; ++t, ++T) {
           const bool more = t + 1 < n_tiles;
           if (more) {
-            if (!mbar_wait(a_done, uint32_t(t & 1), abort_flag)) { ok = false; break; }
-            if (!mbar_wait(&k_full[(t + 1) % 3], uint32_t((t + 1) / 3) & 1u, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            mma_scores<D>(TM_S, sq, sk0 + uint32_t((t + 1) % 3) * L::TILE);
-            tc_commit(s_full);
+            if (!mbar_wait(bar.a_done(), uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
+            issue_s(T + 1);
           }
-          if (!mbar_wait(&ds_full[t & 1], uint32_t(t >> 1) & 1u, abort_flag)) { ok = false; break; }
-          if (more) {
-            if (!mbar_wait(&v_full[(t + 1) & 1], uint32_t((t + 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            mma_scores<D>(TM_DP, sdo, sv0 + uint32_t((t + 1) & 1) * L::TILE);
-            tc_commit(&dp_full[(t + 1) & 1]);
-          }
+          if (!ok || !mbar_wait(bar.ds_full(T), uint32_t(T >> 1) & 1u, abort_flag)) { ok = false; break; }
+          if (more) issue_dp(T + 1);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t ds = TM_DS + uint32_t(t & 1) * 64u;
-          mma_sum<D>(TM_DQ, ds, ds + 32, sk0 + uint32_t(t % 3) * L::TILE, t > 0);
-          tc_commit(&dq_done[t % 6]);
+          // t = 0: the eight warps announce dS behind their epilogue of the previous query tile, so dQ may be overwritten
+          const uint32_t ds = TM_DS + uint32_t(T & 1) * 64u;
+          mma_sum<D>(TM_DQ, ds, ds + 32, sk0 + uint32_t(T % 3) * L::TILE, t > 0);
+          tc_commit(bar.dq_done(T));
+          // the last tile's phase A is waited for by nobody else: every phase of a_done is seen here
+          if (!more) { tc_commit(bar.done()); ok = mbar_wait(bar.a_done(), uint32_t(T) & 1u, abort_flag); }
         }
-        if (ok) tc_commit(done);
       }
-    } else {
-      const int sw = warp - 2;             // 0..7
-      const int q = warp & 3;              // TMEM lane quarter this warp may access
-      const int hf = sw >> 2;              // column half of the tile owned by this warp
-      const int r = q * 32 + lane;
-      const int at = r / p.G, pos = m0 + at;
-      const int head = kv * p.G + (r - at * p.G);
-      const bool live_row = at < p.P && pos < len;
-      const uint32_t lane_addr = uint32_t(q * 32) << 16;
-      const float c = p.scale * LOG2E;
-      const long long stat = (long long)(start + pos) * H + head;
-      const float lse2 = live_row ? p.lse[stat] * LOG2E : INFINITY;
-      const float dlt = live_row ? p.delta[stat] : 0.f;
-      bool ok = true;
-      for (int t = 0; t < n_tiles && ok; ++t) {
-        const int n0 = (j_lo + t) * 128 + hf * 64;   // first key of this thread's 64 columns
+    }
+  } else {
+    const int sw = warp - 2;             // 0..7
+    const int q = warp & 3;              // TMEM lane quarter this warp may access
+    const int hf = sw >> 2;              // column half of the tile owned by this warp
+    const int r = q * 32 + lane;
+    const int at = r / p.G;
+    const uint32_t lane_addr = uint32_t(q * 32) << 16;
+    const float c = p.scale * LOG2E;
+    bool ok = true;
+    int T = 0;
+    float lse2, dlt;
+    auto load_stats = [&](const PackedSlot& s) {
+      const int pos = s.tile * p.P + at;
+      lse2 = INFINITY; dlt = 0.f;
+      if (s.len > 0 && at < p.P && pos < s.len) {
+        const long long stat = (long long)(s.start + pos) * H + s.kv * p.G + (r - at * p.G);
+        lse2 = p.lse[stat] * LOG2E;
+        dlt = p.delta[stat];
+      }
+    };
+    PackedSlot slot = ring.take_warp(0, lane);
+    load_stats(slot);
+    for (int n = 0; ok && slot.len > 0; ++n) {
+      const QueryTile qt(p, slot.len, slot.tile);
+      const int pos = qt.m0 + at;
+      const bool live_row = at < p.P && pos < slot.len;
+      for (int t = 0; t < qt.n_tiles; ++t, ++T) {
+        const int n0 = (qt.j_lo + t) * 128 + hf * 64;   // first key of this thread's 64 columns
         float pr[64];
         // ---- phase A ----
-        if (!mbar_wait(s_full, uint32_t(t & 1), abort_flag)) { ok = false; break; }
+        if (!wait_warp(bar.s_full(), uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
         {
           uint32_t s0[32], s1[32];
           tmem_ld64(TM_S + lane_addr + uint32_t(hf * 64), s0, s1);
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(a_done);
+          if (lane == 0) mbar_arrive(bar.a_done());
           exp2_64<true>(s0, s1, c, lse2, nullptr, pr);
-          if ((n0 + 63 > m0) || (n0 < m_last - p.window)) {
+          if ((n0 + 63 > qt.m0) || (n0 < qt.m_last - p.window)) {
             // the visible keys of a row are one interval of column indices
             const int lo = live_row ? pos - p.window - n0 : 64;
             const unsigned span = live_row ? unsigned(p.window) : 0u;
@@ -679,7 +816,7 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
           }
         }
         // ---- phase B ----
-        if (!mbar_wait(&dp_full[t & 1], uint32_t(t >> 1) & 1u, abort_flag)) { ok = false; break; }
+        if (!wait_warp(bar.dp_full(T), uint32_t(T >> 1) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
         uint32_t pk[32];
         {
@@ -692,200 +829,220 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
                                    pr[32 + 2 * j + 1] * (__uint_as_float(d1[2 * j + 1]) - dlt));
           }
         }
-        // dS buffer t&1 was last read by the dQ MMAs of tile t-2
-        if (t >= 2 && !mbar_wait(&dq_done[(t - 2) % 6], uint32_t((t - 2) / 6) & 1u, abort_flag)) { ok = false; break; }
+        // dS buffer T & 1 was last read by the dQ MMAs of tile T-2
+        if (T >= 2 && !wait_warp(bar.dq_done(T - 2), uint32_t((T - 2) / 6) & 1u, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        tmem_st32(TM_DS + lane_addr + uint32_t((t & 1) * 64 + hf * 32), pk);
+        tmem_st32(TM_DS + lane_addr + uint32_t((T & 1) * 64 + hf * 32), pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ds_full[t & 1]);
+        if (lane == 0) mbar_arrive(bar.ds_full(T));
       }
-      if (ok && mbar_wait(done, 0, abort_flag)) {
-        tc_fence_after();
-        __nv_bfloat16* orow = p.o + (long long)(start + pos) * p.ldo + (long long)head * D + hf * (D / 2);
+      if (!ok) break;
+      const PackedSlot done = slot;
+      slot = ring.take_warp(n + 1, lane);
+      load_stats(slot);                    // in flight while this query tile is finished
+      if (!wait_warp(bar.done(), uint32_t(n) & 1u, abort_flag)) break;
+      tc_fence_after();
+      __nv_bfloat16* orow = p.o + (long long)(done.start + pos) * p.ldo + (long long)(done.kv * p.G + (r - at * p.G)) * D + hf * (D / 2);
 #pragma unroll
-        for (int cc = 0; cc < D / 64; ++cc) {
-          uint32_t v[32];
-          tmem_ld32(TM_DQ + lane_addr + uint32_t(hf * (D / 2) + cc * 32), v);
-          tmem_wait_ld();
-          if (live_row) store32(orow + cc * 32, v, p.scale);
-        }
+      for (int cc = 0; cc < D / 64; ++cc) {
+        uint32_t v[32];
+        tmem_ld32(TM_DQ + lane_addr + uint32_t(hf * (D / 2) + cc * 32), v);
+        tmem_wait_ld();
+        if (live_row) store32(orow + cc * 32, v, p.scale);
       }
     }
   }
-  tc_fence_before();
-  __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, ERR_ATTN_TIMEOUT);
-  if (warp == 1) { __syncwarp(); tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
 // ---- dK / dV: key tile stationary, transposed scores; the query tiles bring all heads of the group -------------------
 template <int D>
+struct DkvBars {
+  uint64_t* b;
+  __device__ __forceinline__ uint64_t* kv_full() const { return b; }            // K + V of the n-th key tile
+  __device__ __forceinline__ uint64_t* q_full(int T) const { return b + 1 + T % 3; }
+  __device__ __forceinline__ uint64_t* q_empty(int T) const { return b + 4 + T % 3; }      // dK(T) complete
+  __device__ __forceinline__ uint64_t* do_full(int T) const { return b + 7 + (T & 1); }
+  __device__ __forceinline__ uint64_t* do_empty(int T) const { return b + 9 + (T & 1); }   // dV(T) complete
+  __device__ __forceinline__ uint64_t* s_full() const { return b + 11; }        // S^T(T) complete
+  __device__ __forceinline__ uint64_t* p_full() const { return b + 12; }        // phase A(T) wrote P^T(T)             (8 arrivals)
+  __device__ __forceinline__ uint64_t* dp_full() const { return b + 13; }       // dP^T(T) complete
+  __device__ __forceinline__ uint64_t* ds_full() const { return b + 14; }       // phase B(T) wrote dS^T(T)            (8 arrivals)
+  __device__ __forceinline__ uint64_t* done() const { return b + 15; }          // dK and dV of the n-th key tile complete
+  __device__ __forceinline__ uint64_t* land(int i) const { return b + 16 + i; } // Q / dO tile that has to be cleaned has landed
+  __device__ __forceinline__ uint64_t* stat() const { return b + 18; }          // statistics of query tile T written (8 arrivals)
+  __device__ __forceinline__ uint64_t* ring() const { return b + 19; }          // 4
+  static constexpr int COUNT = 23;
+  __device__ __forceinline__ void init() const {
+    for (int i = 0; i < 19; ++i) mbar_init(b + i, i == 12 || i == 14 || i == 18 ? 8 : 1);
+  }
+};
+static_assert(DkvBars<64>::COUNT * 8 + 2 * sizeof(PackedSlot) <= 256, "barrier space");
+
+// query tiles of a key tile
+struct KeyTile {
+  int n0, i_lo, n_tiles, live;                           // live: rows of the last query tile that belong to the sequence
+  __device__ __forceinline__ KeyTile(const PackedArgs& p, int len, int tile) {
+    n0 = tile * 128;
+    const int last_q = min(len - 1, min(n0 + 127, len - 1) + p.window);
+    i_lo = n0 / p.P;
+    n_tiles = last_q / p.P - i_lo + 1;
+    live = min(p.P, len - (i_lo + n_tiles - 1) * p.P) * p.G;
+  }
+};
+
+template <int D>
 __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
-                                               const CUtensorMap& tmDO, const PackedArgs& p, int block) {
+                                               const CUtensorMap& tmDO, const PackedArgs& p, const BwdCta& cta) {
   using L = PackedBwdSmem<D>;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
-  uint64_t* kv_full = bars;           // K + V resident
-  uint64_t* q_full = bars + 1;        // [3]
-  uint64_t* q_empty = bars + 4;       // [3] dK(t) complete
-  uint64_t* do_full = bars + 7;       // [2]
-  uint64_t* do_empty = bars + 9;      // [2] dV(t) complete
-  uint64_t* s_full = bars + 11;       // S^T(t) complete
-  uint64_t* p_full = bars + 12;       // phase A(t) wrote P^T(t)              (8 arrivals)
-  uint64_t* dp_full = bars + 13;      // dP^T(t) complete
-  uint64_t* ds_full = bars + 14;      // phase B(t) wrote dS^T(t)             (8 arrivals)
-  uint64_t* done = bars + 15;
-  uint64_t* land = bars + 16;         // [2] Q / dO tile that has to be cleaned has landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* smem = cta.smem;
+  volatile int* abort_flag = cta.abort_flag;
+  const DkvBars<D> bar{reinterpret_cast<uint64_t*>(smem + L::BAR)};
+  SlotRing ring{bar.ring(), bar.ring() + 2, reinterpret_cast<PackedSlot*>(smem + L::BAR + 256 - 2 * sizeof(PackedSlot)), abort_flag};
   float* stat_lse = reinterpret_cast<float*>(smem + L::STAT);   // [2][128]
   float* stat_dl = stat_lse + 256;                               // [2][128]
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = cta.warp, lane = cta.lane;
   const int used = p.P * p.G;           // rows of a query tile that hold queries
-  if (threadIdx.x == 0) {
-    mbar_init(kv_full, 1);
-    for (int i = 0; i < 3; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&do_full[i], 1); mbar_init(&do_empty[i], 1); mbar_init(&land[i], 1); }
-    mbar_init(s_full, 1); mbar_init(p_full, 8); mbar_init(dp_full, 1); mbar_init(ds_full, 8); mbar_init(done, 1);
-    *abort_flag = 0;
-    fence_barrier_init();
-  }
-  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  if (used < 128 && warp >= 2 && warp < 7) {              // rows that no copy fills, in the five slots: they are summed over as well
-    zero_rows<D>(smem + L::RING3 + (warp - 2) * L::TILE, used, 128, lane);
-    fence_proxy_async_smem();
-  }
-  static_assert(L::RING2 == L::RING3 + 3 * L::TILE, "the rings follow one another");
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  grid_enter();                 // global memory is not touched above
-  const uint32_t TM_S = tmem, TM_DP = tmem + 128, TM_DV = tmem + 256, TM_DK = tmem + 384;
-
-  const PackedTile tile = packed_tile(p, p.items_k, p.n_k, block);
-  const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+  const uint32_t TM_S = cta.tmem, TM_DP = cta.tmem + 128, TM_DV = cta.tmem + 256, TM_DK = cta.tmem + 384;
   const int H = p.KV * p.G;
-  if (len > 0 && tile.it.tile < 0) {                     // rows of no sequence
-    zero_out(p.dk + (long long)kv * D, p.lddk, start, len, D);
-    zero_out(p.dv + (long long)kv * D, p.lddv, start, len, D);
-  } else if (len > 0) {
-    const int n0 = tile.it.tile * 128;
-    const int last_key = min(n0 + 127, len - 1);
-    const int last_q = min(len - 1, last_key + p.window);
-    const int i_lo = n0 / p.P;
-    const int n_tiles = last_q / p.P - i_lo + 1;
-    const int live = (len - (i_lo + n_tiles - 1) * p.P) * p.G;     // rows of the last query tile that belong to the sequence
-    const bool clean = live < used;
-    if (warp == 0) {
-      const uint32_t q_bytes = uint32_t(used * D * 2);
-      auto q_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
-      auto do_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
-      auto load_q_tile = [&](int t, uint64_t* bar) -> bool {
-        if (!mbar_wait(&q_empty[t % 3], (uint32_t(t / 3) & 1u) ^ 1u, abort_flag)) return false;
-        mbar_expect_tx(bar, q_bytes);
-        load_q<D>(q_slot(t), &tmQ, bar, kv, start + (i_lo + t) * p.P);
-        return true;
-      };
-      auto load_do_tile = [&](int t, uint64_t* bar) -> bool {
-        if (!mbar_wait(&do_empty[t & 1], (uint32_t(t >> 1) & 1u) ^ 1u, abort_flag)) return false;
-        mbar_expect_tx(bar, q_bytes);
-        load_q<D>(do_slot(t), &tmDO, bar, kv, start + (i_lo + t) * p.P);
-        return true;
-      };
-      const int last = n_tiles - 1;
+
+  if (warp == 0) {
+    const uint32_t q_bytes = uint32_t(used * D * 2);
+    int T = 0, cleaned = 0;
+    bool ok = true;
+    auto q_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
+    auto do_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
+    for (int n = 0; ok;) {
+      const PackedTile tile = next_tile(p, p.items_k, p.n_k, p.next, lane);
+      const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
+      if (len == 0) { if (lane == 0) ring.put(n, tile); break; }
+      if (tile.it.tile < 0) {                            // rows of no sequence
+        zero_out(p.dk + (long long)kv * D, p.lddk, start, len, D, lane);
+        zero_out(p.dv + (long long)kv * D, p.lddv, start, len, D, lane);
+        continue;
+      }
+      const KeyTile kt(p, len, tile.it.tile);
+      const bool clean = kt.live < used;
+      const int last = T + kt.n_tiles - 1;
       if (lane == 0) {
-        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmDO);
-        mbar_expect_tx(kv_full, 2 * L::TILE);
-        load_kv<D>(smem + L::RES0, &tmK, kv_full, kv, start + n0);
-        load_kv<D>(smem + L::RES1, &tmV, kv_full, kv, start + n0);
-        bool ok = true;
-        for (int t = 0; ok && t < n_tiles - (clean ? 1 : 0); ++t)
-          ok = load_q_tile(t, &q_full[t % 3]) && load_do_tile(t, &do_full[t & 1]);
-        if (clean && ok) ok = load_q_tile(last, &land[0]) && load_do_tile(last, &land[1]);
-      }
-      __syncwarp();
-      if (clean && mbar_wait(&land[0], 0, abort_flag)) {
-        clean_tile<D>(q_slot(last), live, used, &q_full[last % 3], lane);
-        if (mbar_wait(&land[1], 0, abort_flag)) clean_tile<D>(do_slot(last), live, used, &do_full[last & 1], lane);
-      }
-    } else if (warp == 1) {
-      if (lane == 0) {
-        const uint32_t sk = smem_u32(smem + L::RES0), sv = smem_u32(smem + L::RES1);
-        const uint32_t sq0 = smem_u32(smem + L::RING3), sdo0 = smem_u32(smem + L::RING2);
-        bool ok = mbar_wait(kv_full, 0, abort_flag);
-        if (ok) ok = mbar_wait(&q_full[0], 0, abort_flag);
+        ok = ring.put(n, tile);
+        // K and V are free behind the last S^T and dP^T of the previous key tile
+        if (ok && T > 0) ok = mbar_wait(bar.dp_full(), uint32_t(T - 1) & 1u, abort_flag);
         if (ok) {
-          tc_fence_after();
-          mma_scores<D>(TM_S, sk, sq0);
-          tc_commit(s_full);
-          ok = mbar_wait(&do_full[0], 0, abort_flag);
+          mbar_expect_tx(bar.kv_full(), 2 * L::TILE);
+          load_kv<D>(smem + L::RES0, &tmK, bar.kv_full(), kv, start + kt.n0);
+          load_kv<D>(smem + L::RES1, &tmV, bar.kv_full(), kv, start + kt.n0);
         }
-        if (ok) {
-          tc_fence_after();
-          mma_scores<D>(TM_DP, sv, sdo0);
-          tc_commit(dp_full);
+        for (int t = T; ok && t <= last; ++t) {
+          const int row = start + (kt.i_lo + t - T) * p.P;
+          if (!mbar_wait(bar.q_empty(t), (uint32_t(t / 3) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+          uint64_t* qb = clean && t == last ? bar.land(0) : bar.q_full(t);
+          mbar_expect_tx(qb, q_bytes);
+          load_q<D>(q_slot(t), &tmQ, qb, kv, row);
+          if (!mbar_wait(bar.do_empty(t), (uint32_t(t >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+          uint64_t* db = clean && t == last ? bar.land(1) : bar.do_full(t);
+          mbar_expect_tx(db, q_bytes);
+          load_q<D>(do_slot(t), &tmDO, db, kv, row);
         }
-        for (int t = 0; t < n_tiles && ok; ++t) {
-          const bool more = t + 1 < n_tiles;
-          const uint32_t sq = sq0 + uint32_t(t % 3) * L::TILE, sdo = sdo0 + uint32_t(t & 1) * L::TILE;
-          // dV(t) reads P^T(t) from the S^T tile; S^T(t+1) is issued after it and may then overwrite it
-          if (!mbar_wait(p_full, uint32_t(t & 1), abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          mma_sum<D>(TM_DV, TM_S, TM_S + 64, sdo, t > 0);
-          tc_commit(&do_empty[t & 1]);
-          if (more) {
-            if (!mbar_wait(&q_full[(t + 1) % 3], uint32_t((t + 1) / 3) & 1u, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            mma_scores<D>(TM_S, sk, sq0 + uint32_t((t + 1) % 3) * L::TILE);
-            tc_commit(s_full);
-          }
-          if (!mbar_wait(ds_full, uint32_t(t & 1), abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          mma_sum<D>(TM_DK, TM_DP, TM_DP + 64, sq, t > 0);
-          tc_commit(&q_empty[t % 3]);
-          if (more) {
-            if (!mbar_wait(&do_full[(t + 1) & 1], uint32_t((t + 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            mma_scores<D>(TM_DP, sv, sdo0 + uint32_t((t + 1) & 1) * L::TILE);
-            tc_commit(dp_full);
-          }
-        }
-        if (ok) tc_commit(done);
       }
-    } else {
-      const int sw = warp - 2;
-      const int q = warp & 3;
-      const int hf = sw >> 2;              // query-column half of the tile owned by this warp
-      const int r = q * 32 + lane;         // key row inside the tile
-      const int key = n0 + r;
-      const int tid = threadIdx.x - 64;    // 0..255
-      const uint32_t lane_addr = uint32_t(q * 32) << 16;
-      const float c = p.scale * LOG2E;
-      const int col = tid & 127, col_at = col / p.G, col_head = kv * p.G + (col - col_at * p.G);
-      auto load_stat = [&](int t) -> float {   // tid < 128: lse2 of column tid of tile t; else delta of column tid-128
-        const int pos = (i_lo + t) * p.P + col_at;
-        if (t >= n_tiles || col_at >= p.P || pos >= len) return (tid < 128) ? INFINITY : 0.f;
-        const long long at = (long long)(start + pos) * H + col_head;
-        return (tid < 128) ? p.lse[at] * LOG2E : p.delta[at];
-      };
-      (tid < 128 ? stat_lse : stat_dl)[col] = load_stat(0);
-      const int last_pos = min(key + min(p.window, len - 1 - n0), len - 1);      // last query that sees this key
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (clean && ok) {
+        ok = wait_warp(bar.land(0), uint32_t(cleaned) & 1u, abort_flag);
+        if (ok) clean_tile<D>(q_slot(last), kt.live, used, bar.q_full(last), lane);
+        ok = ok && wait_warp(bar.land(1), uint32_t(cleaned) & 1u, abort_flag);
+        if (ok) clean_tile<D>(do_slot(last), kt.live, used, bar.do_full(last), lane);
+        ++cleaned;
+      }
+      T = last + 1;
+      ++n;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t sk = smem_u32(smem + L::RES0), sv = smem_u32(smem + L::RES1);
+      const uint32_t sq0 = smem_u32(smem + L::RING3), sdo0 = smem_u32(smem + L::RING2);
       bool ok = true;
-      for (int t = 0; t < n_tiles; ++t) {
-        const int q0 = (i_lo + t) * p.P;             // first position of the tile
-        const int buf = t & 1;
-        named_bar_sync(1, 256);                    // statistics of tile t are visible to all softmax warps
-        const float next_stat = load_stat(t + 1);  // in flight while this tile is processed
+      auto issue_s = [&](int T) {
+        ok = ok && mbar_wait(bar.q_full(T), uint32_t(T / 3) & 1u, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+        mma_scores<D>(TM_S, sk, sq0 + uint32_t(T % 3) * L::TILE);
+        tc_commit(bar.s_full());
+      };
+      auto issue_dp = [&](int T) {
+        ok = ok && mbar_wait(bar.do_full(T), uint32_t(T >> 1) & 1u, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+        mma_scores<D>(TM_DP, sv, sdo0 + uint32_t(T & 1) * L::TILE);
+        tc_commit(bar.dp_full());
+      };
+      int T = 0;
+      for (int n = 0; ok; ++n) {
+        const PackedSlot slot = ring.take(n);
+        if (slot.len == 0) break;
+        const int n_tiles = KeyTile(p, slot.len, slot.tile).n_tiles;
+        ok = mbar_wait(bar.kv_full(), uint32_t(n) & 1u, abort_flag);
+        // behind the previous key tile's last dV and dK, which read columns of the tiles these overwrite
+        issue_s(T);
+        issue_dp(T);
+        for (int t = 0; t < n_tiles && ok; ++t, ++T) {
+          const bool more = t + 1 < n_tiles;
+          // dV(T) reads P^T(T) from the S^T tile; S^T(T+1) is issued after it and may then overwrite it.  t = 0: the eight warps
+          // announce P^T behind their epilogue of the previous key tile, so dV and dK may be overwritten
+          if (!mbar_wait(bar.p_full(), uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          mma_sum<D>(TM_DV, TM_S, TM_S + 64, sdo0 + uint32_t(T & 1) * L::TILE, t > 0);
+          tc_commit(bar.do_empty(T));
+          if (more) issue_s(T + 1);
+          if (!ok || !mbar_wait(bar.ds_full(), uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          mma_sum<D>(TM_DK, TM_DP, TM_DP + 64, sq0 + uint32_t(T % 3) * L::TILE, t > 0);
+          tc_commit(bar.q_empty(T));
+          if (more) issue_dp(T + 1);
+          else tc_commit(bar.done());
+        }
+      }
+    }
+  } else {
+    const int sw = warp - 2;
+    const int q = warp & 3;
+    const int hf = sw >> 2;              // query-column half of the tile owned by this warp
+    const int r = q * 32 + lane;         // key row inside the tile
+    const int tid = threadIdx.x - 64;    // 0..255
+    const uint32_t lane_addr = uint32_t(q * 32) << 16;
+    const float c = p.scale * LOG2E;
+    const int col = tid & 127, col_at = col / p.G, col_g = col - col_at * p.G;
+    // tid < 128: lse2 of column tid of the query tile that begins at position q0; else delta of column tid - 128
+    auto load_stat = [&](const PackedSlot& s, int q0) -> float {
+      const int pos = q0 + col_at;
+      if (s.len == 0 || col_at >= p.P || pos >= s.len) return (tid < 128) ? INFINITY : 0.f;
+      const long long at = (long long)(s.start + pos) * H + s.kv * p.G + col_g;
+      return (tid < 128) ? p.lse[at] * LOG2E : p.delta[at];
+    };
+    float* stat = tid < 128 ? stat_lse : stat_dl;
+    bool ok = true;
+    int T = 0;
+    PackedSlot slot = ring.take_warp(0, lane);
+    if (slot.len > 0) stat[col] = load_stat(slot, KeyTile(p, slot.len, slot.tile).i_lo * p.P);
+    for (int n = 0; slot.len > 0; ++n) {
+      const KeyTile kt(p, slot.len, slot.tile);
+      const int len = slot.len, n0 = kt.n0, key = n0 + r;
+      const int last_pos = min(key + min(p.window, len - 1 - n0), len - 1);      // last query that sees this key
+      for (int t = 0; t < kt.n_tiles; ++t, ++T) {
+        const int q0 = (kt.i_lo + t) * p.P;          // first position of the tile
+        const int buf = T & 1;
+        // statistics of tile T are visible to all eight warps (an mbarrier, whose wait ends, and no named barrier)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar.stat());
+        if (!wait_warp(bar.stat(), uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
+        // in flight while this tile is processed; positions past the last tile belong to nobody here
+        const float next_stat = t + 1 < kt.n_tiles ? load_stat(slot, q0 + p.P) : 0.f;
         const float4* cl = reinterpret_cast<const float4*>(stat_lse + buf * 128 + hf * 64);
         const float4* cd = reinterpret_cast<const float4*>(stat_dl + buf * 128 + hf * 64);
         float pr[64];
         // ---- phase A: P^T = exp2(S^T * c - lse2[query]) ----
-        if (ok && !mbar_wait(s_full, uint32_t(t & 1), abort_flag)) ok = false;
-        if (ok) {
+        if (!wait_warp(bar.s_full(), uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
+        {
           tc_fence_after();
           uint32_t s0[32], s1[32];
           tmem_ld64(TM_S + lane_addr + uint32_t(hf * 64), s0, s1);
@@ -907,11 +1064,11 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(p_full);
+          if (lane == 0) mbar_arrive(bar.p_full());
         }
         // ---- phase B: dS^T = P^T * (dP^T - delta[query]) ----
-        if (ok && !mbar_wait(dp_full, uint32_t(t & 1), abort_flag)) ok = false;
-        if (ok) {
+        if (!wait_warp(bar.dp_full(), uint32_t(T) & 1u, abort_flag)) { ok = false; break; }
+        {
           tc_fence_after();
           uint32_t d0[32], d1[32];
           tmem_ld64(TM_DP + lane_addr + uint32_t(hf * 64), d0, d1);
@@ -931,15 +1088,20 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(ds_full);
+          if (lane == 0) mbar_arrive(bar.ds_full());
         }
-        (tid < 128 ? stat_lse : stat_dl)[((t + 1) & 1) * 128 + col] = next_stat;
+        if (t + 1 < kt.n_tiles) stat[((T + 1) & 1) * 128 + col] = next_stat;
       }
-      if (ok && mbar_wait(done, 0, abort_flag)) {
+      if (!ok) break;
+      const PackedSlot done = slot;
+      slot = ring.take_warp(n + 1, lane);
+      const float first_stat = slot.len > 0 ? load_stat(slot, KeyTile(p, slot.len, slot.tile).i_lo * p.P) : 0.f;
+      if (!wait_warp(bar.done(), uint32_t(n) & 1u, abort_flag)) break;
+      {
         tc_fence_after();
-        const long long at = kv * D + hf * (D / 2);
-        __nv_bfloat16* dkrow = p.dk + (long long)(start + key) * p.lddk + at;
-        __nv_bfloat16* dvrow = p.dv + (long long)(start + key) * p.lddv + at;
+        const long long at = (long long)done.kv * D + hf * (D / 2);
+        __nv_bfloat16* dkrow = p.dk + (long long)(done.start + key) * p.lddk + at;
+        __nv_bfloat16* dvrow = p.dv + (long long)(done.start + key) * p.lddv + at;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
 #pragma unroll
@@ -951,48 +1113,89 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
           }
         }
       }
+      if (slot.len > 0) stat[(T & 1) * 128 + col] = first_stat;
     }
   }
-  tc_fence_before();
-  __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, ERR_ATTN_TIMEOUT);
-  if (warp == 1) { __syncwarp(); tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-// One grid for both, the longer half first (attn_wide_sm100.cu).
 template <int D>
 __global__ void __launch_bounds__(ATT_WIDE_THREADS, 1)
 attn_packed_bwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ PackedArgs p) {
+  using L = PackedBwdSmem<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {   // the swizzled tiles need 1 KB alignment; nothing has been allocated yet
     grid_wait();
     if (threadIdx.x == 0 && p.err) atomicExch(p.err, ERR_SMEM_ALIGN);
     return;
   }
-  const int key_blocks = p.n_k * p.KV;
-  if (int(blockIdx.x) < key_blocks) packed_bwd_dkv<D>(tmQ, tmK, tmV, tmDO, p, int(blockIdx.x));
-  else packed_bwd_dq<D>(tmQ, tmK, tmV, tmDO, p, int(blockIdx.x) - key_blocks);
+  BwdCta cta;
+  cta.smem = smem;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::COMMON);
+  cta.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  cta.warp = threadIdx.x >> 5;
+  cta.lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    const DkvBars<D> kb{reinterpret_cast<uint64_t*>(smem + L::BAR)};
+    const DqBars<D> qb{reinterpret_cast<uint64_t*>(smem + L::BAR_DQ)};
+    kb.init();
+    qb.init();
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(kb.ring() + i, 1); mbar_init(kb.ring() + 2 + i, 1 + 8);
+      mbar_init(qb.ring() + i, 1); mbar_init(qb.ring() + 2 + i, 1 + 8);
+    }
+    *cta.abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmDO);
+  }
+  if (cta.warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  const int used = p.P * p.G;
+  if (used < 128 && cta.warp >= 2 && cta.warp < 7) {      // rows that no copy fills, in the five slots: they are summed over as well
+    zero_rows<D>(smem + L::RING3 + (cta.warp - 2) * L::TILE, used, 128, cta.lane);
+    fence_proxy_async_smem();
+  }
+  static_assert(L::RING2 == L::RING3 + 3 * L::TILE, "the rings follow one another");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  cta.tmem = *tmem_slot;
+  grid_enter();                 // global memory is not touched above
+  packed_bwd_dkv<D>(tmQ, tmK, tmV, tmDO, p, cta);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();              // every role has left the key tiles: their shared memory and TMEM are free
+  tc_fence_after();
+  if (!*cta.abort_flag) packed_bwd_dq<D>(tmQ, tmK, tmV, tmDO, p, cta);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *cta.abort_flag && p.err) atomicExch(p.err, ERR_ATTN_TIMEOUT);
+  if (cta.warp == 1) { __syncwarp(); tc_fence_after(); tmem_dealloc(cta.tmem, 512); }
 }
 
-// delta[row, head] = sum_d dO * O in fp32: D / 8 lanes per (row, head)
+// delta[row, head] = sum_d dO * O in fp32, with the part of O that its rounding left over: dS = P (dP - delta) cancels, and the error
+// of delta would add as much to dQ and dK as the rounding of dS itself.  D / 8 lanes per (row, head).  Also starts the two lists of
+// the kernel behind it.
 template <int D>
-__global__ void __launch_bounds__(256) attn_packed_delta_k(const __nv_bfloat16* o, long long ldo, const __nv_bfloat16* d_o, long long row_do,
-                                                           long long head_do, float* delta, long long n, int H) {
+__global__ void __launch_bounds__(256) attn_packed_delta_k(const __nv_bfloat16* o, const __nv_bfloat16* o_lo, long long ldo,
+                                                           const __nv_bfloat16* d_o, long long row_do, long long head_do, float* delta, int* next,
+                                                           long long n, int H) {
   constexpr int LANES = D / 8;
   grid_enter();
+  if (blockIdx.x == 0 && threadIdx.x < 2) next[threadIdx.x] = 0;
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
   const int l = threadIdx.x % LANES;
   float acc = 0.f;
   if (i < n) {
     const long long row = i / H, head = i - row * H;
     const uint4 a = *reinterpret_cast<const uint4*>(o + row * ldo + head * D + l * 8);
+    const uint4 a2 = *reinterpret_cast<const uint4*>(o_lo + row * ldo + head * D + l * 8);
     const uint4 b = *reinterpret_cast<const uint4*>(d_o + row * row_do + head * head_do + l * 8);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {a2.x, a2.y, a2.z, a2.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 x = unpack_bf16(aw[e]), y = unpack_bf16(bw[e]);
-      acc += x.x * y.x + x.y * y.y;
+      const float2 x = unpack_bf16(aw[e]), z = unpack_bf16(cw[e]), y = unpack_bf16(bw[e]);
+      acc += (x.x + z.x) * y.x + (x.y + z.y) * y.y;
     }
   }
 #pragma unroll
@@ -1020,11 +1223,21 @@ static int check_packed(const ArbPacked& a) {
   // positions plus a window stay within 31 bits
   if (a.rows <= 0 || a.rows > PACKED_MAX_ROWS || a.KV <= 0 || a.KV > 65535 || a.G <= 0 || a.G > 128 || (a.D != 64 && a.D != 128) || a.window < 0) return -3;
   if (!a.items || bad_ptr(a.items) || a.cap_q <= 0 || a.cap_k <= 0 || (a.cap_q + a.cap_k) * a.KV > 0x7fffffffll) return -3;
-  const void* ptrs[] = {a.q, a.k, a.v, a.o, a.d_o, a.dq, a.dk, a.dv};
+  const void* ptrs[] = {a.q, a.k, a.v, a.o, a.o_lo, a.d_o, a.dq, a.dk, a.dv};
   const long long strides[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.v_row, a.v_head, a.o_row, a.do_row, a.do_head, a.dq_row, a.dk_row, a.dv_row};
   for (const void* p : ptrs) if (bad_ptr(p)) return -4;
   for (long long s : strides) if (s < 0 || (s & 7)) return -4;
   return 0;
+}
+
+static int packed_sms() {
+  static int n = 0;
+  if (!n) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  }
+  return n;
 }
 
 static PackedArgs packed_args(const ArbPacked& a, int* err) {
@@ -1051,7 +1264,10 @@ static int packed_fwd(const ArbPacked& a, int* err, cudaStream_t stream) {
   if ((r = make_key_tmap(&tv, a.v, a, a.v_row, a.v_head))) return 1000 + r;
   PackedArgs p = packed_args(a, err);
   p.o = reinterpret_cast<__nv_bfloat16*>(a.o); p.ldo = a.o_row;
-  return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(a.cap_q * a.KV), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk, tv, p);
+  p.o_lo = reinterpret_cast<__nv_bfloat16*>(a.o_lo);
+  const long long tiles = a.cap_q * a.KV, ctas = 2ll * packed_sms();
+  return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(tiles < ctas ? tiles : ctas), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk,
+                          tv, p);
 }
 
 template <int D>
@@ -1067,16 +1283,19 @@ static int packed_bwd(const ArbPacked& a, int* err, cudaStream_t stream) {
   const int H = int(a.KV * a.G);
   const long long n = a.rows * H, blocks = (n * (D / 8) + 255) / 256;
   if (blocks > 0x7fffffffll) return -3;
+  int* next = reinterpret_cast<int*>(a.delta + n);
   if ((r = launch_dependent(n * D * 2 <= EARLY_BYTES, attn_packed_delta_k<D>, unsigned(blocks), 256, 0, stream,
-                            reinterpret_cast<const __nv_bfloat16*>(a.o), a.o_row, reinterpret_cast<const __nv_bfloat16*>(a.d_o), a.do_row,
-                            a.do_head, a.delta, n, H)))
+                            reinterpret_cast<const __nv_bfloat16*>(a.o), reinterpret_cast<const __nv_bfloat16*>(a.o_lo), a.o_row,
+                            reinterpret_cast<const __nv_bfloat16*>(a.d_o), a.do_row, a.do_head, a.delta, next, n, H)))
     return r;
   PackedArgs p = packed_args(a, err);
   p.o = reinterpret_cast<__nv_bfloat16*>(a.dq); p.ldo = a.dq_row;
   p.dk = reinterpret_cast<__nv_bfloat16*>(a.dk); p.lddk = a.dk_row;
   p.dv = reinterpret_cast<__nv_bfloat16*>(a.dv); p.lddv = a.dv_row;
-  return launch_dependent(true, attn_packed_bwd_k<D>, unsigned((a.cap_q + a.cap_k) * a.KV), ATT_WIDE_THREADS, PackedBwdSmem<D>::TOTAL, stream,
-                          tq, tk, tv, tdo, p);
+  p.next = next;
+  const long long most = (a.cap_q > a.cap_k ? a.cap_q : a.cap_k) * a.KV, ctas = packed_sms();
+  return launch_dependent(true, attn_packed_bwd_k<D>, unsigned(most < ctas ? most : ctas), ATT_WIDE_THREADS, PackedBwdSmem<D>::TOTAL, stream, tq, tk,
+                          tv, tdo, p);
 }
 
 }  // namespace arb
@@ -1107,7 +1326,7 @@ extern "C" int arb_packed_attn_fwd(const ArbPacked* a, int* err_flag, cudaStream
 }
 
 extern "C" int arb_packed_attn_bwd(const ArbPacked* a, int* err_flag, cudaStream_t stream) {
-  if (!a || !a->q || !a->k || !a->v || !a->o || !a->lse || !a->d_o || !a->delta || !a->dq || !a->dk || !a->dv) return -3;
+  if (!a || !a->q || !a->k || !a->v || !a->o || !a->o_lo || !a->lse || !a->d_o || !a->delta || !a->dq || !a->dk || !a->dv) return -3;
   if (int r = check_packed(*a)) return r;
   return a->D == 64 ? packed_bwd<64>(*a, err_flag, stream) : packed_bwd<128>(*a, err_flag, stream);
 }

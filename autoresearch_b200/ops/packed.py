@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 
-_ARGS = struct.Struct("=30qd")          # ArbPacked of csrc/api.h: 11 pointers, 7 sizes, 12 strides, the scale
+_ARGS = struct.Struct("=31qd")          # ArbPacked of csrc/api.h: 12 pointers, 7 sizes, 12 strides, the scale
 MAX_ROWS = 1 << 30
 L2_SPAN_BYTES = 48 << 20                # keys and values whose tiles run together (126 MB of L2; attn_common.cuh)
 
@@ -97,27 +97,28 @@ def _layout(t: torch.Tensor):
     return t.clone(memory_format=torch.contiguous_format), n1 * d, d
 
 
-def _forward(q, k, v, strides, seqs, window, scale):
-    """(O, lse).  ``strides``: row and head stride of q, k and v."""
+def _forward(q, k, v, strides, seqs, window, scale, keep):
+    """(O, lse, what O's rounding left over where ``keep``).  ``strides``: row and head stride of q, k and v."""
     rows, H, d = q.shape
     out = q.new_empty((rows, H, d))
+    rest = q.new_empty((rows, H, d)) if keep else None
     lse = q.new_empty((rows, H), dtype=torch.float32)
     if rows:
-        args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, seqs._items_ptr, rows,
-                          seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k, *strides, H * d, 0, 0, 0, 0, 0, scale)
+        args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr() if keep else 0, lse.data_ptr(),
+                          0, 0, 0, 0, 0, seqs._items_ptr, rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k, *strides, H * d, 0, 0, 0, 0, 0, scale)
         with K.on_device(seqs.device):
             K._check(K.lib().arb_packed_attn_fwd(args, seqs._err_ptr, K._stream()), "packed_attn_fwd")
-    return out, lse
+    return out, lse, rest
 
 
-def _backward(q, k, v, out, lse, d_out, dq, dk, dv, strides, row_strides, seqs, window, scale):
+def _backward(q, k, v, out, rest, lse, d_out, dq, dk, dv, strides, row_strides, seqs, window, scale):
     """``row_strides``: those of dq, dk and dv, whose heads are d apart."""
     rows, H, d = q.shape
     if not rows:
         return
     d_out, do_row, do_head = _layout(d_out)
-    delta = lse.new_empty(lse.shape)
-    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), d_out.data_ptr(), delta.data_ptr(),
+    delta = lse.new_empty(rows * H + 2)
+    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), d_out.data_ptr(), delta.data_ptr(),
                       dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), seqs._items_ptr, rows, seqs.n_kv_head, seqs.group, d, window,
                       seqs.cap_q, seqs.cap_k, *strides, H * d, do_row, do_head, *row_strides, scale)
     with K.on_device(seqs.device):
@@ -129,11 +130,11 @@ class PackedAttentionFn(torch.autograd.Function):
     """q [rows, H, d], k and v [rows, KV, d] -> [rows, H, d]."""
 
     @staticmethod
-    def forward(ctx, q, k, v, seqs, window, scale):
+    def forward(ctx, q, k, v, seqs, window, scale, keep):
         (q, q0, q1), (k, k0, k1), (v, v0, v1) = _layout(q), _layout(k), _layout(v)
         strides = (q0, q1, k0, k1, v0, v1)
-        out, lse = _forward(q, k, v, strides, seqs, window, scale)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, lse, rest = _forward(q, k, v, strides, seqs, window, scale, keep)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
         ctx.args = (seqs, window, scale)
         ctx.strides = strides
         return out
@@ -141,34 +142,34 @@ class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
         d = q.shape[2]
         rows = (q.shape[1] * d, k.shape[1] * d, k.shape[1] * d)
-        _backward(q, k, v, out, lse, d_out, dq, dk, dv, ctx.strides, rows, *ctx.args)
-        return dq, dk, dv, None, None, None
+        _backward(q, k, v, out, rest, lse, d_out, dq, dk, dv, ctx.strides, rows, *ctx.args)
+        return dq, dk, dv, None, None, None, None
 
 
 class PackedQKVAttentionFn(torch.autograd.Function):
     """The same on the packed projection output [rows, (H + 2 KV) d]; its gradient is written in place of three tensors."""
 
     @staticmethod
-    def forward(ctx, qkv, seqs, window, scale, d):
+    def forward(ctx, qkv, seqs, window, scale, d, keep):
         ld = qkv.shape[1]
         ctx.args, ctx.d, ctx.strides = (seqs, window, scale), d, (ld, d) * 3
-        out, lse = _forward(*_blocks(qkv, seqs, d), ctx.strides, seqs, window, scale)
-        ctx.save_for_backward(qkv, out, lse)
+        out, lse, rest = _forward(*_blocks(qkv, seqs, d), ctx.strides, seqs, window, scale, keep)
+        ctx.save_for_backward(qkv, out, rest, lse)
         return out.view(qkv.shape[0], -1)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        qkv, out, lse = ctx.saved_tensors
+        qkv, out, rest, lse = ctx.saved_tensors
         seqs = ctx.args[0]
         d_qkv = qkv.new_empty(qkv.shape)
-        _backward(*_blocks(qkv, seqs, ctx.d), out, lse, d_out.contiguous().view(out.shape), *_blocks(d_qkv, seqs, ctx.d), ctx.strides,
+        _backward(*_blocks(qkv, seqs, ctx.d), out, rest, lse, d_out.contiguous().view(out.shape), *_blocks(d_qkv, seqs, ctx.d), ctx.strides,
                   (qkv.shape[1],) * 3, *ctx.args)
-        return d_qkv, None, None, None, None
+        return d_qkv, None, None, None, None, None
 
 
 def _blocks(qkv, seqs, d):
@@ -208,7 +209,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: Pa
                          f"{seqs.n_kv_head} key heads")
     if k.device != q.device or v.device != q.device:
         raise ValueError("q, k and v must be on one device")
-    return PackedAttentionFn.apply(q, k, v, seqs, window, scale)
+    keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return PackedAttentionFn.apply(q, k, v, seqs, window, scale, keep)
 
 
 def packed_qkv_attention(qkv: torch.Tensor, seqs: PackedSequences, window: Optional[int] = None, scale: Optional[float] = None,
@@ -221,4 +223,4 @@ def packed_qkv_attention(qkv: torch.Tensor, seqs: PackedSequences, window: Optio
     window, scale = _common(qkv.device, rows, head_dim, seqs, window, scale)
     if qkv.shape[1] != (seqs.n_head + 2 * seqs.n_kv_head) * head_dim:
         raise ValueError(f"qkv has {qkv.shape[1]} columns for {seqs.n_head} + 2 x {seqs.n_kv_head} heads of {head_dim}")
-    return PackedQKVAttentionFn.apply(qkv, seqs, window, scale, head_dim)
+    return PackedQKVAttentionFn.apply(qkv, seqs, window, scale, head_dim, torch.is_grad_enabled() and qkv.requires_grad)

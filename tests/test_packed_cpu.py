@@ -59,7 +59,7 @@ def test_argument_block_matches_the_header():
     text = (Path(K.__file__).parent / "csrc" / "api.h").read_text()
     body = re.sub(r"//[^\n]*", "", text[text.index("typedef struct ArbPacked"):text.index("} ArbPacked;")])
     fields = [f for line in body[body.index("{") + 1:].split(";") for f in line.split(",") if f.strip()]
-    assert len(fields) == 31 and P._ARGS.size == 8 * len(fields)
+    assert len(fields) == 32 and P._ARGS.size == 8 * len(fields)
 
 
 def test_backward_formula_against_differences():
