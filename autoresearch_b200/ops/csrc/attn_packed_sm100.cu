@@ -344,14 +344,17 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* p_full = bars + 4;        // [2] P(T) of keys 64..127, then of keys 0..63, written (4 arrivals)
   uint64_t* pv_done = bars + 6;       // P V(T) complete: V slot free, behind the last one O is final
   uint64_t* v_land = bars + 7;        // a V tile that has to be cleaned has landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  uint64_t* next_full = bars + 12;    // which block to take over has been answered
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   SlotRing ring{bars + 8, bars + 10, reinterpret_cast<PackedSlot*>(bars + 14), abort_flag};
+  uint4* next_block = reinterpret_cast<uint4*>(bars + 18);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1); mbar_init(k_full, 1); mbar_init(v_full, 1);
     mbar_init(s_full, 1); mbar_init(&p_full[0], 4); mbar_init(&p_full[1], 4); mbar_init(pv_done, 1); mbar_init(v_land, 1);
+    mbar_init(next_full, 1);
     ring.init(1 + 4);
     *abort_flag = 0;
     fence_barrier_init();
@@ -367,49 +370,64 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   if (warp == 0) {
     if (lane == 0) { tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
-    const int total = p.n_q * p.KV, width = int(gridDim.x);
     int T = 0, n = 0, cleaned = 0;
-    bool ok = true;
-    // rounds over the list in turn from either end of the grid, so that every CTA gets long and short tiles
-    for (int round = 0; ok; ++round) {
-      const int i = round * width + ((round & 1) ? width - 1 - int(blockIdx.x) : int(blockIdx.x));
-      if (round * width >= total) break;
-      if (i >= total) continue;
+    bool ok = true, more = true;
+    // the grid has a block for every tile; one that runs takes over those that have not started, longest tiles first
+    for (int i = int(blockIdx.x), k = 0; ok && more; ++k) {
+      // asked for behind the tile's last loads: whoever asks early takes a second tile while others run out of them
+      auto request = [&]() {
+        if (lane == 0) {
+          mbar_expect_tx(next_full, 16);
+          take_block_request(next_block + (k & 1), next_full);
+        }
+      };
       const PackedTile tile = packed_tile(p, p.items_q, p.n_q, i);
       const int start = tile.it.start, len = tile.it.len, kv = tile.kv;
-      if (len == 0) continue;
-      if (tile.it.tile < 0) {                            // rows of no sequence
+      if (len <= 0) {
+        request();
+      } else if (tile.it.tile < 0) {                     // rows of no sequence
+        request();
         zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D, lane);
         if (p.o_lo) zero_out(p.o_lo + (long long)kv * p.G * D, p.ldo, start, len, p.G * D, lane);
         for (int e = lane; e < len * p.G; e += 32) p.lse[(long long)(start + e / p.G) * H + kv * p.G + e % p.G] = -INFINITY;
-        continue;
-      }
-      const QueryTile qt(p, len, tile.it.tile);
-      const bool clean = qt.live < 128;
-      if (lane == 0) {
-        ok = ring.put(n, tile);
-        for (int t = 0; ok && t < qt.n_tiles; ++t, ++T) {
-          const int row = start + (qt.j_lo + t) * 128;
-          if (T > 0 && !mbar_wait(s_full, uint32_t(T - 1) & 1u, abort_flag)) { ok = false; break; }
-          if (t == 0) {
-            mbar_expect_tx(q_full, uint32_t(p.P * p.G * D * 2));          // rows past the end of the tensor are zero-filled
-            load_q<D>(smem + L::Q, &tmQ, q_full, kv, start + qt.m0);
+      } else {
+        const QueryTile qt(p, len, tile.it.tile);
+        const bool clean = qt.live < 128;
+        if (lane == 0) {
+          ok = ring.put(n, tile);
+          for (int t = 0; ok && t < qt.n_tiles; ++t, ++T) {
+            const int row = start + (qt.j_lo + t) * 128;
+            if (T > 0 && !mbar_wait(s_full, uint32_t(T - 1) & 1u, abort_flag)) { ok = false; break; }
+            if (t == 0) {
+              mbar_expect_tx(q_full, uint32_t(p.P * p.G * D * 2));          // rows past the end of the tensor are zero-filled
+              load_q<D>(smem + L::Q, &tmQ, q_full, kv, start + qt.m0);
+            }
+            mbar_expect_tx(k_full, L::TILE);
+            load_kv<D>(smem + L::K, &tmK, k_full, kv, row);
+            if (T > 0 && !mbar_wait(pv_done, uint32_t(T - 1) & 1u, abort_flag)) { ok = false; break; }
+            uint64_t* bar = (clean && t == qt.n_tiles - 1) ? v_land : v_full;
+            mbar_expect_tx(bar, L::TILE);
+            load_kv<D>(smem + L::V, &tmV, bar, kv, row);
           }
-          mbar_expect_tx(k_full, L::TILE);
-          load_kv<D>(smem + L::K, &tmK, k_full, kv, row);
-          if (T > 0 && !mbar_wait(pv_done, uint32_t(T - 1) & 1u, abort_flag)) { ok = false; break; }
-          uint64_t* bar = (clean && t == qt.n_tiles - 1) ? v_land : v_full;
-          mbar_expect_tx(bar, L::TILE);
-          load_kv<D>(smem + L::V, &tmV, bar, kv, row);
         }
+        request();
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (clean && ok) {
+          ok = wait_warp(v_land, uint32_t(cleaned) & 1u, abort_flag);
+          ++cleaned;
+          if (ok) clean_tile<D>(smem + L::V, qt.live, 128, v_full, lane);
+        }
+        ++n;
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      if (clean && ok) {
-        ok = wait_warp(v_land, uint32_t(cleaned) & 1u, abort_flag);
-        ++cleaned;
-        if (ok) clean_tile<D>(smem + L::V, qt.live, 128, v_full, lane);
-      }
-      ++n;
+      // every request is answered before the block ends
+      uint32_t x = 0;
+      const bool answered = wait_warp(next_full, uint32_t(k) & 1u, abort_flag);
+      for (uint32_t spin = 0; !answered && spin < 65536 && !mbar_try_wait(next_full, uint32_t(k) & 1u); ++spin) {}
+      more = answered && take_block_answer(next_block + (k & 1), x);
+      i = int(x);
+      fence_proxy_async_smem();                          // the answer has been read before the request after the next overwrites it
+      __syncwarp();
+      ok = ok && answered;
     }
     if (ok && lane == 0) ring.put(n, PackedTile{PackedItem{0, 0, 0, 0}, 0});
   } else if (warp == 1) {
@@ -1265,9 +1283,7 @@ static int packed_fwd(const ArbPacked& a, int* err, cudaStream_t stream) {
   PackedArgs p = packed_args(a, err);
   p.o = reinterpret_cast<__nv_bfloat16*>(a.o); p.ldo = a.o_row;
   p.o_lo = reinterpret_cast<__nv_bfloat16*>(a.o_lo);
-  const long long tiles = a.cap_q * a.KV, ctas = 2ll * packed_sms();
-  return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(tiles < ctas ? tiles : ctas), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk,
-                          tv, p);
+  return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(a.cap_q * a.KV), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk, tv, p);
 }
 
 template <int D>

@@ -101,6 +101,28 @@ inline int launch_dependent(bool early, void (*kern)(Formal...), dim3 grid, dim3
   return launch_status(cudaLaunchKernelEx(&cfg, kern, static_cast<Formal>(args)...));
 }
 
+// ---- taking over a block of this grid that has not started yet ---------------------------------------
+// The response (16 bytes, 16-byte aligned) lands in shared memory and completes 16 bytes on `bar`.  No further request after one that
+// found nothing.
+__device__ __forceinline__ void take_block_request(void* response, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(response)), "r"(smem_u32(bar)) : "memory");
+}
+// whether a block was taken, and its index in x
+__device__ __forceinline__ bool take_block_answer(const void* response, uint32_t& x) {
+  uint32_t got, bx;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(bx) : "r"(smem_u32(response)) : "memory");
+  x = bx;
+  return got != 0;
+}
+
 // ---- TMA -------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
