@@ -288,16 +288,6 @@ __device__ __forceinline__ void store32(__nv_bfloat16* dst, const uint32_t (&v)[
     *reinterpret_cast<uint4*>(dst + j) = u;
   }
 }
-// ... and what that rounding leaves over, rounded in turn
-__device__ __forceinline__ void store32_rest(__nv_bfloat16* dst, const uint32_t (&v)[32], float s) {
-  uint32_t rest[32];
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float x = __uint_as_float(v[j]) * s;
-    rest[j] = __float_as_uint(x - __bfloat162float(__float2bfloat16(x)));
-  }
-  store32(dst, rest, 1.f);
-}
 // `n` rows from `row` of `width` elements each, zero, by a warp
 __device__ __forceinline__ void zero_out(__nv_bfloat16* dst, long long ld, int row, int n, int width, int lane) {
   const int per = width / 8;
@@ -312,10 +302,28 @@ template <int D>
 struct PackedFwdSmem {
   static constexpr int TILE = 128 * D * 2;
   static constexpr int Q = 0, K = TILE, V = 2 * TILE;
-  static constexpr int BAR = 3 * TILE;
-  static constexpr int TOTAL = BAR + 192 + 1024;         // + alignment slack
+  static constexpr int OUT = 3 * TILE;                   // 4 KB for each of the four epilogue warps
+  static constexpr int BAR = OUT + 16384;
+  static constexpr int TOTAL = BAR + 192;
 };
 static_assert(2 * (PackedFwdSmem<128>::TOTAL + 1024) <= 233472, "two CTAs must fit the 228 KB of an SM");
+
+// 32 rows of 64 bf16 columns, a row in each lane (32 words), to rows `off` elements from `dst` (off < 0: not written).  Through 4 KB of
+// shared memory of the warp's own, so that eight lanes write 128 adjacent bytes and not each 16 bytes of another row (32768 rows,
+// window 256, 8 heads on 4, both parts of O: 131 -> 121 us).
+__device__ __forceinline__ void store_rows(__nv_bfloat16* dst, long long off, const uint32_t (&w)[32], uint32_t stage, int lane) {
+  __syncwarp();                                          // the previous use has been read
+#pragma unroll
+  for (int j = 0; j < 8; ++j) st_sw128(stage, 32, lane, j * 8, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = i * 4 + (lane >> 3), col = (lane & 7) * 8;
+    const long long o = __shfl_sync(0xffffffffu, off, row);
+    const uint4 u = ld_sw128(stage, 32, row, col);
+    if (o >= 0) *reinterpret_cast<uint4*>(dst + o + col) = u;
+  }
+}
 
 // positions and key tiles of a query tile
 struct QueryTile {
@@ -334,8 +342,12 @@ __global__ void __launch_bounds__(ATT_THREADS, 2)
 attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const PackedArgs p) {
   using L = PackedFwdSmem<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {   // the swizzled tiles need 1 KB alignment; nothing has been allocated yet
+    grid_wait();
+    if (threadIdx.x == 0 && p.err) atomicExch(p.err, ERR_SMEM_ALIGN);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* q_full = bars;            // Q of the n-th query tile
   uint64_t* k_full = bars + 1;        // below, T counts the key tiles of all query tiles
@@ -579,16 +591,26 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_after();
       const float inv_l = (l > 0.f) ? 1.f / l : 0.f;
       const int head = slot.kv * p.G + (r - at * p.G);
-      const long long row = (long long)(slot.start + pos) * p.ldo + (long long)head * D;
+      const long long off = live_row ? (long long)(slot.start + pos) * p.ldo + (long long)head * D : -1;
+      const uint32_t stage = smem_u32(smem + L::OUT) + uint32_t(q) * 4096u;
+#pragma unroll 1
+      for (int cc = 0; cc < D; cc += 64) {
+        uint32_t v[32], w[32], rest[32];
 #pragma unroll
-      for (int cc = 0; cc < D / 32; ++cc) {
-        uint32_t v[32];
-        tmem_ld32(TM_O + lane_addr + uint32_t(cc * 32), v);
-        tmem_wait_ld();
-        if (live_row) {
-          store32(p.o + row + cc * 32, v, inv_l);
-          if (p.o_lo) store32_rest(p.o_lo + row + cc * 32, v, inv_l);
+        for (int hf = 0; hf < 2; ++hf) {
+          tmem_ld32(TM_O + lane_addr + uint32_t(cc + hf * 32), v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float x = __uint_as_float(v[2 * j]) * inv_l, y = __uint_as_float(v[2 * j + 1]) * inv_l;
+            const uint32_t u = pack_bf16(x, y);
+            const float2 r2 = unpack_bf16(u);
+            w[hf * 16 + j] = u;
+            rest[hf * 16 + j] = pack_bf16(x - r2.x, y - r2.y);
+          }
         }
+        store_rows(p.o + cc, off, w, stage, lane);
+        if (p.o_lo) store_rows(p.o_lo + cc, off, rest, stage, lane);
       }
       if (live_row) p.lse[(long long)(slot.start + pos) * H + head] = (l > 0.f) ? (m_used * p.scale + __logf(l)) : -INFINITY;
     }
@@ -707,7 +729,8 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
       const int last = T + qt.n_tiles - 1;
       if (lane == 0) {
         ok = ring.put(n, tile);
-        // Q and dO are free behind the last S and dP of the previous query tile
+        // Q and dO are free behind the last S and dP of the previous query tile (dP of T-3, the phase before on this barrier, was waited
+        // for when V's slot was taken for T-1)
         if (ok && T > 0) ok = mbar_wait(bar.dp_full(T - 1), uint32_t((T - 1) >> 1) & 1u, abort_flag);
         if (ok) {
           mbar_expect_tx(bar.q_full(), 2 * q_bytes);
@@ -890,10 +913,13 @@ struct DkvBars {
   __device__ __forceinline__ uint64_t* done() const { return b + 15; }          // dK and dV of the n-th key tile complete
   __device__ __forceinline__ uint64_t* land(int i) const { return b + 16 + i; } // Q / dO tile that has to be cleaned has landed
   __device__ __forceinline__ uint64_t* stat() const { return b + 18; }          // statistics of query tile T written (8 arrivals)
-  __device__ __forceinline__ uint64_t* ring() const { return b + 19; }          // 4
-  static constexpr int COUNT = 23;
+  // all S^T and dP^T of the n-th key tile complete.  (dp_full would say so too, but a parity tells a phase only from the one before and
+  // the one behind it: who waits for a barrier visits all of its phases, which the loading warp does not with dp_full's.)
+  __device__ __forceinline__ uint64_t* kv_free() const { return b + 19; }
+  __device__ __forceinline__ uint64_t* ring() const { return b + 20; }          // 4
+  static constexpr int COUNT = 24;
   __device__ __forceinline__ void init() const {
-    for (int i = 0; i < 19; ++i) mbar_init(b + i, i == 12 || i == 14 || i == 18 ? 8 : 1);
+    for (int i = 0; i < 20; ++i) mbar_init(b + i, i == 12 || i == 14 || i == 18 ? 8 : 1);
   }
 };
 static_assert(DkvBars<64>::COUNT * 8 + 2 * sizeof(PackedSlot) <= 256, "barrier space");
@@ -945,8 +971,7 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
       const int last = T + kt.n_tiles - 1;
       if (lane == 0) {
         ok = ring.put(n, tile);
-        // K and V are free behind the last S^T and dP^T of the previous key tile
-        if (ok && T > 0) ok = mbar_wait(bar.dp_full(), uint32_t(T - 1) & 1u, abort_flag);
+        if (ok && n > 0) ok = mbar_wait(bar.kv_free(), uint32_t(n - 1) & 1u, abort_flag);
         if (ok) {
           mbar_expect_tx(bar.kv_full(), 2 * L::TILE);
           load_kv<D>(smem + L::RES0, &tmK, bar.kv_full(), kv, start + kt.n0);
@@ -1003,6 +1028,7 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
         // behind the previous key tile's last dV and dK, which read columns of the tiles these overwrite
         issue_s(T);
         issue_dp(T);
+        if (ok && n_tiles == 1) tc_commit(bar.kv_free());
         for (int t = 0; t < n_tiles && ok; ++t, ++T) {
           const bool more = t + 1 < n_tiles;
           // dV(T) reads P^T(T) from the S^T tile; S^T(T+1) is issued after it and may then overwrite it.  t = 0: the eight warps
@@ -1018,6 +1044,7 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
           tc_commit(bar.q_empty(T));
           if (more) issue_dp(T + 1);
           else tc_commit(bar.done());
+          if (ok && t + 2 == n_tiles) tc_commit(bar.kv_free());
         }
       }
     }

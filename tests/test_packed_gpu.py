@@ -157,6 +157,21 @@ def test_many_short_sequences():
     _check([1, 2, 3, 4, 5, 6, 7] * 60, 4, 4, 128)
 
 
+@pytest.mark.parametrize("n", [200, 256, 384, 520])
+def test_many_sequences_of_a_few_tiles(n):
+    """Blocks that take many tiles of two to five steps each, without a pause between them: every sequence comes out as it does
+    alone, three times over."""
+    from autoresearch_b200.ops.packed import PackedSequences
+    many, H, KV, d = 400, 2, 1, 128
+    one = _inputs(n, H, KV, d)
+    alone = _run(*one, PackedSequences([0, n], n, H, KV))
+    all_ = [t.repeat(many, 1, 1) for t in one]
+    seqs = PackedSequences([i * n for i in range(many + 1)], many * n, H, KV)
+    for _ in range(3):
+        for x, y in zip(_run(*all_, seqs), alone):
+            assert torch.equal(x, y.repeat(many, 1, 1))
+
+
 def test_scale_is_the_callers():
     _check([400], 2, 1, 128, scale=0.02)
 
