@@ -7,6 +7,8 @@ positional ``train``; unknown flags are ignored like there.  ``--max-steps`` bea
 Environment: ``SYNTHETIC MAX_STEPS COOLDOWN_STEPS BATCH_SIZE NUM_TRAIN_SHARDS TOTAL_BATCH PEAK_LR
 WARMDOWN_RATIO WARMUP_RATIO WEIGHT_DECAY SCHEDULE FINAL_LR_FRAC CHECKPOINT_DIR EVAL_EVERY
 CHECKPOINT_EVERY INIT_WEIGHTS_PATH PIPELINE_RANK PIPELINE_WORLD_SIZE``.
+Of this package: ``GRAD_CLIP`` (largest 2-norm of all gradients, one GPU), ``DOC_BOS`` (id of the token that begins a document:
+attention stays inside of documents), ``VOCAB_PIECES=1`` (the head's loss without logits in memory).
 
 Additions (the reference fixes these at compile time): ``--model PRESET`` (or ``MODEL``),
 ``--impl oracle|baseline|sm100|auto``, ``--synthetic-kind lcg|zipf``, ``--comm fused|nccl``,

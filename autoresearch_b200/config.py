@@ -261,6 +261,9 @@ class TrainConfig:
     metrics_jsonl: Optional[str] = None
     resume: bool = False
     heartbeat_timeout_s: float = 0.0  # > 0: watch peer liveness through the process group's store
+    grad_clip: float = 0.0  # > 0: all gradients together are scaled to at most this 2-norm before the optimizer step (one GPU)
+    doc_bos: Optional[int] = None  # token id that begins a document: attention stays inside of documents (data parallel only)
+    vocab_pieces: bool = False  # the head's loss in pieces of the vocabulary, without logits in memory
     peak_flops: Optional[float] = None  # MFU denominator per GPU; None = ARB_PEAK_TFLOPS or the nominal B200 peak
     parallel: ParallelConfig = field(default_factory=ParallelConfig)
 
@@ -290,6 +293,9 @@ class TrainConfig:
             num_train_shards=(i("NUM_TRAIN_SHARDS", -1) if i("NUM_TRAIN_SHARDS", -1) >= 0 else None),
             synthetic_data=env.get("SYNTHETIC", "") in ("1", "true"),
             heartbeat_timeout_s=float(env.get("HEARTBEAT_TIMEOUT", "0") or 0),
+            grad_clip=float(env.get("GRAD_CLIP", "0") or 0),
+            doc_bos=(i("DOC_BOS", -1) if i("DOC_BOS", -1) >= 0 else None),
+            vocab_pieces=env.get("VOCAB_PIECES", "") in ("1", "true"),
             schedule_cfg=ScheduleConfig.from_env(env),
         )
 

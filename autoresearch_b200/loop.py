@@ -50,11 +50,17 @@ class TrainerBase:
     accum: int = 1
     log_rank: int = 0        # the rank that prints and writes the metrics file
     impl: str = "oracle"
+    clips_gradients: bool = False    # whether this trainer sees all gradients before the optimizer step
+    masks_documents: bool = False    # whether its attention can stay inside of documents
 
     # -------------------------------------------------------------------------------------------
     def _init_common(self) -> None:
         t, m = self.tcfg, self.mcfg
         on_gpu = self.device.type == "cuda"
+        if not t.grad_clip >= 0.0 or (t.grad_clip > 0.0 and not self.clips_gradients):
+            raise ValueError(f"grad_clip={t.grad_clip}: a norm that is not negative, in training on one GPU")
+        if t.doc_bos is not None and not self.masks_documents:
+            raise ValueError("doc_bos: attention inside of documents needs the data-parallel trainer")
         self.step = 0
         self.loss_ema = 0.0
         self.ema_steps = 0
@@ -148,6 +154,10 @@ class TrainerBase:
         if got is None:
             return None
         slot, h_ids, h_tgt = got
+        self._documents = None
+        if self.tcfg.doc_bos is not None:
+            from .ops.packed import document_bounds
+            self._documents = document_bounds(h_ids, self.tcfg.doc_bos)      # on the host, before the slot goes back
         d_ids, d_tgt = self._d[micro & 1]
         d_ids.copy_(h_ids, non_blocking=True)
         d_tgt.copy_(h_tgt, non_blocking=True)

@@ -104,11 +104,14 @@ class GPT(nn.Module):
         return be.rmsnorm(emb)
 
     def run_layers(self, x: torch.Tensor, x0: torch.Tensor, ids: torch.Tensor,
-                   B: int, T: int) -> torch.Tensor:
+                   B: int, T: int, seqs=None) -> torch.Tensor:
         cfg, be = self.cfg, self.backend
         ids_flat = ids.reshape(-1)
         aux_total = None
         whole_layer, first_half = getattr(be, "dense_layer", None), getattr(be, "attention_half", None)
+        docs = {} if seqs is None else dict(seqs=seqs)
+        if docs:
+            whole_layer = first_half = None          # the native layer calls attend over whole rows
         for bi, blk in enumerate(self.blocks):
             l = blk.layer
             if self.grad_bucket_cb is not None and l in self.grad_bucket_boundaries and x.requires_grad:
@@ -127,7 +130,7 @@ class GPT(nn.Module):
                 else:
                     x, xn = be.resid_scale_norm(x, x0, self.resid_lambdas, self.x0_lambdas, bi)
                     a = be.attention_block(xn, blk, ids_flat, B, T, cfg, self.rope_cos, self.rope_sin,
-                                           cfg.window(l))
+                                           cfg.window(l), **docs)
                     x, xn = be.proj_add_norm(a, blk.wo, x)
                 if blk.router is not None:
                     x, aux = be.moe_mlp_add(xn, x, blk, cfg.moe)
@@ -146,10 +149,15 @@ class GPT(nn.Module):
 
     def forward(self, ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
                 grad_scale: float = 1.0, x_in: Optional[torch.Tensor] = None,
-                x0_in: Optional[torch.Tensor] = None):
+                x0_in: Optional[torch.Tensor] = None, cu_seqlens=None):
         """ids/targets: [B, T] integer tensors.  Full model: returns
-        (scaled_loss_sum, per_token_losses).  Pipeline stage without a head: returns (x, x0)."""
+        (scaled_loss_sum, per_token_losses).  Pipeline stage without a head: returns (x, x0).
+        ``cu_seqlens``: bounds of the documents in the flattened batch, as of ``ops.packed.document_bounds``; attention then
+        stays inside of a document (positions within a row count from the row's start: rotations are relative)."""
         B, T = ids.shape
+        seqs = None
+        if cu_seqlens is not None:
+            seqs = self.backend.packed_sequences(cu_seqlens, B * T, self.cfg.n_head // self.tp)
         tp = getattr(self.backend, "tp", None)
         if tp is not None and tp.size > 1:
             # sequence parallel: this rank embeds, normalises and scores only its token shard
@@ -164,7 +172,7 @@ class GPT(nn.Module):
             x0 = x
         else:
             x, x0 = x_in, x0_in
-        x = self.run_layers(x, x0, ids, B, T)
+        x = self.run_layers(x, x0, ids, B, T, seqs)
         if not self.has_head:
             return x, x0
         scaled, per_tok = self.head_loss(x, targets, grad_scale)

@@ -71,9 +71,17 @@ class OracleBackend:
     def attention(self, q, k, v, window):
         return R.attention(q, k, v, window)
 
+    def packed_sequences(self, cu_seqlens, rows, n_head):
+        """What ``attention_block`` takes as ``seqs``: the documents of a batch, made once for all layers of a pass."""
+        from .packed import check_bounds
+        bounds = [int(b) for b in cu_seqlens]
+        check_bounds(bounds, rows)
+        return bounds
+
     # -- coarse blocks (a backend may fuse across these boundaries) ------------------
-    def attention_block(self, xn, blk, ids_flat, B, T, cfg, cos, sin, window):
-        """xn [N, D] -> attention output [N, H*hd] (before the output projection)."""
+    def attention_block(self, xn, blk, ids_flat, B, T, cfg, cos, sin, window, seqs=None):
+        """xn [N, D] -> attention output [N, H*hd] (before the output projection).  ``seqs``: the documents that attention stays
+        inside of, from ``packed_sequences``."""
         hd = cfg.head_dim
         Dl = blk.wqkv.shape[0] // 3
         H = Dl // hd
@@ -89,6 +97,9 @@ class OracleBackend:
             v = self.ve_apply(v, ve.view(B, T, H, hd), gate.view(B, T, H))
         q = self.rope_qknorm(q.reshape(B, T, H, hd), cos, sin)
         k = self.rope_qknorm(k.reshape(B, T, H, hd), cos, sin)
+        if seqs is not None:
+            q, k, v = (t.reshape(B * T, H, hd) for t in (q, k, v))
+            return R.packed_attention(q, k, v, seqs, window).reshape(B * T, Dl)
         return self.attention(q, k, v, window).reshape(B * T, Dl)
 
     def proj_add_norm(self, a, w, x):

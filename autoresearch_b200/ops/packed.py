@@ -35,6 +35,16 @@ def check_bounds(bounds, rows: int) -> None:
         last = b
 
 
+def document_bounds(ids: torch.Tensor, bos: int) -> torch.Tensor:
+    """Bounds (int32, on the device of ``ids``) of the documents of a batch [B, T] of rows, flattened: one begins at every row and
+    at every token ``bos``.  For ids on a GPU their number is read back."""
+    B, T = ids.shape
+    starts = ids == bos
+    starts[:, 0] = True
+    at = starts.reshape(-1).nonzero().reshape(-1).to(torch.int32)
+    return torch.cat([at, torch.tensor([B * T], dtype=torch.int32, device=ids.device)])
+
+
 class PackedSequences:
     """Which tiles the sequences of a packed batch have.
 

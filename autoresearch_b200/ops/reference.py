@@ -81,6 +81,43 @@ def attention(q, k, v, window: int):
     return o.to(q.dtype).contiguous()
 
 
+def packed_attention(q, k, v, bounds, window: int):
+    """The same over packed sequences: rows [bounds[i], bounds[i + 1]) of q [N, H, hd] and k, v [N, KV, hd] see themselves only,
+    query head h reads key head h // (H / KV); rows of no sequence give zero."""
+    N, H, hd = q.shape
+    G = H // k.shape[1]
+    out = []
+    at = 0
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        if a > at:
+            out.append(torch.zeros(a - at, H, hd, dtype=q.dtype, device=q.device))
+        if b > a:
+            out.append(attention(q[None, a:b], k[None, a:b].repeat_interleave(G, 2), v[None, a:b].repeat_interleave(G, 2), window)[0])
+        at = max(at, b)
+    if N > at:
+        out.append(torch.zeros(N - at, H, hd, dtype=q.dtype, device=q.device))
+    return torch.cat(out) if out else q.new_zeros(q.shape)
+
+
+def linear_cross_entropy(x, w, targets, softcap: float):
+    """Per-row losses of a linear head, soft-capped where softcap > 0; a target outside of the vocabulary gives 0."""
+    s = x.float() @ w.float().t()
+    if softcap:
+        s = softcap * torch.tanh(s / softcap)
+    ok = (targets >= 0) & (targets < w.shape[0])
+    at = torch.where(ok, targets, torch.zeros_like(targets)).long()
+    return torch.where(ok, torch.logsumexp(s, -1) - s.gather(-1, at.view(-1, 1)).squeeze(-1), torch.zeros((), device=x.device))
+
+
+def clip_grad_norm(grads, max_norm: float):
+    """Scales the tensors in place by min(1, max_norm / norm) and returns their 2-norm; one that is not finite scales nothing."""
+    norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
+    scale = torch.where(torch.isfinite(norm) & (norm > max_norm), max_norm / norm, torch.ones_like(norm))
+    for g in grads:
+        g.mul_(scale.to(g.dtype))
+    return norm.float()
+
+
 def ve_apply(v, ve, gate_logits):
     """v += 2*sigmoid(gate)[..., h, None] * ve[..., h, :]
     (brain/kernels/ve_apply.cu:10-43).  v, ve: [B,T,H,hd]; gate_logits: [B,T,H]."""

@@ -13,6 +13,8 @@ Granularity follows what fuses well on a B200 rather than the reference's op lis
                     recovers 2*relu(h) as 2*sqrt of it inside the dX GEMM epilogue).
 * ``LMHeadCEFn``  – chunked LM head + soft-capped CE; logits are turned into their
                     gradient in place during the forward so nothing is recomputed.
+* documents packed into rows (``seqs``): packed attention (ops/packed.py) in place of AttentionFn, layer by layer;
+  large vocabularies: the head's loss in pieces (ops/linear_ce.py) in place of LMHeadCEFn.
 * weight gradients accumulate in fp32 (``param.main_grad``) inside the dW GEMM epilogue.
 """
 from __future__ import annotations
@@ -25,6 +27,8 @@ import torch
 
 from . import kernels as K
 from .backend import OracleBackend
+from .linear_ce import linear_cross_entropy
+from .packed import PackedSequences, packed_qkv_attention
 
 
 def _main_grad(p: torch.Tensor) -> Optional[torch.Tensor]:
@@ -711,6 +715,7 @@ class Sm100Backend(OracleBackend):
         K.lib()  # fail loudly when the native library is missing
         self.attn = attn
         self.big_ce_chunk = 16384
+        self.vocab_pieces = False     # True: the head's loss without logits in memory, at the price of a second logits product
         self.layer_calls = True       # False: one autograd node and one native call per step of a layer
         self._pass = None             # the forward pass in progress, and the same for the layer whose steps run one by one
         self._layer_pass = None
@@ -797,7 +802,10 @@ class Sm100Backend(OracleBackend):
     def residual_add(self, x, y):
         return ResidualAddFn.apply(x, y)
 
-    def attention_block(self, xn, blk, ids_flat, B, T, cfg, cos, sin, window):
+    def packed_sequences(self, cu_seqlens, rows, n_head):
+        return PackedSequences(cu_seqlens, rows, n_head)
+
+    def attention_block(self, xn, blk, ids_flat, B, T, cfg, cos, sin, window, seqs=None):
         tp = self._tp()
         fused_tp = tp if (tp is not None and tp.mode == "fused") else None
         if tp is not None and fused_tp is None:
@@ -809,6 +817,10 @@ class Sm100Backend(OracleBackend):
         of_pass, self._layer_pass = self._layer_pass, None
         qkv = AttnPreFn.apply(xn, blk.wqkv, ids_flat, blk.ve, blk.ve_gate, cos, sin, T, H, cfg.ve_gate_ch, self.eps,
                               fused_tp, of_pass)
+        if seqs is not None:
+            if self.attn != "own":
+                raise ValueError("the library attention does not take documents")
+            return packed_qkv_attention(qkv, seqs, window=window)
         fn = AttentionFn if self.attn == "own" else LibraryAttentionFn
         return fn.apply(qkv, B, T, H, window)
 
@@ -835,7 +847,15 @@ class Sm100Backend(OracleBackend):
         return MoEFn.apply(xn, x, blk.router, blk.expert_fc, blk.expert_proj, moe.top_k, moe.aux_coeff,
                            moe.capacity_factor, getattr(self, "ep", None), blk.layer)
 
+    def takes_vocab_pieces(self, vocab: int) -> bool:
+        """Whether the head's loss goes through the vocabulary piece by piece (ops/linear_ce.py): where it is asked for, and for the
+        vocabularies that whole rows of logits are not made for (csrc/cross_entropy.cu)."""
+        return self.vocab_pieces or vocab > 32768 or vocab % 8 != 0
+
     def lm_head_ce(self, xf, w, targets, grad_scale):
+        if self.takes_vocab_pieces(w.shape[0]):
+            per_tok = linear_cross_entropy(xf, w, targets, softcap=self.softcap)
+            return per_tok.sum() * grad_scale, per_tok.detach()
         need = torch.is_grad_enabled() and (xf.requires_grad or w.requires_grad)
         chunk = max(self.ce_chunk, self.big_ce_chunk)
         return LMHeadCEFn.apply(xf, w, targets.contiguous(), self.softcap, grad_scale, chunk, need)

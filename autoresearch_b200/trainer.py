@@ -106,10 +106,18 @@ class Trainer(TrainerBase):
                                       mcfg.moe.top_k, mcfg.moe.capacity_factor)
         self.wsd = WSDState(tcfg.max_steps, tcfg.cooldown_steps, tcfg.schedule_cfg.warmdown_ratio,
                             warmup_steps=int(round(tcfg.schedule_cfg.warmup_ratio * (tcfg.max_steps or 0))))
+        self.clips_gradients = self.world == 1
+        self.masks_documents = True
+        self._grads = None
+        self.grad_norm = None         # of the last step, where gradients are clipped (a device scalar)
         self._init_common()
+        if hasattr(self.backend, "vocab_pieces"):
+            self.backend.vocab_pieces = tcfg.vocab_pieces
+        pieces = getattr(self.backend, "takes_vocab_pieces", None)
         self.plan_memory(dp=self.world, ep=self.ep, fused_dp=(self.comm.name == "fused"),
                          act_bytes=2 if self.dtype == torch.bfloat16 else 4,
-                         ce_chunk=max(mcfg.ce_chunk, getattr(self.backend, "big_ce_chunk", 0)))
+                         ce_chunk=max(mcfg.ce_chunk, getattr(self.backend, "big_ce_chunk", 0)),
+                         documents=tcfg.doc_bos is not None, vocab_pieces=pieces is not None and pieces(mcfg.vocab))
         if tcfg.resume and tcfg.checkpoint_dir:
             self._resume()
 
@@ -196,7 +204,7 @@ class Trainer(TrainerBase):
             ids, tgt = self._stage_batch(micro)
             self.model.grad_bucket_cb = bucket_ready if (overlap and micro == self.accum - 1) else None
             with nvtx_range(f"forward micro {micro}"):
-                scaled, per_tok = self.model(ids, tgt, grad_scale=grad_scale)
+                scaled, per_tok = self.model(ids, tgt, grad_scale=grad_scale, cu_seqlens=self._documents)
             with nvtx_range(f"backward micro {micro}"):
                 scaled.backward()
             self.layout.accumulate_autograd_grads()
@@ -218,6 +226,9 @@ class Trainer(TrainerBase):
             torch.cuda.current_stream(self.device).wait_stream(self._side)
             self.comm.activate_staged()
         else:
+            if t.grad_clip > 0.0:
+                with nvtx_range("gradient clipping"):
+                    self.grad_norm = self._clip_gradients(t.grad_clip)
             with nvtx_range("gradient exchange"):
                 self.comm.reduce_scatter_grads(self.layout)
             gs = self.comm.grad_source(self.layout) if hasattr(self.comm, "grad_source") else None
@@ -231,6 +242,16 @@ class Trainer(TrainerBase):
         self.timer.mark("end")
         self.step += 1
         return self._loss_acc
+
+    def _clip_gradients(self, max_norm: float) -> torch.Tensor:
+        """All gradients of the model together, in place; the norm they had."""
+        if self.impl != "sm100":
+            from .ops.reference import clip_grad_norm
+            return clip_grad_norm([self.layout.flat_grad], max_norm)
+        from .optim.clip import GradSet, clip_grad_norm
+        if self._grads is None:
+            self._grads = GradSet([self.layout.flat_grad])       # the same buffer every step
+        return clip_grad_norm(self._grads, max_norm)
 
     def _print_grad_norms(self):
         for a in self.layout.atoms:
@@ -261,8 +282,14 @@ class Trainer(TrainerBase):
         if self.token_bytes is None:
             self.token_bytes = load_token_bytes(self.tcfg.tokenizer_dir, self.mcfg.vocab, self.device)
         loader = self._make_loader("val")
+        forward = None
+        if self.tcfg.doc_bos is not None:
+            from .ops.packed import document_bounds
+
+            def forward(ids, tgt):           # scored as it is trained
+                return self.model(ids, tgt, cu_seqlens=document_bounds(ids, self.tcfg.doc_bos))[1], tgt
         return eval_bpb(self.model, loader, self.token_bytes, max_batches, self.device,
-                        group=self.group if self.world > 1 else None)
+                        group=self.group if self.world > 1 else None, forward=forward)
 
     def save(self, step: Optional[int]) -> Optional[str]:
         if hasattr(self.comm, "flush"):

@@ -57,7 +57,7 @@ class MemoryPlan:
 
 def plan(mcfg: ModelConfig, micro_batch: int, *, dp: int = 1, tp: int = 1, ep: int = 1, n_layer_local: int = None,
          has_embedding: bool = True, has_head: bool = True, fused_dp: bool = False, act_bytes: int = 2,
-         ce_chunk: int = 16384) -> MemoryPlan:
+         ce_chunk: int = 16384, documents: bool = False, vocab_pieces: bool = False) -> MemoryPlan:
     """Plan for one rank.  `dp`: ranks that share the optimizer state (ZeRO-1 owner shards); `tp`: tensor-parallel
     ranks (weights and the wide activations are split, the residual stream is split along the sequence);
     `n_layer_local`: layers of this pipeline stage.  Sizes follow the tensors kept by ops/sm100.py."""
@@ -103,6 +103,8 @@ def plan(mcfg: ModelConfig, micro_batch: int, *, dp: int = 1, tp: int = 1, ep: i
         ("layer: x mid", Ns * D * a),
         ("layer: xn2", Ns * D * a),
     ]
+    if documents:
+        layer.append(("layer: rest of the attention out", N * Dl * a))       # ops/packed.py
     if tp > 1:
         layer += [("layer: gathered xn (TP)", 2 * N * D * a)]
     if moe is None:
@@ -118,7 +120,13 @@ def plan(mcfg: ModelConfig, micro_batch: int, *, dp: int = 1, tp: int = 1, ep: i
         p.step.append(("embedding out + x0", 2 * Ns * D * a))
     if has_head:
         p.step.append(("final norm in/out, d_xf, losses", 3 * Ns * D * a + Ns * 4))
-        p.step.append(("logits chunk", min(ce_chunk, Ns) * V * a))
+        if vocab_pieces:
+            from ..ops.linear_ce import TILE, piece_columns
+            cols = piece_columns(Ns, V)
+            p.step.append(("vocabulary piece, row statistics", (cols + 8) * Ns * a + (2 * -(-V // TILE) + 3) * Ns * 4))
+            p.step.append(("head input gradient (fp32)", Ns * D * 4 if cols < V else 0))
+        else:
+            p.step.append(("logits chunk", min(ce_chunk, Ns) * V * a))
     # widest moment of the backward pass: d(out), d(hidden) or d(qkv) with the attention statistics, and two
     # residual-stream gradients; the native call of a small layer holds d(hidden) beside d(qkv), for one launch of its weight gradients
     from ..ops.sm100 import GROUP_DW_FLOPS
