@@ -13,7 +13,7 @@ enum ArbEpilogue {
   EPI_ATOMIC_F32 = 2,   // C += acc   (fp32, red.global; split-K allowed)
   EPI_NS_COMBINE = 3,   // C = alpha*I + beta*aux + gamma*acc   (bf16)
   EPI_RELU2_BWD = 4,    // C = acc * 2*sqrt(max(aux, 0)): aux = relu(h)^2 saved by the forward (bf16)
-  EPI_STORE_F32 = 5,    // C = acc                      (fp32)
+  EPI_STORE_F32 = 5,    // C = acc                      (fp32; splitk > 1 of an unbatched product: the parts stride_c apart)
   EPI_ADD_AUX = 6,      // C = aux + acc                (bf16)
   EPI_QKV_POST = 7,     // packed q|k|v projection: RoPE + RMS norm on q and k heads, value embedding on v heads (bf16);
                         // 2-CTA tiles, NT layout; parameters from arb_gemm_qkv_post_args
@@ -109,7 +109,7 @@ int arb_gemm_bf16_ex(const void* A, const void* B, void* C, const void* aux, int
 // row, log2 sum_v exp s.
 // bwd: `piece` ids at a time (a multiple of 256, or all), d_logits[n, v] = weight[n] (softmax(s)[n, v] - [v = target]) ds/dx in bf16
 // (scratch of rows x ldd), then dx (+)= d_logits w and dw = d_logits^T x.  dx: [rows, dim] bf16 or null; acc: fp32 scratch of its size
-// where there are several pieces.  dw: [vocab, dim] bf16, or main: fp32 rows ld_main apart that the gradient is added to, or both null.
+// where there are several pieces, or as many times that as arb_linear_ce_parts says where there is one and it says more than one.  dw: [vocab, dim] bf16, or main: fp32 rows ld_main apart that the gradient is added to, or both null.
 typedef struct ArbLinearCE {
   const void *x, *w, *targets;       // [rows, dim] bf16, [cols, dim] bf16, [rows] int32 or int64
   float *part, *target_score, *lse, *loss;
@@ -119,6 +119,7 @@ typedef struct ArbLinearCE {
   double softcap;
 } ArbLinearCE;
 int arb_linear_ce_fwd(const ArbLinearCE* a, int* err_flag, cudaStream_t stream);
+int arb_linear_ce_parts(long long rows, long long dim, long long piece);
 int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx, float* acc, void* dw, float* main, long long ld_main, int* err_flag,
                       cudaStream_t stream);
 

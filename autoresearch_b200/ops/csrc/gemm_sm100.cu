@@ -405,7 +405,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       tc_fence_after();
       const int row = mt * BM + q * 32 + lane;
       const bool row_ok = row < p.M;
-      const long long row_off = (long long)b * p.stride_c + (long long)row * p.ldc;
+      const long long row_off = (long long)(EPI == EPI_STORE_F32 ? b * p.splitk + ks : b) * p.stride_c + (long long)row * p.ldc;
 #pragma unroll 1
       for (int c = 0; c < BN / 32; ++c) {
         uint32_t v[32];
@@ -884,7 +884,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (t0) {
               if (col_s < p.N && row0 < p.M) {
                 if (EPI == EPI_ATOMIC_F32) tma_reduce_add_3d(&tmC, smem + L::C_STAGE + buf * 16384, col_s, row0, b);
-                else tma_store_3d(&tmC, smem + L::C_STAGE + buf * 16384, col_s, row0, b);
+                else tma_store_3d(&tmC, smem + L::C_STAGE + buf * 16384, col_s, row0, b * p.splitk + ks);
               }
               tma_store_commit();
             }
@@ -1328,8 +1328,9 @@ static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmA
   std::memset(&tx, 0, sizeof tx);
   if (EPI != EPI_CE_STATS) {
     const uint64_t es = epi_is_bf16(EPI) ? 2 : 4;
-    uint64_t dims[3] = {uint64_t(a.N), uint64_t(a.M), uint64_t(a.batch)};
-    uint64_t str[2] = {uint64_t(a.ldc) * es, a.batch > 1 ? uint64_t(a.stride_c) * es : uint64_t(a.M) * uint64_t(a.ldc) * es};
+    const int slabs = EPI == EPI_STORE_F32 ? a.batch * a.splitk : a.batch;
+    uint64_t dims[3] = {uint64_t(a.N), uint64_t(a.M), uint64_t(slabs)};
+    uint64_t str[2] = {uint64_t(a.ldc) * es, slabs > 1 ? uint64_t(a.stride_c) * es : uint64_t(a.M) * uint64_t(a.ldc) * es};
     uint32_t box[3] = {uint32_t(epi_is_bf16(EPI) ? 64 : 32), 128, 1};
     int r = make_tmap_typed(&tc, a.C, 3, dims, str, box,
                             epi_is_bf16(EPI) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32);
@@ -1503,9 +1504,41 @@ static int ce_grad(const ArbLinearCE& a, int* err_flag, cudaStream_t stream) {
   return launch_pair<false, false, EPI_CE_GRAD>(ta, tb, g, stream);
 }
 
+// out = sum of n fp32 slabs in their order, bf16
+__global__ void __launch_bounds__(256) ce_sum_slabs_k(const float4* slabs, uint2* out, long long n4, int n) {
+  grid_enter();
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
+    float4 s = slabs[i];
+    for (int k = 1; k < n; ++k) {
+      const float4 v = slabs[i + k * n4];
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    out[i] = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+  }
+}
+
+// Parts that the sum over a piece of the vocabulary is cut into for dx [rows, dim]: where its 256 x 256 tiles leave the pairs of SMs idle,
+// as many (at most four, each of at least 4096 ids) as fill them best.  The parts go to slabs of their own and are added in order, so
+// that the result is the same every time (4099 x 384 from 50021 ids: 34 tiles on 74 pairs, 260 -> 163 us and the pass with both gradients
+// 780 -> 718 us).
+extern "C" int arb_linear_ce_parts(long long rows, long long dim, long long piece) {
+  const long long tiles = ((rows + 255) / 256) * ((dim + 255) / 256), units = 74;
+  int best = 1;
+  double eff = double(tiles) / double(units);
+  for (int s = 2; tiles < units && s <= 4 && piece / s >= 4096; ++s) {
+    const long long it = tiles * s;
+    const double e = double(it) / double((it + units - 1) / units * units);
+    if (e > 1.15 * eff) { eff = e; best = s; }
+  }
+  // the K loop is cut in whole blocks of 64: every part gets some
+  const long long kb = (piece + BK - 1) / BK;
+  while (best > 1 && (kb + (kb + best - 1) / best - 1) / ((kb + best - 1) / best) != best) --best;
+  return best;
+}
+
 extern "C" int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx, float* acc, void* dw, float* main, long long ld_main,
                                  int* err_flag, cudaStream_t stream) {
-  if (!a || a->col0 != 0 || a->cols != a->vocab || piece <= 0 || (piece < a->vocab && (piece % 256 || (dx && !acc)))) return -3;
+  if (!a || a->col0 != 0 || a->cols != a->vocab || piece <= 0 || (piece < a->vocab && piece % 256)) return -3;
   if (!a->lse || !a->weight || !a->d_logits || (dw && main)) return -3;
   if (((reinterpret_cast<uintptr_t>(a->d_logits) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(acc) |
         reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(main)) & 15) || (a->ldd % 8) || a->ldd < (piece < a->vocab ? piece : a->vocab))
@@ -1513,6 +1546,8 @@ extern "C" int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx
   if (main && ((ld_main % 4) || ld_main < a->dim)) return -4;
   const int N = int(a->rows), D = int(a->dim);
   const bool one = piece >= a->vocab;
+  const int parts = one ? arb_linear_ce_parts(a->rows, a->dim, a->vocab) : 1;
+  if (dx && !acc && (!one || parts > 1)) return -3;
   for (long long c = 0; c < a->vocab; c += piece) {
     ArbLinearCE b = *a;
     b.w = reinterpret_cast<const __nv_bfloat16*>(a->w) + c * a->ldw;
@@ -1521,9 +1556,9 @@ extern "C" int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx
     if (int r = ce_grad(b, err_flag, stream)) return r;
     if (dx) {
       // several pieces meet in fp32, one after the other and without a split of the summed dimension: the same bits every time
-      const int epi = one ? EPI_STORE_BF16 : c == 0 ? EPI_STORE_F32 : EPI_ATOMIC_F32;
-      if (int r = arb_gemm_bf16(a->d_logits, b.w, one ? dx : acc, nullptr, N, D, int(b.cols), 1, a->ldd, a->ldw, D, 0, 0, 0, 0, 1, epi, 1, 0.f,
-                                0.f, 1.f, err_flag, stream))
+      const int epi = one && parts == 1 ? EPI_STORE_BF16 : c == 0 ? EPI_STORE_F32 : EPI_ATOMIC_F32;
+      if (int r = arb_gemm_bf16(a->d_logits, b.w, one && parts == 1 ? dx : acc, nullptr, N, D, int(b.cols), 1, a->ldd, a->ldw, D, 0, 0,
+                                parts > 1 ? (long long)N * D : 0, 0, 1, epi, parts, 0.f, 0.f, 1.f, err_flag, stream))
         return r;
     }
     if (main) {
@@ -1536,7 +1571,11 @@ extern "C" int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx
         return r;
     }
   }
-  if (dx && !one) return arb_cast_f32_to_bf16(acc, dx, (long long)N * D, 1.f, stream);
+  if (dx && (!one || parts > 1)) {
+    const long long n4 = (long long)N * D / 4, blocks = (n4 + 255) / 256;
+    return launch_dependent(n4 * 16 * parts <= EARLY_BYTES, ce_sum_slabs_k, unsigned(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream,
+                            reinterpret_cast<const float4*>(acc), reinterpret_cast<uint2*>(dx), n4, parts);
+  }
   return 0;
 }
 
@@ -1645,7 +1684,8 @@ extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const
   // 128 x 128, operands from HBM: 2048 x 512 x 2048 22.5 -> 18.4, 2048 x 512 x 1536 19.3 -> 17.3, 1024 x 1024 x 4096 32.8 -> 28.7,
   // 1024 x 256 x 256 15.2 -> 13.2; with 256 tiles of 128 x 128, i.e. two waves, 2048 x 2048 x 512 gains nothing).
   const long long tiles128 = (long long)batch * ((M + 127) / 128) * ((N + 127) / 128);
-  const bool few = g_gemm_mode == 0 && tiles128 <= 148 && epi != EPI_ATOMIC_F32 && epi != EPI_QKV_POST;
+  const bool slabs = epi == EPI_STORE_F32 && splitk > 1;      // the parts of a split sum side by side, stride_c apart
+  const bool few = g_gemm_mode == 0 && tiles128 <= 148 && epi != EPI_ATOMIC_F32 && epi != EPI_QKV_POST && !slabs;
   const int BN = (N > 128 && !few) ? 256 : 128;
   const bool pair = (g_gemm_mode != 1) && (g_gemm_mode == 2 || (M >= 512 && N >= 256 && !few));
   if (sym) {
@@ -1661,12 +1701,14 @@ extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const
   a.m_tiles = (M + bm_eff - 1) / bm_eff;
   a.n_tiles = pair ? (N + 255) / 256 : (N + BN - 1) / BN;
   a.kb_total = (K + BK - 1) / BK;
-  if (epi != EPI_ATOMIC_F32) splitk = 1;
+  if (slabs && (batch != 1 || stride_c <= 0 || (stride_c % 4))) return -3;
+  if (epi != EPI_ATOMIC_F32 && !slabs) splitk = 1;
   if (splitk <= 0)  // automatic: fill the SMs when there are few output tiles
     splitk = pick_split(batch * a.m_tiles * a.n_tiles, a.kb_total, pair ? g_num_sms / 2 : g_num_sms);
   if (splitk > a.kb_total) splitk = a.kb_total;
   a.kb_per_split = (a.kb_total + splitk - 1) / splitk;
   a.splitk = (a.kb_total + a.kb_per_split - 1) / a.kb_per_split;
+  if (slabs && a.splitk != splitk) return -3;                 // the caller sums that many
   a.C = C; a.aux = aux; a.ldc = ldc; a.stride_c = stride_c;
   a.alpha = alpha; a.beta = beta; a.gamma = gamma; a.err = err_flag;
   a.pull_src = reinterpret_cast<const uint4*>(pull_src);

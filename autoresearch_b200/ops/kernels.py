@@ -72,6 +72,7 @@ def _signatures() -> dict:
         "arb_attn_fwd": [vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, i32, f32, vp, vp],
         "arb_attn_bwd": [vp] * 11 + [i32, i32, i32] + [i64] * 8 + [i32, f32, vp, vp],
         "arb_linear_ce_fwd": [vp, vp, vp],
+        "arb_linear_ce_parts": [i64, i64, i64],
         "arb_linear_ce_bwd": [vp, i64, vp, vp, vp, vp, i64, vp, vp],
         "arb_grad_squares": [vp, i32, vp, i32, vp],
         "arb_grad_scale": [vp, i32, vp, i32, f32, vp, i32, vp],

@@ -97,8 +97,9 @@ def _gradients(x, w, targets, lse, g, softcap, need_x, need_w):
     d = x.new_empty(N * ldd)
     dx = x.new_empty((N, D)) if need_x else None
     dw = w.new_empty((V, D)) if need_w and main is None else None
-    # several pieces meet in fp32, in the order of the vocabulary
-    acc = x.new_empty((N, D), dtype=torch.float32) if need_x and cols < V else None
+    # several pieces meet in fp32, in the order of the vocabulary; a single one may be summed in parts
+    parts = K.lib().arb_linear_ce_parts(N, D, V) if cols == V else 1
+    acc = x.new_empty((parts, N, D), dtype=torch.float32) if need_x and (cols < V or parts > 1) else None
     ptr = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
     args = _args(xr, wr, targets, softcap, lse=lse.data_ptr(), weight=g.data_ptr(), d_logits=d.data_ptr(), ldd=ldd)
     K._check(K.lib().arb_linear_ce_bwd(args, cols, ptr(dx), ptr(acc), ptr(dw), ptr(main), main.stride(0) if main is not None else 0,

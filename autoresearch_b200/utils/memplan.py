@@ -124,7 +124,7 @@ def plan(mcfg: ModelConfig, micro_batch: int, *, dp: int = 1, tp: int = 1, ep: i
             from ..ops.linear_ce import TILE, piece_columns
             cols = piece_columns(Ns, V)
             p.step.append(("vocabulary piece, row statistics", (cols + 8) * Ns * a + (2 * -(-V // TILE) + 3) * Ns * 4))
-            p.step.append(("head input gradient (fp32)", Ns * D * 4 if cols < V else 0))
+            p.step.append(("head input gradient (fp32, up to four parts)", Ns * D * 4 * (1 if cols < V else 4 if Ns * D < 74 * 65536 else 0)))
         else:
             p.step.append(("logits chunk", min(ce_chunk, Ns) * V * a))
     # widest moment of the backward pass: d(out), d(hidden) or d(qkv) with the attention statistics, and two

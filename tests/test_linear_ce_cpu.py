@@ -49,3 +49,13 @@ def test_target_types_that_are_refused(no_device_check):
     for dtype in (torch.int16, torch.float32, torch.bool):
         with pytest.raises(ValueError, match="targets"):
             L.linear_cross_entropy(x, w, torch.zeros(4, dtype=dtype))
+
+
+@pytest.mark.parametrize("rows,dim,piece,want", [(4099, 384, 50021, 2), (16384, 1024, 65536, 1), (512, 256, 1024, 1), (512, 256, 20000, 4),
+                                                 (1, 8, 8191, 1), (1, 8, 8192, 2), (300, 512, 17003, 4)])
+def test_parts_fill_the_pairs_of_multiprocessors(rows, dim, piece, want):
+    got = K.lib().arb_linear_ce_parts(rows, dim, piece)
+    assert got == want
+    blocks = -(-piece // 64)
+    per = -(-blocks // got)
+    assert -(-blocks // per) == got          # no part is empty
