@@ -210,6 +210,18 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
 }
 
+// Bits of the visible ones of 32 columns, those of [lo, hi] (relative to the first).  A masked score becomes -inf in its register, a
+// bit test and a select per element; comparing every column with the row's interval takes three instructions, in both passes over
+// the scores.
+__device__ __forceinline__ uint32_t visible(int lo, int hi) {
+  const int a = max(lo, 0), b = min(hi, 31);
+  return b < a ? 0u : ((2u << b) - 1u) & ~((1u << a) - 1u);      // 2 << 31 is 0: all bits from a
+}
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t bits) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[j] = (bits & (1u << j)) ? s[j] : 0xff800000u;
+}
+
 // CTAs stay and take tile after tile: barriers, TMEM and the pipeline's start are paid once, and a tile's first loads run under the
 // previous tile's last products and epilogue (as one CTA per tile, sequences of 128 rows cost 10 us of an SM per backward tile).
 // The loading warp decides which tile is next and hands it to the other roles through two slots.
@@ -276,16 +288,38 @@ __device__ __forceinline__ void load_q(uint8_t* dst, const CUtensorMap* m, uint6
   if (D == 128) tma_load_4d(dst + 16384, m, bar, 64, 0, kv, row);
 }
 
-// 32 accumulator columns of one row as bf16
-__device__ __forceinline__ void store32(__nv_bfloat16* dst, const uint32_t (&v)[32], float s) {
+// 32 rows of COLS (32 or 64) bf16 columns, a row in each lane, to rows `off` elements from `dst` (off < 0: not written).  Through 64
+// bytes a column of shared memory of the warp's own, so that neighbouring lanes write neighbouring bytes and not each 16 bytes of
+// another row (32768 rows, window 256, 8 heads on 4: forward with both parts of O 131 -> 121 us, backward 316 -> 291 us).
+template <int COLS>
+__device__ __forceinline__ void store_rows(__nv_bfloat16* dst, long long off, const uint32_t* w, uint32_t stage, int lane) {
+  constexpr int PIECES = COLS / 8;                       // 16 bytes each
+  // pieces of a row change places with its number, so that eight lanes meet no bank twice
+  auto at = [&](int row, int piece) { return stage + uint32_t(row * COLS * 2 + ((piece ^ (PIECES == 8 ? row & 7 : (row >> 1) & 3)) << 4)); };
+  __syncwarp();                                          // the previous use has been read
 #pragma unroll
-  for (int j = 0; j < 32; j += 8) {
+  for (int j = 0; j < PIECES; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(lane, j)), "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int row = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
+    const long long o = __shfl_sync(0xffffffffu, off, row);
     uint4 u;
-    u.x = pack_bf16(__uint_as_float(v[j]) * s, __uint_as_float(v[j + 1]) * s);
-    u.y = pack_bf16(__uint_as_float(v[j + 2]) * s, __uint_as_float(v[j + 3]) * s);
-    u.z = pack_bf16(__uint_as_float(v[j + 4]) * s, __uint_as_float(v[j + 5]) * s);
-    u.w = pack_bf16(__uint_as_float(v[j + 6]) * s, __uint_as_float(v[j + 7]) * s);
-    *reinterpret_cast<uint4*>(dst + j) = u;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at(row, piece)) : "memory");
+    if (o >= 0) *reinterpret_cast<uint4*>(dst + o + piece * 8) = u;
+  }
+}
+// COLS accumulator columns of the lane's row, times s, as bf16 pairs
+template <int COLS>
+__device__ __forceinline__ void pack_columns(uint32_t taddr, float s, uint32_t (&w)[COLS / 2]) {
+#pragma unroll
+  for (int c = 0; c < COLS / 32; ++c) {
+    uint32_t v[32];
+    tmem_ld32(taddr + uint32_t(c * 32), v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[c * 16 + j] = pack_bf16(__uint_as_float(v[2 * j]) * s, __uint_as_float(v[2 * j + 1]) * s);
   }
 }
 // `n` rows from `row` of `width` elements each, zero, by a warp
@@ -307,23 +341,6 @@ struct PackedFwdSmem {
   static constexpr int TOTAL = BAR + 192;
 };
 static_assert(2 * (PackedFwdSmem<128>::TOTAL + 1024) <= 233472, "two CTAs must fit the 228 KB of an SM");
-
-// 32 rows of 64 bf16 columns, a row in each lane (32 words), to rows `off` elements from `dst` (off < 0: not written).  Through 4 KB of
-// shared memory of the warp's own, so that eight lanes write 128 adjacent bytes and not each 16 bytes of another row (32768 rows,
-// window 256, 8 heads on 4, both parts of O: 131 -> 121 us).
-__device__ __forceinline__ void store_rows(__nv_bfloat16* dst, long long off, const uint32_t (&w)[32], uint32_t stage, int lane) {
-  __syncwarp();                                          // the previous use has been read
-#pragma unroll
-  for (int j = 0; j < 8; ++j) st_sw128(stage, 32, lane, j * 8, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = i * 4 + (lane >> 3), col = (lane & 7) * 8;
-    const long long o = __shfl_sync(0xffffffffu, off, row);
-    const uint4 u = ld_sw128(stage, 32, row, col);
-    if (o >= 0) *reinterpret_cast<uint4*>(dst + o + col) = u;
-  }
-}
 
 // positions and key tiles of a query tile
 struct QueryTile {
@@ -510,9 +527,8 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tc_fence_after();
         // in unmasked tiles rows without a query compute results of their own that nothing uses
         const bool need_mask = (n0 + 127 > qt.m0) || (n0 < qt.m_last - p.window);
-        // visible keys of this row inside the tile: column indices [mlo, mlo + span]
-        const int mlo = live_row ? pos - p.window - n0 : 128;
-        const unsigned span = live_row ? unsigned(p.window) : 0u;
+        // visible keys of this row inside the tile: columns [lo, hi]
+        const int lo = live_row ? pos - p.window - n0 : 128, hi = live_row ? pos - n0 : 0;
         uint32_t sc[32], sd[32];                           // columns 64..127 stay in registers
         float mx;
         {
@@ -522,12 +538,12 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           tmem_wait_ld();
           tmem_ld32(TM_S + lane_addr + 64u, sc);
           tmem_ld32(TM_S + lane_addr + 96u, sd);
-          if (need_mask) mx = max32<true>(sb, 32, mlo, span, max32<true>(sa, 0, mlo, span, -INFINITY));
-          else mx = max32<false>(sb, 32, mlo, span, max32<false>(sa, 0, mlo, span, -INFINITY));
+          if (need_mask) { hide(sa, visible(lo, hi)); hide(sb, visible(lo - 32, hi - 32)); }
+          mx = max32<false>(sb, 32, 0, 0u, max32<false>(sa, 0, 0, 0u, -INFINITY));
           tmem_wait_ld();
         }
-        if (need_mask) mx = max32<true>(sd, 96, mlo, span, max32<true>(sc, 64, mlo, span, mx));
-        else mx = max32<false>(sd, 96, mlo, span, max32<false>(sc, 64, mlo, span, mx));
+        if (need_mask) { hide(sc, visible(lo - 64, hi - 64)); hide(sd, visible(lo - 96, hi - 96)); }
+        mx = max32<false>(sd, 96, 0, 0u, max32<false>(sc, 64, 0, 0u, mx));
         const float m_new = fmaxf(m_used, mx);
         bool resc = false;
         if (m_used == -INFINITY) m_used = m_new;            // nothing accumulated for this row yet
@@ -552,13 +568,8 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         unsigned long long rs2 = pk2(0.f, 0.f);
         {
           uint32_t pk[32];
-          if (need_mask) {
-            exp32_mufu<true>(sc, pk, c2, nmc2, 64, mlo, span, rs2);
-            exp32_mufu<true>(sd, pk + 16, c2, nmc2, 96, mlo, span, rs2);
-          } else {
-            exp32_mufu<false>(sc, pk, c2, nmc2, 64, mlo, span, rs2);
-            exp32_mufu<false>(sd, pk + 16, c2, nmc2, 96, mlo, span, rs2);
-          }
+          exp32_mufu<false>(sc, pk, c2, nmc2, 64, 0, 0u, rs2);
+          exp32_mufu<false>(sd, pk + 16, c2, nmc2, 96, 0, 0u, rs2);
           tmem_st32(TM_P + lane_addr + 32u, pk);           // over scores that have been read
         }
         tmem_wait_st();
@@ -570,13 +581,9 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           tmem_ld32(TM_S + lane_addr, sa);
           tmem_ld32(TM_S + lane_addr + 32u, sb);
           tmem_wait_ld();
-          if (need_mask) {
-            exp32_mufu<true>(sa, pk, c2, nmc2, 0, mlo, span, rs2);
-            exp32_mufu<true>(sb, pk + 16, c2, nmc2, 32, mlo, span, rs2);
-          } else {
-            exp32_mufu<false>(sa, pk, c2, nmc2, 0, mlo, span, rs2);
-            exp32_mufu<false>(sb, pk + 16, c2, nmc2, 32, mlo, span, rs2);
-          }
+          if (need_mask) { hide(sa, visible(lo, hi)); hide(sb, visible(lo - 32, hi - 32)); }
+          exp32_mufu<false>(sa, pk, c2, nmc2, 0, 0, 0u, rs2);
+          exp32_mufu<false>(sb, pk + 16, c2, nmc2, 32, 0, 0u, rs2);
           tmem_st32(TM_P + lane_addr, pk);
         }
         float r0, r1;
@@ -609,8 +616,8 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             rest[hf * 16 + j] = pack_bf16(x - r2.x, y - r2.y);
           }
         }
-        store_rows(p.o + cc, off, w, stage, lane);
-        if (p.o_lo) store_rows(p.o_lo + cc, off, rest, stage, lane);
+        store_rows<64>(p.o + cc, off, w, stage, lane);
+        if (p.o_lo) store_rows<64>(p.o_lo + cc, off, rest, stage, lane);
       }
       if (live_row) p.lse[(long long)(slot.start + pos) * H + head] = (l > 0.f) ? (m_used * p.scale + __logf(l)) : -INFINITY;
     }
@@ -677,6 +684,11 @@ __device__ __forceinline__ void mma_sum(uint32_t d_tmem, uint32_t a_lo, uint32_t
 }
 
 // ---- dQ: query tile stationary -----------------------------------------------------------------
+// A finished tile leaves through the last ring slot that it used (V's for dQ, dO's for dK and dV), whose next load, two steps on, waits
+// for that: the n-th tile's slot is asked for in the second step of the tile behind it, or in the first of the one after where that
+// has a single step.  Two barriers in turn: the tile behind may be finished, too, before the loading warp asks for this one.
+__device__ __forceinline__ int left_through(int step, int n, bool single) { return step == 1 ? n - 1 : step == 0 && single ? n - 2 : -1; }
+
 template <int D>
 struct DqBars {
   uint64_t* b;
@@ -690,10 +702,11 @@ struct DqBars {
   __device__ __forceinline__ uint64_t* dq_done(int T) const { return b + 12 + T % 6; }     // dQ(T) complete: K(T)'s slot and dS buffer T & 1 free
   __device__ __forceinline__ uint64_t* done() const { return b + 18; }          // dQ of the n-th query tile complete
   __device__ __forceinline__ uint64_t* land(int i) const { return b + 19 + i; } // K / V tile that has to be cleaned has landed
-  __device__ __forceinline__ uint64_t* ring() const { return b + 21; }          // 4
-  static constexpr int COUNT = 25;
+  __device__ __forceinline__ uint64_t* out_free(int n) const { return b + 21 + (n & 1); }  // dQ of the n-th query tile written (8 arrivals)
+  __device__ __forceinline__ uint64_t* ring() const { return b + 23; }          // 4
+  static constexpr int COUNT = 27;
   __device__ __forceinline__ void init() const {
-    for (int i = 0; i < 21; ++i) mbar_init(b + i, i == 7 || i == 10 || i == 11 ? 8 : 1);
+    for (int i = 0; i < 23; ++i) mbar_init(b + i, i == 7 || i == 10 || i == 11 || i >= 21 ? 8 : 1);
   }
 };
 static_assert(DqBars<64>::COUNT * 8 + 2 * sizeof(PackedSlot) <= 256, "barrier space");
@@ -713,7 +726,7 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
   if (warp == 0) {
     const uint32_t q_bytes = uint32_t(p.P * p.G * D * 2);
     int T = 0, cleaned = 0;
-    bool ok = true;
+    bool ok = true, single = false;                      // whether the tile before had a single step
     auto k_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
     auto v_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
     for (int n = 0; ok;) {
@@ -745,6 +758,8 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
           mbar_expect_tx(kb, L::TILE);
           load_kv<D>(k_slot(t), &tmK, kb, kv, row);
           if (t >= 2 && !mbar_wait(bar.dp_full(t), uint32_t((t - 2) >> 1) & 1u, abort_flag)) { ok = false; break; }
+          const int left = left_through(t - T, n, single);
+          if (left >= 0 && !mbar_wait(bar.out_free(left), uint32_t(left >> 1) & 1u, abort_flag)) { ok = false; break; }
           uint64_t* vb = clean && t == last ? bar.land(1) : bar.v_full(t);
           mbar_expect_tx(vb, L::TILE);
           load_kv<D>(v_slot(t), &tmV, vb, kv, row);
@@ -760,6 +775,7 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
         ++cleaned;
       }
       T = last + 1;
+      single = qt.n_tiles == 1;
       ++n;
     }
   } else if (warp == 1) {
@@ -847,14 +863,13 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar.a_done());
-          exp2_64<true>(s0, s1, c, lse2, nullptr, pr);
           if ((n0 + 63 > qt.m0) || (n0 < qt.m_last - p.window)) {
-            // the visible keys of a row are one interval of column indices
-            const int lo = live_row ? pos - p.window - n0 : 64;
-            const unsigned span = live_row ? unsigned(p.window) : 0u;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) pr[j] = (unsigned(j - lo) <= span) ? pr[j] : 0.f;
+            // the visible keys of a row are one interval of columns
+            const int lo = live_row ? pos - p.window - n0 : 64, hi = live_row ? pos - n0 : 0;
+            hide(s0, visible(lo, hi));
+            hide(s1, visible(lo - 32, hi - 32));
           }
+          exp2_64<true>(s0, s1, c, lse2, nullptr, pr);
         }
         // ---- phase B ----
         if (!wait_warp(bar.dp_full(T), uint32_t(T >> 1) & 1u, abort_flag)) { ok = false; break; }
@@ -885,14 +900,13 @@ __device__ __forceinline__ void packed_bwd_dq(const CUtensorMap& tmQ, const CUte
       load_stats(slot);                    // in flight while this query tile is finished
       if (!wait_warp(bar.done(), uint32_t(n) & 1u, abort_flag)) break;
       tc_fence_after();
-      __nv_bfloat16* orow = p.o + (long long)(done.start + pos) * p.ldo + (long long)(done.kv * p.G + (r - at * p.G)) * D + hf * (D / 2);
-#pragma unroll
-      for (int cc = 0; cc < D / 64; ++cc) {
-        uint32_t v[32];
-        tmem_ld32(TM_DQ + lane_addr + uint32_t(hf * (D / 2) + cc * 32), v);
-        tmem_wait_ld();
-        if (live_row) store32(orow + cc * 32, v, p.scale);
-      }
+      const long long off = live_row ? (long long)(done.start + pos) * p.ldo + (long long)(done.kv * p.G + (r - at * p.G)) * D : -1;
+      uint32_t w[D / 4];
+      pack_columns<D / 2>(TM_DQ + lane_addr + uint32_t(hf * (D / 2)), p.scale, w);
+      store_rows<D / 2>(p.o + hf * (D / 2), off, w, smem_u32(smem + L::RING2 + ((T - 1) & 1) * L::TILE) + uint32_t(sw * (32 * D)), lane);
+      fence_proxy_async_smem();            // read before the slot's next load overwrites it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar.out_free(n));
     }
   }
 }
@@ -916,10 +930,11 @@ struct DkvBars {
   // all S^T and dP^T of the n-th key tile complete.  (dp_full would say so too, but a parity tells a phase only from the one before and
   // the one behind it: who waits for a barrier visits all of its phases, which the loading warp does not with dp_full's.)
   __device__ __forceinline__ uint64_t* kv_free() const { return b + 19; }
-  __device__ __forceinline__ uint64_t* ring() const { return b + 20; }          // 4
-  static constexpr int COUNT = 24;
+  __device__ __forceinline__ uint64_t* out_free(int n) const { return b + 20 + (n & 1); }  // dK and dV of the n-th key tile written (8 arrivals)
+  __device__ __forceinline__ uint64_t* ring() const { return b + 22; }          // 4
+  static constexpr int COUNT = 26;
   __device__ __forceinline__ void init() const {
-    for (int i = 0; i < 20; ++i) mbar_init(b + i, i == 12 || i == 14 || i == 18 ? 8 : 1);
+    for (int i = 0; i < 22; ++i) mbar_init(b + i, i == 12 || i == 14 || i == 18 || i >= 20 ? 8 : 1);
   }
 };
 static_assert(DkvBars<64>::COUNT * 8 + 2 * sizeof(PackedSlot) <= 256, "barrier space");
@@ -954,7 +969,7 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
   if (warp == 0) {
     const uint32_t q_bytes = uint32_t(used * D * 2);
     int T = 0, cleaned = 0;
-    bool ok = true;
+    bool ok = true, single = false;                      // whether the tile before had a single step
     auto q_slot = [&](int t) { return smem + L::RING3 + (t % 3) * L::TILE; };
     auto do_slot = [&](int t) { return smem + L::RING2 + (t & 1) * L::TILE; };
     for (int n = 0; ok;) {
@@ -984,6 +999,8 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
           mbar_expect_tx(qb, q_bytes);
           load_q<D>(q_slot(t), &tmQ, qb, kv, row);
           if (!mbar_wait(bar.do_empty(t), (uint32_t(t >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+          const int left = left_through(t - T, n, single);
+          if (left >= 0 && !mbar_wait(bar.out_free(left), uint32_t(left >> 1) & 1u, abort_flag)) { ok = false; break; }
           uint64_t* db = clean && t == last ? bar.land(1) : bar.do_full(t);
           mbar_expect_tx(db, q_bytes);
           load_q<D>(do_slot(t), &tmDO, db, kv, row);
@@ -998,6 +1015,7 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
         ++cleaned;
       }
       T = last + 1;
+      single = kt.n_tiles == 1;
       ++n;
     }
   } else if (warp == 1) {
@@ -1091,17 +1109,15 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
           tc_fence_after();
           uint32_t s0[32], s1[32];
           tmem_ld64(TM_S + lane_addr + uint32_t(hf * 64), s0, s1);
-          exp2_64<false>(s0, s1, c, 0.f, cl, pr);
           if (q0 < n0 + 127 || q0 + p.P - 1 > n0 + p.window) {
             // the queries that see a key are one interval of positions, key ... last_pos, and so of columns
-            const int lo = max(key - q0, 0) * p.G - hf * 64;
-            const int hi = (min(last_pos - q0, p.P - 1) + 1) * p.G - 1 - hf * 64;
-            const bool seen = key < len && last_pos >= q0 && hi >= lo;
-            const unsigned span = seen ? unsigned(hi - lo) : 0u;
-            const int lo_eff = seen ? lo : 64;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) pr[j] = (unsigned(j - lo_eff) <= span) ? pr[j] : 0.f;
+            const bool seen = key < len && last_pos >= q0;
+            const int lo = seen ? max(key - q0, 0) * p.G - hf * 64 : 64;
+            const int hi = seen ? (min(last_pos - q0, p.P - 1) + 1) * p.G - 1 - hf * 64 : 0;
+            hide(s0, visible(lo, hi));
+            hide(s1, visible(lo - 32, hi - 32));
           }
+          exp2_64<false>(s0, s1, c, 0.f, cl, pr);
           uint32_t pk[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) pk[j] = pack_bf16(pr[2 * j], pr[2 * j + 1]);
@@ -1144,19 +1160,25 @@ __device__ __forceinline__ void packed_bwd_dkv(const CUtensorMap& tmQ, const CUt
       if (!wait_warp(bar.done(), uint32_t(n) & 1u, abort_flag)) break;
       {
         tc_fence_after();
+        const uint32_t stage = smem_u32(smem + L::RING2 + ((T - 1) & 1) * L::TILE) + uint32_t(sw * (32 * D));
         const long long at = (long long)done.kv * D + hf * (D / 2);
-        __nv_bfloat16* dkrow = p.dk + (long long)(done.start + key) * p.lddk + at;
-        __nv_bfloat16* dvrow = p.dv + (long long)(done.start + key) * p.lddv + at;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
-#pragma unroll
-          for (int cc = 0; cc < D / 64; ++cc) {
-            uint32_t v[32];
-            tmem_ld32((which ? TM_DK : TM_DV) + lane_addr + uint32_t(hf * (D / 2) + cc * 32), v);
-            tmem_wait_ld();
-            if (key < len) store32((which ? dkrow : dvrow) + cc * 32, v, which ? p.scale : 1.f);
-          }
+          const long long off = key < len ? (long long)(done.start + key) * (which ? p.lddk : p.lddv) + at : -1;
+          uint32_t w[D / 4];
+          pack_columns<D / 2>((which ? TM_DK : TM_DV) + lane_addr + uint32_t(hf * (D / 2)), which ? p.scale : 1.f, w);
+          store_rows<D / 2>(which ? p.dk : p.dv, off, w, stage, lane);
         }
+        // rows of the slot that no load of dO fills are zero again
+        constexpr int OWN = D / 4;                         // rows of 128 bytes that this warp has used
+        const int first = (sw * OWN) & 127;
+        __syncwarp();
+        for (int e = lane; e < OWN * 8; e += 32) {
+          if (first + (e >> 3) >= used) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + uint32_t(e) * 16u), "r"(0) : "memory");
+        }
+        fence_proxy_async_smem();                          // before the slot's next load overwrites it
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar.out_free(n));
       }
       if (slot.len > 0) stat[(T & 1) * 128 + col] = first_stat;
     }
@@ -1266,6 +1288,7 @@ static int make_key_tmap(CUtensorMap* m, const void* base, const ArbPacked& a, l
 
 static int check_packed(const ArbPacked& a) {
   // positions plus a window stay within 31 bits
+  if (!(a.scale > 0.0)) return -3;                       // masked scores are -inf, rows take the largest score
   if (a.rows <= 0 || a.rows > PACKED_MAX_ROWS || a.KV <= 0 || a.KV > 65535 || a.G <= 0 || a.G > 128 || (a.D != 64 && a.D != 128) || a.window < 0) return -3;
   if (!a.items || bad_ptr(a.items) || a.cap_q <= 0 || a.cap_k <= 0 || (a.cap_q + a.cap_k) * a.KV > 0x7fffffffll) return -3;
   const void* ptrs[] = {a.q, a.k, a.v, a.o, a.o_lo, a.d_o, a.dq, a.dk, a.dv};

@@ -199,6 +199,8 @@ def _common(device, rows, d, seqs, window, scale):
         window = rows
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
     return min(int(window), rows), 1.0 / math.sqrt(d) if scale is None else float(scale)
 
 
@@ -207,7 +209,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: Pa
     """Attention of packed sequences: q [rows, H, d], k and v [rows, KV, d], bf16, d = 64 or 128, any strides -> [rows, H, d].
 
     Query head h reads key head h // (H / KV).  ``window``: how many positions back a query sees (None: all); ``scale``
-    defaults to 1 / sqrt(d).  The inputs of a sequence reach no other sequence's outputs or gradients, not even as NaN."""
+    (positive) defaults to 1 / sqrt(d).  The inputs of a sequence reach no other sequence's outputs or gradients, not even as NaN."""
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         K._bf16(t, name)
         if t.dim() != 3:

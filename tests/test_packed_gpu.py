@@ -342,6 +342,9 @@ def test_refusals():
         packed_attention(q, k, v[:32], seqs)
     with pytest.raises(ValueError):
         packed_attention(q, k, v, seqs, window=-1)
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            packed_attention(q, k, v, seqs, scale=scale)
     with pytest.raises(ValueError):
         packed_attention(q[0], k[0], v[0], seqs)
     with pytest.raises(TypeError):
