@@ -13,6 +13,7 @@ a query sees the keys of its own sequence at most ``window`` positions back:
 from __future__ import annotations
 
 import math
+import operator
 import struct
 from typing import Optional
 
@@ -63,7 +64,9 @@ class PackedSequences:
         if not 0 <= rows <= MAX_ROWS:
             raise ValueError(f"rows must lie in [0, {MAX_ROWS}], got {rows}")
         if not (torch.is_tensor(cu_seqlens) and cu_seqlens.is_cuda):
-            values = cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else [int(b) for b in cu_seqlens]
+            if torch.is_tensor(cu_seqlens) and (cu_seqlens.dim() != 1 or cu_seqlens.dtype not in (torch.int32, torch.int64)):
+                raise TypeError("cu_seqlens must be a 1-D tensor of integers")
+            values = cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else [operator.index(b) for b in cu_seqlens]
             if not values:
                 raise ValueError("cu_seqlens needs at least one bound")
             check_bounds(values, rows)
@@ -209,7 +212,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: Pa
     """Attention of packed sequences: q [rows, H, d], k and v [rows, KV, d], bf16, d = 64 or 128, any strides -> [rows, H, d].
 
     Query head h reads key head h // (H / KV).  ``window``: how many positions back a query sees (None: all); ``scale``
-    (positive) defaults to 1 / sqrt(d).  The inputs of a sequence reach no other sequence's outputs or gradients, not even as NaN."""
+    (positive) defaults to 1 / sqrt(d).  The inputs of a sequence reach no other sequence's outputs or gradients, not even as NaN.
+    Within a sequence every row has to be finite: a weight of zero does not silence a NaN in a later key's value."""
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         K._bf16(t, name)
         if t.dim() != 3:

@@ -151,6 +151,27 @@ def test_twice_the_same_bits_and_graph_replay():
         _check_scaled(out, grads, min(1.0, 1.0 / want))
 
 
+def test_tensors_that_were_given_other_memory():
+    from autoresearch_b200.optim.clip import GradSet, grad_norm
+    grads = _grads([(1000,), (2000,)], torch.float32)
+    s = GradSet(grads)
+    grads[1].data = torch.full((2000,), 2.0, device="cuda")
+    want = _norm(grads)
+    assert abs(float(grad_norm(s)) - want) <= 2.0 ** -19 * want
+
+
+def test_more_elements_than_32_bits_count():
+    from autoresearch_b200.optim.clip import clip_grad_norm
+    n = (1 << 31) + 4099
+    t = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    t[-5:] = 3.0
+    t[(1 << 31) - 2:(1 << 31) + 2] = 1.0
+    assert abs(float(clip_grad_norm([t], 3.5)) - 7.0) <= 2.0 ** -16
+    assert float(t[-1]) == 1.5 and float(t[1 << 31]) == 0.5 and float(t[0]) == 0.0
+    del t
+    torch.cuda.empty_cache()
+
+
 def test_refusals():
     from autoresearch_b200.optim.clip import GradSet, clip_grad_norm, grad_norm
     t = torch.zeros(10, 10, device="cuda")

@@ -206,6 +206,30 @@ def test_only_one_gradient_asked_for():
     assert not linear_cross_entropy(x, w, t).requires_grad
 
 
+def test_a_weight_of_more_elements_than_32_bits_count():
+    """The last ids of 2.1 million: their gradient rows and a loss whose target is the very last one."""
+    D, V, N = 1024, (1 << 21) + 300, 40
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty(V, D, dtype=torch.bfloat16, device="cuda").normal_(0.0, 0.05, generator=g)
+    x = torch.empty(N, D, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    t[:4] = torch.arange(V - 4, V, device="cuda")
+    weight = torch.ones(N, device="cuda")
+    loss, dx, dw = _run(x, w, t, weight, 15.0)
+    s = 15 * torch.tanh(x.double() @ w.double().T / 15)
+    lse = torch.logsumexp(s, 1)
+    want = lse - s.gather(1, t[:, None])[:, 0]
+    assert float((loss.double() - want).abs().max()) <= _loss_bound(x, w[-1000:], 15.0) * 4
+    d = torch.exp(s[:, -300:] - lse[:, None])
+    for i in range(4):
+        d[i, 300 - 4 + i] -= 1
+    d *= 1 - (s[:, -300:] / 15) ** 2
+    rows = d.T @ x.double()
+    assert float((dw[-300:].double() - rows).norm()) <= 2.0 ** -7 * float(rows.norm())
+    del w, dw, s
+    torch.cuda.empty_cache()
+
+
 def test_no_tokens():
     x, w, t, weight = _inputs(0, 64, 300)
     loss, dx, dw = _run(x, w, t, weight, 0.0)

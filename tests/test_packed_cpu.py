@@ -30,6 +30,12 @@ def test_empty_bounds_and_rows_out_of_range():
             P.PackedSequences([0], rows, 2, 1)
 
 
+def test_bounds_that_are_no_whole_numbers():
+    for bad in (torch.tensor([0.0, 4.0]), torch.tensor([[0, 4]]), [0, 2.5], torch.tensor([False, True])):
+        with pytest.raises(TypeError):
+            P.PackedSequences(bad, 4, 2, 1)
+
+
 def test_cpu_tensors_are_refused():
     t = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
     with pytest.raises(TypeError, match="CUDA"):

@@ -312,6 +312,24 @@ def test_other_stream():
         assert torch.equal(x, y)
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements of q: the last sequences come out as they do alone."""
+    from autoresearch_b200.ops.packed import PackedSequences
+    rows, H, KV, d = 140_000, 128, 8, 128
+    assert rows * H * d > 1 << 31
+    n, last = 200, 140_000 - 200
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, do = (torch.empty(rows, H, d, dtype=torch.bfloat16, device="cuda").normal_(generator=g) for _ in range(2))
+    k, v = (torch.empty(rows, KV, d, dtype=torch.bfloat16, device="cuda").normal_(generator=g) for _ in range(2))
+    bounds = list(range(0, rows + 1, n))
+    got = [t[last:].clone() for t in _run(q, k, v, do, PackedSequences(bounds, rows, H, KV))]
+    want = _run(q[last:], k[last:], v[last:], do[last:], PackedSequences([0, n], n, H, KV))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    del q, do, k, v, got, want
+    torch.cuda.empty_cache()
+
+
 def test_no_rows_and_no_sequences():
     from autoresearch_b200.ops.packed import PackedSequences
     q, k, v, g = _inputs(0, 2, 1, 128)
