@@ -18,11 +18,12 @@ import struct
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 
 _ARGS = struct.Struct("=31qd")          # ArbPacked of csrc/api.h: 12 pointers, 7 sizes, 12 strides, the scale
+_GRADS, _GRADS_AT = struct.Struct("=5q"), 6 * 8                          # d_o, delta, dq, dk, dv
+_D_OUT_STRIDES, _D_OUT_STRIDES_AT = struct.Struct("=2q"), (12 + 7 + 7) * 8      # do_row, do_head
 MAX_ROWS = 1 << 30
 L2_SPAN_BYTES = 48 << 20                # keys and values whose tiles run together (126 MB of L2; attn_common.cuh)
 
@@ -110,33 +111,49 @@ def _layout(t: torch.Tensor):
     return t.clone(memory_format=torch.contiguous_format), n1 * d, d
 
 
-def _forward(q, k, v, strides, seqs, window, scale, keep):
-    """(O, lse, what O's rounding left over where ``keep``).  ``strides``: row and head stride of q, k and v."""
+def _forward(q, k, v, strides, seqs, window, scale, keep, grad_rows):
+    """(O, lse, what O's rounding left over where ``keep``, argument block).  ``strides``: row and head stride of q, k and v;
+    ``grad_rows``: row strides of dq, dk and dv, whose heads are d apart.  The block holds what the backward call takes as well,
+    but for the tensors that call brings, so that little is left to do on the thread that the backward pass runs on."""
     rows, H, d = q.shape
     out = q.new_empty((rows, H, d))
-    rest = q.new_empty((rows, H, d)) if keep else None
     lse = q.new_empty((rows, H), dtype=torch.float32)
+    rest = q.new_empty((rows, H, d)) if keep else None
+    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr() if keep else 0, lse.data_ptr(),
+                      0, 0, 0, 0, 0, seqs._items_ptr, rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k,
+                      *strides, H * d, H * d, d, *grad_rows, scale)
     if rows:
-        args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr() if keep else 0, lse.data_ptr(),
-                          0, 0, 0, 0, 0, seqs._items_ptr, rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k, *strides, H * d, 0, 0, 0, 0, 0, scale)
-        with K.on_device(seqs.device):
-            K._check(K.lib().arb_packed_attn_fwd(args, seqs._err_ptr, K._stream()), "packed_attn_fwd")
-    return out, lse, rest
+        _launch("arb_packed_attn_fwd", args, seqs)
+    return out, lse, rest, args
 
 
-def _backward(q, k, v, out, rest, lse, d_out, dq, dk, dv, strides, row_strides, seqs, window, scale):
-    """``row_strides``: those of dq, dk and dv, whose heads are d apart."""
-    rows, H, d = q.shape
-    if not rows:
+def _launch(entry, args, seqs):
+    if seqs.device.index == torch._C._cuda_getDevice():
+        K._check(getattr(K.lib(), entry)(args, seqs._err_ptr, K._stream()), entry)
         return
-    d_out, do_row, do_head = _layout(d_out)
-    delta = lse.new_empty(rows * H + 2)
-    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), d_out.data_ptr(), delta.data_ptr(),
-                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), seqs._items_ptr, rows, seqs.n_kv_head, seqs.group, d, window,
-                      seqs.cap_q, seqs.cap_k, *strides, H * d, do_row, do_head, *row_strides, scale)
-    with K.on_device(seqs.device):
-        K._check(K.lib().arb_packed_attn_bwd(args, seqs._err_ptr, K._stream()), "packed_attn_bwd")
+    with torch.cuda.device(seqs.device):
+        K._check(getattr(K.lib(), entry)(args, seqs._err_ptr, K._stream()), entry)
+
+
+def _backward(args, lse, d_out, dq, dk, dv, seqs):
+    """``args``: the forward call's block."""
+    if not seqs.rows:
+        return
+    block = bytearray(args)
+    if d_out.is_contiguous() and not d_out.data_ptr() & 15:
+        same = d_out
+    else:
+        same, row, head = _layout(d_out)
+        _D_OUT_STRIDES.pack_into(block, _D_OUT_STRIDES_AT, row, head)
+    delta = lse.new_empty(lse.numel() + 2)
+    _GRADS.pack_into(block, _GRADS_AT, same.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+    _launch("arb_packed_attn_bwd", bytes(block), seqs)
     K.count_launch()                     # the row sums of dO o O and the gradient grid
+
+
+def _first_order_only():
+    if torch.is_grad_enabled():
+        raise RuntimeError("packed attention has no second derivative (create_graph=True)")
 
 
 class PackedAttentionFn(torch.autograd.Function):
@@ -145,21 +162,21 @@ class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, seqs, window, scale, keep):
         (q, q0, q1), (k, k0, k1), (v, v0, v1) = _layout(q), _layout(k), _layout(v)
-        strides = (q0, q1, k0, k1, v0, v1)
-        out, lse, rest = _forward(q, k, v, strides, seqs, window, scale, keep)
-        ctx.save_for_backward(q, k, v, out, rest, lse)
-        ctx.args = (seqs, window, scale)
-        ctx.strides = strides
+        H, d = q.shape[1:]
+        kv = seqs.n_kv_head * d
+        out, lse, rest, args = _forward(q, k, v, (q0, q1, k0, k1, v0, v1), seqs, window, scale, keep, (H * d, kv, kv))
+        if keep:
+            ctx.save_for_backward(q, k, v, out)
+            ctx.kept = (args, lse, rest, seqs)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out):
-        q, k, v, out, rest, lse = ctx.saved_tensors
+        _first_order_only()
+        q, k, _, _ = ctx.saved_tensors
+        args, lse, _, seqs = ctx.kept
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
-        d = q.shape[2]
-        rows = (q.shape[1] * d, k.shape[1] * d, k.shape[1] * d)
-        _backward(q, k, v, out, rest, lse, d_out, dq, dk, dv, ctx.strides, rows, *ctx.args)
+        _backward(args, lse, d_out, dq, dk, dv, seqs)
         return dq, dk, dv, None, None, None, None
 
 
@@ -169,19 +186,20 @@ class PackedQKVAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, seqs, window, scale, d, keep):
         ld = qkv.shape[1]
-        ctx.args, ctx.d, ctx.strides = (seqs, window, scale), d, (ld, d) * 3
-        out, lse, rest = _forward(*_blocks(qkv, seqs, d), ctx.strides, seqs, window, scale, keep)
-        ctx.save_for_backward(qkv, out, rest, lse)
-        return out.view(qkv.shape[0], -1)
+        out, lse, rest, args = _forward(*_blocks(qkv, seqs, d), (ld, d) * 3, seqs, window, scale, keep, (ld,) * 3)
+        out = out.view(qkv.shape[0], -1)
+        if keep:
+            ctx.save_for_backward(qkv, out)
+            ctx.kept = (args, lse, rest, seqs, d)
+        return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out):
-        qkv, out, rest, lse = ctx.saved_tensors
-        seqs = ctx.args[0]
+        _first_order_only()
+        qkv, _ = ctx.saved_tensors
+        args, lse, _, seqs, d = ctx.kept
         d_qkv = qkv.new_empty(qkv.shape)
-        _backward(*_blocks(qkv, seqs, ctx.d), out, rest, lse, d_out.contiguous().view(out.shape), *_blocks(d_qkv, seqs, ctx.d), ctx.strides,
-                  (qkv.shape[1],) * 3, *ctx.args)
+        _backward(args, lse, d_out.view(-1, seqs.n_head, d), *_blocks(d_qkv, seqs, d), seqs)
         return d_qkv, None, None, None, None, None
 
 

@@ -230,6 +230,14 @@ def test_a_weight_of_more_elements_than_32_bits_count():
     torch.cuda.empty_cache()
 
 
+def test_second_derivatives_are_refused():
+    from autoresearch_b200.ops.linear_ce import linear_cross_entropy
+    x, w, t, weight = _inputs(10, 64, 300)
+    x.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(linear_cross_entropy(x, w, t), x, weight, create_graph=True)
+
+
 def test_no_tokens():
     x, w, t, weight = _inputs(0, 64, 300)
     loss, dx, dw = _run(x, w, t, weight, 0.0)

@@ -65,7 +65,10 @@ def test_argument_block_matches_the_header():
     text = (Path(K.__file__).parent / "csrc" / "api.h").read_text()
     body = re.sub(r"//[^\n]*", "", text[text.index("typedef struct ArbPacked"):text.index("} ArbPacked;")])
     fields = [f for line in body[body.index("{") + 1:].split(";") for f in line.split(",") if f.strip()]
+    fields = [re.sub(r"^(const )?(void|int|float|double|long long)", "", f.strip()).strip(" *") for f in fields]
     assert len(fields) == 32 and P._ARGS.size == 8 * len(fields)
+    assert fields[P._GRADS_AT // 8:][:5] == ["d_o", "delta", "dq", "dk", "dv"]
+    assert fields[P._D_OUT_STRIDES_AT // 8:][:2] == ["do_row", "do_head"]
 
 
 def test_backward_formula_against_differences():

@@ -330,6 +330,32 @@ def test_offsets_beyond_32_bits():
     torch.cuda.empty_cache()
 
 
+def test_second_derivatives_are_refused():
+    from autoresearch_b200.ops.packed import PackedSequences, packed_attention, packed_qkv_attention
+    q, k, v, g = (t.requires_grad_(True) for t in _inputs(64, 2, 1, 128))
+    seqs = PackedSequences([0, 64], 64, 2, 1)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(packed_attention(q, k, v, seqs), q, g, create_graph=True)
+    qkv = torch.cat([q, k, v], 1).detach().view(64, -1).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(packed_qkv_attention(qkv, seqs), qkv, g.view(64, -1), create_graph=True)
+
+
+def test_the_same_graph_twice_and_inputs_changed_in_between():
+    from autoresearch_b200.ops.packed import PackedSequences, packed_attention
+    q, k, v, g = _inputs(300, 2, 1, 128)
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    out = packed_attention(q, k, v, PackedSequences([0, 300], 300, 2, 1))
+    a = torch.autograd.grad(out, (q, k, v), g, retain_graph=True)
+    b = torch.autograd.grad(out, (q, k, v), g, retain_graph=True)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    with torch.no_grad():
+        k.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(out, (q, k, v), g)
+
+
 def test_no_rows_and_no_sequences():
     from autoresearch_b200.ops.packed import PackedSequences
     q, k, v, g = _inputs(0, 2, 1, 128)
