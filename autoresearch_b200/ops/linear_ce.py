@@ -13,6 +13,7 @@ forward pass, this form returns per-token losses with any later weighting and ne
 """
 from __future__ import annotations
 
+import functools
 import struct
 
 import torch
@@ -20,6 +21,8 @@ import torch
 from . import kernels as K
 
 _ARGS = struct.Struct("=9q9qd")         # ArbLinearCE of csrc/api.h: 9 pointers, 9 sizes, the soft cap
+_WEIGHT_D, _WEIGHT_D_AT = struct.Struct("=2q"), 7 * 8        # weight, d_logits
+_LDD, _LDD_AT = struct.Struct("=q"), 17 * 8
 PIECE_BYTES = 1 << 29                   # bf16 gradient of a piece of logits
 TILE = 256
 
@@ -42,45 +45,52 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _args(x, w, targets, softcap, part=0, target_score=0, lse=0, loss=0, weight=0, d_logits=0, ldd=0):
-    return _ARGS.pack(x.data_ptr(), w.data_ptr(), targets.data_ptr(), part, target_score, lse, loss, weight, d_logits, x.shape[0],
-                      w.shape[0], x.shape[1], w.shape[0], 0, int(targets.dtype is torch.int64), _ld(x), _ld(w), ldd, softcap)
+@functools.lru_cache(maxsize=256)
+def _backward_plan(rows: int, dim: int, vocab: int):
+    """(ids per piece, row stride of its gradient, fp32 slabs of dx, kernels without those of dx and dw)."""
+    cols = piece_columns(rows, vocab)
+    parts = K.lib().arb_linear_ce_parts(rows, dim, vocab) if cols == vocab else 1
+    return cols, -(-cols // 8) * 8, parts if cols < vocab or parts > 1 else 0, -(-vocab // cols)
 
 
 class LinearCEFn(torch.autograd.Function):
     """Per-row losses [N] fp32.  A weight with a ``main_grad`` takes its gradient up there, as in the other products."""
 
     @staticmethod
-    def forward(ctx, x, w, targets, softcap):
-        N, V = x.shape[0], w.shape[0]
+    def forward(ctx, x, w, targets, softcap, keep):
+        N, D = x.shape
+        V = w.shape[0]
         loss = x.new_empty(N, dtype=torch.float32)
         lse = x.new_empty(N, dtype=torch.float32)
+        xr, wr = _rows(x), _rows(w)
+        args = None
         if N:
-            xr, wr = _rows(x), _rows(w)
             with K.on_device(x.device):
                 if K.pending_pulls:
                     K.flush_pending_pulls()
                 tiles = -(-V // TILE)
                 scratch = x.new_empty((2 * tiles + 1) * N, dtype=torch.float32)
                 part = scratch.data_ptr()
-                K._check(K.lib().arb_linear_ce_fwd(_args(xr, wr, targets, softcap, part, part + 8 * tiles * N, lse.data_ptr(), loss.data_ptr()),
-                                                   K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_fwd")
+                args = _ARGS.pack(xr.data_ptr(), wr.data_ptr(), targets.data_ptr(), part, part + 8 * tiles * N, lse.data_ptr(),
+                                  loss.data_ptr(), 0, 0, N, V, D, V, 0, int(targets.dtype is torch.int64), _ld(xr), _ld(wr), 0, softcap)
+                K._check(K.lib().arb_linear_ce_fwd(args, K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_fwd")
                 K.count_launch()                                     # the product and the join
-        ctx.save_for_backward(x, w, targets, lse)
-        ctx.softcap = softcap
+        if keep:
+            ctx.save_for_backward(x, w, targets)
+            ctx.kept = (args, lse, xr, wr)
         return loss
 
     @staticmethod
     def backward(ctx, g):
         if torch.is_grad_enabled():
             raise RuntimeError("linear cross entropy has no second derivative (create_graph=True)")
-        x, w, targets, lse = ctx.saved_tensors
+        x, w, _ = ctx.saved_tensors
         with K.on_device(x.device):
-            return (*_gradients(x, w, targets, lse, g.contiguous(), ctx.softcap, *ctx.needs_input_grad[:2]), None, None)
+            return (*_gradients(x, w, *ctx.kept, g.contiguous(), *ctx.needs_input_grad[:2]), None, None, None)
 
 
-def _gradients(x, w, targets, lse, g, softcap, need_x, need_w):
-    """(dx, dw); dw is None where the main gradient of w has taken it up."""
+def _gradients(x, w, args, lse, xr, wr, g, need_x, need_w):
+    """(dx, dw); dw is None where the main gradient of w has taken it up.  ``args``: the forward call's block."""
     N, D = x.shape
     V = w.shape[0]
     main = getattr(w, "main_grad", None) if need_w else None
@@ -91,20 +101,18 @@ def _gradients(x, w, targets, lse, g, softcap, need_x, need_w):
         return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w and main is None else None)
     if K.pending_pulls:
         K.flush_pending_pulls()
-    xr, wr = _rows(x), _rows(w)
-    cols = piece_columns(N, V)
-    ldd = -(-cols // 8) * 8
+    cols, ldd, slabs, pieces = _backward_plan(N, D, V)
     d = x.new_empty(N * ldd)
     dx = x.new_empty((N, D)) if need_x else None
     dw = w.new_empty((V, D)) if need_w and main is None else None
     # several pieces meet in fp32, in the order of the vocabulary; a single one may be summed in parts
-    parts = K.lib().arb_linear_ce_parts(N, D, V) if cols == V else 1
-    acc = x.new_empty((parts, N, D), dtype=torch.float32) if need_x and (cols < V or parts > 1) else None
-    ptr = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
-    args = _args(xr, wr, targets, softcap, lse=lse.data_ptr(), weight=g.data_ptr(), d_logits=d.data_ptr(), ldd=ldd)
-    K._check(K.lib().arb_linear_ce_bwd(args, cols, ptr(dx), ptr(acc), ptr(dw), ptr(main), main.stride(0) if main is not None else 0,
-                                       K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_bwd")
-    pieces = -(-V // cols)
+    acc = x.new_empty((slabs, N, D), dtype=torch.float32) if need_x and slabs else None
+    block = bytearray(args)
+    _WEIGHT_D.pack_into(block, _WEIGHT_D_AT, g.data_ptr(), d.data_ptr())
+    _LDD.pack_into(block, _LDD_AT, ldd)
+    K._check(K.lib().arb_linear_ce_bwd(bytes(block), cols, dx.data_ptr() if need_x else 0, acc.data_ptr() if acc is not None else 0,
+                                       dw.data_ptr() if dw is not None else 0, main.data_ptr() if main is not None else 0,
+                                       main.stride(0) if main is not None else 0, K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_bwd")
     K.count_launch(pieces * (1 + need_x + need_w) - 1 + (acc is not None))
     return dx, dw
 
@@ -128,4 +136,5 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
         raise ValueError("x, w and targets must be on one device")
     if not 0.0 <= softcap < float("inf"):
         raise ValueError(f"softcap must be finite and not negative, got {softcap}")
-    return LinearCEFn.apply(x, w, targets.contiguous(), float(softcap))
+    keep = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+    return LinearCEFn.apply(x, w, targets.contiguous(), float(softcap), keep)
