@@ -494,6 +494,8 @@ __device__ __forceinline__ void qkv_post_head(float (&f)[128], const QkvPostArgs
 constexpr float CE_LOG2E = 1.4426950408889634f, CE_LN2 = 0.6931471805599453f;
 // capped scores lie in [-cap, cap]: up to this cap 2^(s - cap) neither overflows nor vanishes in fp32 and no maximum is needed
 constexpr float CE_FIXED_MAX = 40.f;
+// s = cap (1 - 2 r) loses what r = 1/2 + ... rounds: 2^-22 of the cap
+constexpr double CE_MAX_CAP = 100.0;
 __device__ __forceinline__ float ce_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -562,7 +564,7 @@ __host__ __device__ __forceinline__ TileXY tile_of(const GemmArgs& p, int w) {
   if (GROUPED) {
     // CE_GROUP rows of tiles together, column by column: the weight matrix of a large vocabulary outgrows L2, and row by row it would
     // be read from HBM once for every 256 tokens (16384 x 1024 x 131072, forward: 4.88 ms row by row with four warps, 4.25 in groups
-    // of 8 and 3.79 in groups of 16 with eight; boxes under their power cap differ by 10 %)
+    // of 8 and 3.79 in groups of 16 with eight; GPUs under their power cap differ by 10 %)
     const int per = CE_GROUP * p.n_tiles, g = w / per, i = w - g * per;
     const int rows = p.m_tiles - g * CE_GROUP < CE_GROUP ? p.m_tiles - g * CE_GROUP : CE_GROUP;
     t.nt = i / rows;
@@ -1459,7 +1461,7 @@ static int ce_operands(const ArbLinearCE* a, GemmArgs& g, CUtensorMap& ta, CUten
   if (a->rows > 0x7fffff00ll || a->vocab > 0x7fffff00ll || a->dim > 0x7fffff00ll || a->cols > a->vocab - a->col0) return -3;
   if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->w)) & 15) return -4;
   if ((a->ldx % 8) || (a->ldw % 8) || a->ldx < a->dim || a->ldw < a->dim) return -4;
-  if (!(a->softcap >= 0.0)) return -3;
+  if (!(a->softcap >= 0.0 && a->softcap <= CE_MAX_CAP)) return -3;
   if (g_num_sms == 0) {
     int dev = 0;
     cudaGetDevice(&dev);

@@ -76,7 +76,7 @@ def _check(N, D, V, cap, ignored=0.0, seed=0, scale=2.5, wide=True):
 
 @pytest.mark.parametrize("N,D,V", [(1, 8, 1), (1, 64, 2), (3, 8, 255), (255, 72, 256), (256, 128, 257), (257, 256, 1000), (512, 256, 1024),
                                    (700, 200, 5003), (1500, 512, 8192), (130, 384, 50021), (2049, 1024, 2047), (515, 200, 9001), (300, 512, 17003)])
-@pytest.mark.parametrize("cap", [0.0, 15.0, 50.0])
+@pytest.mark.parametrize("cap", [0.0, 15.0, 50.0, 100.0])
 def test_linear_cross_entropy(N, D, V, cap):
     _check(N, D, V, cap, ignored=0.2 if N > 3 else 0.0)
 
