@@ -22,8 +22,6 @@ import torch
 from . import kernels as K
 
 _ARGS = struct.Struct("=31qd")          # ArbPacked of csrc/api.h: 12 pointers, 7 sizes, 12 strides, the scale
-_GRADS, _GRADS_AT = struct.Struct("=5q"), 6 * 8                          # d_o, delta, dq, dk, dv
-_D_OUT_STRIDES, _D_OUT_STRIDES_AT = struct.Struct("=2q"), (12 + 7 + 7) * 8      # do_row, do_head
 MAX_ROWS = 1 << 30
 L2_SPAN_BYTES = 48 << 20                # keys and values whose tiles run together (126 MB of L2; attn_common.cuh)
 
@@ -87,13 +85,13 @@ class PackedSequences:
             raise ValueError("too many tiles for one launch")
         items = 4 * (self.cap_q + self.cap_k)
         self.items = torch.empty(items + 4 * (self.n_seq + 3), dtype=torch.int32, device=self.device)
-        self._items_ptr, self._err_ptr = self.items.data_ptr(), self._err.data_ptr()
+        self._err_ptr = self._err.data_ptr()
         if rows:
             span = max(128, L2_SPAN_BYTES // (512 * min(n_kv_head, 8)))
             with K.on_device(self.device):
                 K._check(K.lib().arb_packed_plan(self.cu_seqlens.data_ptr(), self.n_seq, rows, self.group, span, self.items.data_ptr(),
                                                  self.cap_q, self.cap_k, self.items.data_ptr() + 4 * items,
-                                                 self._err.data_ptr(), K._stream()), "packed_plan")
+                                                 self._err_ptr, K._stream()), "packed_plan")
 
 
 def _layout(t: torch.Tensor):
@@ -111,43 +109,45 @@ def _layout(t: torch.Tensor):
     return t.clone(memory_format=torch.contiguous_format), n1 * d, d
 
 
-def _forward(q, k, v, strides, seqs, window, scale, keep, grad_rows):
-    """(O, lse, what O's rounding left over where ``keep``, argument block).  ``strides``: row and head stride of q, k and v;
-    ``grad_rows``: row strides of dq, dk and dv, whose heads are d apart.  The block holds what the backward call takes as well,
-    but for the tensors that call brings, so that little is left to do on the thread that the backward pass runs on."""
+def _forward(q, k, v, strides, seqs, window, scale, keep):
+    """(O, lse, what O's rounding left over where ``keep``).  ``strides``: row and head stride of q, k and v."""
     rows, H, d = q.shape
     out = q.new_empty((rows, H, d))
     lse = q.new_empty((rows, H), dtype=torch.float32)
     rest = q.new_empty((rows, H, d)) if keep else None
-    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr() if keep else 0, lse.data_ptr(),
-                      0, 0, 0, 0, 0, seqs._items_ptr, rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k,
-                      *strides, H * d, H * d, d, *grad_rows, scale)
     if rows:
-        _launch("arb_packed_attn_fwd", args, seqs)
-    return out, lse, rest, args
+        _launch("arb_packed_attn_fwd", _ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr() if keep else 0, lse.data_ptr(), 0, 0, 0, 0, 0,
+            seqs.items.data_ptr(), rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k,
+            *strides, H * d, 0, 0, 0, 0, 0, scale), seqs)
+    return out, lse, rest
 
 
 def _launch(entry, args, seqs):
-    if seqs.device.index == torch._C._cuda_getDevice():
-        K._check(getattr(K.lib(), entry)(args, seqs._err_ptr, K._stream()), entry)
-        return
-    with torch.cuda.device(seqs.device):
+    with K.on_device(seqs.device):
         K._check(getattr(K.lib(), entry)(args, seqs._err_ptr, K._stream()), entry)
 
 
-def _backward(args, lse, d_out, dq, dk, dv, seqs):
-    """``args``: the forward call's block."""
-    if not seqs.rows:
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _backward(q, k, v, strides, out, lse, rest, d_out, grads, grad_rows, seqs, window, scale):
+    """Writes ``grads`` (dq, dk, dv), whose rows are ``grad_rows`` apart and whose heads are dense.  All that the forward call read
+    or wrote comes in as autograd kept it: hooks on saved tensors (checkpointing, offloading) hand back others than the call had."""
+    rows, H, d = q.shape
+    if not rows:
         return
-    block = bytearray(args)
-    if d_out.is_contiguous() and not d_out.data_ptr() & 15:
-        same = d_out
-    else:
-        same, row, head = _layout(d_out)
-        _D_OUT_STRIDES.pack_into(block, _D_OUT_STRIDES_AT, row, head)
+    for t in (q, k, v, out, lse, rest):
+        if t.device != seqs.device:
+            raise ValueError(f"a saved tensor came back on {t.device}, the sequences are on {seqs.device}")
+    d_out, do_row, do_head = _layout(d_out)
+    out, rest, lse = _dense(out), _dense(rest), _dense(lse)
     delta = lse.new_empty(lse.numel() + 2)
-    _GRADS.pack_into(block, _GRADS_AT, same.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
-    _launch("arb_packed_attn_bwd", bytes(block), seqs)
+    _launch("arb_packed_attn_bwd", _ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), d_out.data_ptr(), delta.data_ptr(),
+        *[g.data_ptr() for g in grads], seqs.items.data_ptr(), rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k,
+        *strides, H * d, do_row, do_head, *grad_rows, scale), seqs)
     K.count_launch()                     # the row sums of dO o O and the gradient grid
 
 
@@ -162,22 +162,21 @@ class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, seqs, window, scale, keep):
         (q, q0, q1), (k, k0, k1), (v, v0, v1) = _layout(q), _layout(k), _layout(v)
-        H, d = q.shape[1:]
-        kv = seqs.n_kv_head * d
-        out, lse, rest, args = _forward(q, k, v, (q0, q1, k0, k1, v0, v1), seqs, window, scale, keep, (H * d, kv, kv))
+        out, lse, rest = _forward(q, k, v, (q0, q1, k0, k1, v0, v1), seqs, window, scale, keep)
         if keep:
-            ctx.save_for_backward(q, k, v, out)
-            ctx.kept = (args, lse, rest, seqs)
+            ctx.save_for_backward(q, k, v, out, lse, rest)
+            ctx.call = (seqs, window, scale)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
         _first_order_only()
-        q, k, _, _ = ctx.saved_tensors
-        args, lse, _, seqs = ctx.kept
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
-        _backward(args, lse, d_out, dq, dk, dv, seqs)
-        return dq, dk, dv, None, None, None, None
+        q, k, v, out, lse, rest = ctx.saved_tensors
+        (q, q0, q1), (k, k0, k1), (v, v0, v1) = _layout(q), _layout(k), _layout(v)
+        grads = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        row, kv_row = q.shape[1] * q.shape[2], k.shape[1] * k.shape[2]
+        _backward(q, k, v, (q0, q1, k0, k1, v0, v1), out, lse, rest, d_out, grads, (row, kv_row, kv_row), *ctx.call)
+        return (*grads, None, None, None, None)
 
 
 class PackedQKVAttentionFn(torch.autograd.Function):
@@ -185,21 +184,22 @@ class PackedQKVAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, seqs, window, scale, d, keep):
-        ld = qkv.shape[1]
-        out, lse, rest, args = _forward(*_blocks(qkv, seqs, d), (ld, d) * 3, seqs, window, scale, keep, (ld,) * 3)
+        out, lse, rest = _forward(*_blocks(qkv, seqs, d), (qkv.shape[1], d) * 3, seqs, window, scale, keep)
         out = out.view(qkv.shape[0], -1)
         if keep:
-            ctx.save_for_backward(qkv, out)
-            ctx.kept = (args, lse, rest, seqs, d)
+            ctx.save_for_backward(qkv, out, lse, rest)
+            ctx.call = (seqs, window, scale)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
         _first_order_only()
-        qkv, _ = ctx.saved_tensors
-        args, lse, _, seqs, d = ctx.kept
-        d_qkv = qkv.new_empty(qkv.shape)
-        _backward(args, lse, d_out.view(-1, seqs.n_head, d), *_blocks(d_qkv, seqs, d), seqs)
+        qkv, out, lse, rest = ctx.saved_tensors
+        qkv, d = _dense(qkv), rest.shape[2]
+        d_qkv, ld = qkv.new_empty(qkv.shape), qkv.shape[1]
+        seqs = ctx.call[0]
+        _backward(*_blocks(qkv, seqs, d), (ld, d) * 3, out, lse, rest, d_out.view(-1, seqs.n_head, d), _blocks(d_qkv, seqs, d), (ld,) * 3,
+                  *ctx.call)
         return d_qkv, None, None, None, None, None
 
 

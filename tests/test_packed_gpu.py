@@ -356,6 +356,66 @@ def test_the_same_graph_twice_and_inputs_changed_in_between():
         torch.autograd.grad(out, (q, k, v), g)
 
 
+class _Elsewhere(torch.autograd.graph.saved_tensors_hooks):
+    """Keeps dense copies of what is saved; ``spoil`` overwrites all the originals."""
+
+    def __init__(self):
+        self.seen = []
+        super().__init__(self._pack, lambda t: t)
+
+    def _pack(self, t):
+        self.seen.append(t)
+        return t.detach().clone(memory_format=torch.contiguous_format)
+
+    def spoil(self):
+        for t in self.seen:
+            t.data.fill_(math.nan)
+
+
+@pytest.mark.parametrize("form", ["separate", "projection"])
+def test_hooks_may_hand_back_other_tensors(form):
+    """What hooks on saved tensors return is read, in its layout, and not the forward call's memory."""
+    from autoresearch_b200.ops.packed import PackedSequences, packed_attention, packed_qkv_attention
+    rows, H, KV, d = 333, 4, 2, 128
+    q, k, v, g = _inputs(rows, H, KV, d)
+    seqs = PackedSequences([0, 200, 333], rows, H, KV)
+    want = torch.cat(_run(q, k, v, g, seqs)[1:], 1)
+    qkv = torch.cat([q, k, v], 1).requires_grad_(True)
+    hooks = _Elsewhere()
+    if form == "separate":
+        parts = qkv[:, :H], qkv[:, H:H + KV], qkv[:, H + KV:]
+        with hooks:
+            out = packed_attention(*parts, seqs)
+        hooks.spoil()
+        got = torch.cat(torch.autograd.grad(out, parts, g), 1)
+    else:
+        flat = qkv.detach().view(rows, -1).requires_grad_(True)
+        with hooks:
+            out = packed_qkv_attention(flat, seqs)
+        hooks.spoil()
+        got = torch.autograd.grad(out, flat, g.view(rows, -1))[0].view(rows, -1, d)
+    assert hooks.seen and torch.equal(got, want)
+
+
+def test_activation_checkpointing():
+    from torch.utils.checkpoint import checkpoint
+
+    from autoresearch_b200.ops.packed import PackedSequences, packed_attention
+    q, k, v, g = _inputs(700, 4, 2, 64)
+    seqs = PackedSequences([0, 333, 700], 700, 4, 2)
+    f = lambda a, b, c: packed_attention(a * 2, b * 0.5, c + 1, seqs)  # noqa: E731
+    grads = []
+    for run in (f, lambda *x: checkpoint(f, *x, use_reentrant=False), lambda *x: checkpoint(f, *x, use_reentrant=True)):
+        x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = run(*x)
+        junk = [torch.full_like(t, math.nan) for t in (q, k, v, g) * 3]          # takes memory that was let go of
+        grads.append(torch.autograd.grad(out, x, g) if run is f else (out.backward(g), *(t.grad for t in x))[1:])
+        del junk
+    for other in grads[1:]:
+        for a, b in zip(other, grads[0]):
+            assert torch.equal(a, b)
+
+
 def test_no_rows_and_no_sequences():
     from autoresearch_b200.ops.packed import PackedSequences
     q, k, v, g = _inputs(0, 2, 1, 128)
