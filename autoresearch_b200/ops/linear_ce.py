@@ -21,8 +21,6 @@ import torch
 from . import kernels as K
 
 _ARGS = struct.Struct("=9q9qd")         # ArbLinearCE of csrc/api.h: 9 pointers, 9 sizes, the soft cap
-_WEIGHT_D, _WEIGHT_D_AT = struct.Struct("=2q"), 7 * 8        # weight, d_logits
-_LDD, _LDD_AT = struct.Struct("=q"), 17 * 8
 PIECE_BYTES = 1 << 29                   # bf16 gradient of a piece of logits
 TILE = 256
 MAX_SOFTCAP = 100.0                     # a capped logit is off by up to 2^-22 of the cap
@@ -64,7 +62,6 @@ class LinearCEFn(torch.autograd.Function):
         loss = x.new_empty(N, dtype=torch.float32)
         lse = x.new_empty(N, dtype=torch.float32)
         xr, wr = _rows(x), _rows(w)
-        args = None
         if N:
             with K.on_device(x.device):
                 if K.pending_pulls:
@@ -77,41 +74,46 @@ class LinearCEFn(torch.autograd.Function):
                 K._check(K.lib().arb_linear_ce_fwd(args, K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_fwd")
                 K.count_launch()                                     # the product and the join
         if keep:
-            ctx.save_for_backward(x, w, targets)
-            ctx.kept = (args, lse, xr, wr)
+            ctx.save_for_backward(xr, wr, targets, lse)
+            ctx.parameter = w if w.is_leaf else None                 # hooks on saved tensors hand back others, without its main gradient
+            ctx.softcap = softcap
         return loss
 
     @staticmethod
     def backward(ctx, g):
         if torch.is_grad_enabled():
             raise RuntimeError("linear cross entropy has no second derivative (create_graph=True)")
-        x, w, _ = ctx.saved_tensors
-        with K.on_device(x.device):
-            return (*_gradients(x, w, *ctx.kept, g.contiguous(), *ctx.needs_input_grad[:2]), None, None, None)
+        x, w, targets, lse = ctx.saved_tensors
+        with K.on_device(g.device):
+            return (*_gradients(x, w, ctx.parameter, targets, lse, g.contiguous(), ctx.softcap, *ctx.needs_input_grad[:2]), None, None, None)
 
 
-def _gradients(x, w, args, lse, xr, wr, g, need_x, need_w):
-    """(dx, dw); dw is None where the main gradient of w has taken it up.  ``args``: the forward call's block."""
+def _gradients(x, w, parameter, targets, lse, g, softcap, need_x, need_w):
+    """(dx, dw); dw is None where the main gradient of the parameter has taken it up.  All that the forward call read or wrote comes
+    in as autograd kept it: hooks on saved tensors (checkpointing, offloading) hand back others than the call had."""
     N, D = x.shape
     V = w.shape[0]
-    main = getattr(w, "main_grad", None) if need_w else None
+    main = getattr(w if parameter is None else parameter, "main_grad", None) if need_w else None
     if main is not None and (main.dtype is not torch.float32 or main.shape != w.shape or main.device != w.device or main.stride(1) != 1
                              or main.stride(0) % 4 or main.data_ptr() & 15):
         raise ValueError(f"main_grad of a {tuple(w.shape)} weight must be fp32 of that shape with unit inner stride and 16-byte aligned rows")
     if not N:
         return (torch.zeros_like(x) if need_x else None), (torch.zeros_like(w) if need_w and main is None else None)
+    for t in (x, w, targets, lse):
+        if t.device != g.device:
+            raise ValueError(f"a saved tensor came back on {t.device}, the gradient is on {g.device}")
     if K.pending_pulls:
         K.flush_pending_pulls()
+    xr, wr, targets, lse = _rows(x), _rows(w), targets.contiguous(), lse.contiguous()
     cols, ldd, slabs, pieces = _backward_plan(N, D, V)
     d = x.new_empty(N * ldd)
     dx = x.new_empty((N, D)) if need_x else None
     dw = w.new_empty((V, D)) if need_w and main is None else None
     # several pieces meet in fp32, in the order of the vocabulary; a single one may be summed in parts
     acc = x.new_empty((slabs, N, D), dtype=torch.float32) if need_x and slabs else None
-    block = bytearray(args)
-    _WEIGHT_D.pack_into(block, _WEIGHT_D_AT, g.data_ptr(), d.data_ptr())
-    _LDD.pack_into(block, _LDD_AT, ldd)
-    K._check(K.lib().arb_linear_ce_bwd(bytes(block), cols, dx.data_ptr() if need_x else 0, acc.data_ptr() if acc is not None else 0,
+    args = _ARGS.pack(xr.data_ptr(), wr.data_ptr(), targets.data_ptr(), 0, 0, lse.data_ptr(), 0, g.data_ptr(), d.data_ptr(),
+                      N, V, D, V, 0, int(targets.dtype is torch.int64), _ld(xr), _ld(wr), ldd, softcap)
+    K._check(K.lib().arb_linear_ce_bwd(args, cols, dx.data_ptr() if need_x else 0, acc.data_ptr() if acc is not None else 0,
                                        dw.data_ptr() if dw is not None else 0, main.data_ptr() if main is not None else 0,
                                        main.stride(0) if main is not None else 0, K.err_flag(x.device).data_ptr(), K._stream()), "linear_ce_bwd")
     K.count_launch(pieces * (1 + need_x + need_w) - 1 + (acc is not None))

@@ -242,6 +242,55 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(linear_cross_entropy(x, w, t), x, weight, create_graph=True)
 
 
+def test_hooks_may_hand_back_other_tensors():
+    """What hooks on saved tensors return is read, in its layout, and not the forward call's memory; the main gradient of a
+    parameter takes its share all the same."""
+    from autoresearch_b200.ops.linear_ce import linear_cross_entropy
+    x, w, t, weight = _inputs(300, 128, 1111, 0.2)
+    _, dx, dw = _run(x, w, t, weight, 15.0)
+    seen = []
+
+    def pack(s):
+        seen.append(s)
+        return s.detach().clone(memory_format=torch.contiguous_format)
+    for main in (False, True):
+        wide = torch.cat([x, x], 1).requires_grad_(True)
+        rows = wide[:, 128:]
+        p = torch.nn.Parameter(w.clone())
+        if main:
+            p.main_grad = torch.zeros(w.shape, device="cuda")
+        at = t.clone()
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda s: s):
+            loss = linear_cross_entropy(rows, p, at, softcap=15.0)
+        for s in seen:
+            s.data.fill_(float("nan") if s.is_floating_point() else -1)
+        loss.backward(weight)
+        assert torch.equal(wide.grad[:, 128:], dx)
+        if main:
+            assert p.grad is None
+            assert float((p.main_grad - dw.float()).norm()) <= 2.0 ** -8 * float(dw.float().norm())
+        else:
+            assert torch.equal(p.grad, dw)
+
+
+def test_activation_checkpointing():
+    from torch.utils.checkpoint import checkpoint
+
+    from autoresearch_b200.ops.linear_ce import linear_cross_entropy
+    x, w, t, weight = _inputs(700, 64, 3001, 0.2)
+    f = lambda a, b: linear_cross_entropy(a * 2, b * 0.5, t + 0, softcap=15.0)  # noqa: E731
+    grads = []
+    for run in (f, lambda *a: checkpoint(f, *a, use_reentrant=False)):
+        a = [s.detach().requires_grad_(True) for s in (x, w)]
+        loss = run(*a)
+        junk = [torch.full_like(s, float("nan")) for s in (x, w)] + [torch.full_like(t, -1) for _ in range(3)]
+        loss.backward(weight)
+        del junk
+        grads.append([s.grad for s in a])
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
 def test_no_tokens():
     x, w, t, weight = _inputs(0, 64, 300)
     loss, dx, dw = _run(x, w, t, weight, 0.0)
