@@ -161,7 +161,7 @@ def test_the_operators_in_a_chain():
     ok = tgt >= 0
     l64 = torch.where(ok, torch.logsumexp(z, 1) - z.gather(1, tgt.clamp(min=0)[:, None])[:, 0], 0.0)
     want = torch.autograd.grad(l64.sum() / N, (w64, h64))
-    assert float((losses.double() - l64).abs().max()) < 0.05
+    assert float((losses.detach().double() - l64.detach()).abs().max()) < 0.05
     tol = 10 * 2.0 ** -8
     norm64 = math.sqrt(sum(float(t.square().sum()) for t in want))
     assert abs(float(norm) - norm64) <= tol * norm64 and norm64 > 0.01

@@ -15,7 +15,7 @@ def test_argument_block_matches_the_header():
     fields = [f for line in body[body.index("{") + 1:].split(";") for f in line.split(",") if f.strip()]
     fields = [re.sub(r"^(const )?(void|float|double|long long)", "", f.strip()).strip(" *") for f in fields]
     assert len(fields) == 19 and L._ARGS.size == 8 * len(fields)
-    assert fields[L._WEIGHT_D_AT // 8:][:2] == ["weight", "d_logits"] and fields[L._LDD_AT // 8] == "ldd"
+    assert " ".join(fields) == "x w targets part target_score lse loss weight d_logits rows cols dim vocab col0 targets_64 ldx ldw ldd softcap"
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (512, 1024), (16384, 65536), (16384, 65537), (1 << 20, 131072), (1 << 24, 300), (7, 50021)])

@@ -67,8 +67,8 @@ def test_argument_block_matches_the_header():
     fields = [f for line in body[body.index("{") + 1:].split(";") for f in line.split(",") if f.strip()]
     fields = [re.sub(r"^(const )?(void|int|float|double|long long)", "", f.strip()).strip(" *") for f in fields]
     assert len(fields) == 32 and P._ARGS.size == 8 * len(fields)
-    assert fields[P._GRADS_AT // 8:][:5] == ["d_o", "delta", "dq", "dk", "dv"]
-    assert fields[P._D_OUT_STRIDES_AT // 8:][:2] == ["do_row", "do_head"]
+    assert " ".join(fields) == ("q k v o o_lo lse d_o delta dq dk dv items rows KV G D window cap_q cap_k q_row q_head k_row k_head "
+                                "v_row v_head o_row do_row do_head dq_row dk_row dv_row scale")
 
 
 def test_backward_formula_against_differences():
