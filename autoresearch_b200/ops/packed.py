@@ -69,7 +69,10 @@ class PackedSequences:
             if not values:
                 raise ValueError("cu_seqlens needs at least one bound")
             check_bounds(values, rows)
-            cu_seqlens = torch.tensor(values, dtype=torch.int32, device=device if device is not None else "cuda")
+            device = torch.device(device if device is not None else "cuda")
+            if device.type != "cuda":
+                raise ValueError(f"the sequences must be packed on a CUDA device, not {device}")
+            cu_seqlens = torch.tensor(values, dtype=torch.int32, device=device)
         elif cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype is not torch.int32:
             raise TypeError("cu_seqlens must be a 1-D int32 tensor of at least one element")
         self.cu_seqlens = cu_seqlens.contiguous()

@@ -36,6 +36,13 @@ def test_bounds_that_are_no_whole_numbers():
             P.PackedSequences(bad, 4, 2, 1)
 
 
+@pytest.mark.parametrize("device", ["cpu", torch.device("cpu"), "meta"])
+def test_packing_on_another_kind_of_device_is_refused(device):
+    """Before anything is launched: the plan kernel would be given host addresses."""
+    with pytest.raises(ValueError, match="CUDA device"):
+        P.PackedSequences([0, 4], 4, 2, 1, device=device)
+
+
 def test_cpu_tensors_are_refused():
     t = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
     with pytest.raises(TypeError, match="CUDA"):
