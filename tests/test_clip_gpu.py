@@ -160,6 +160,19 @@ def test_tensors_that_were_given_other_memory():
     assert abs(float(grad_norm(s)) - want) <= 2.0 ** -19 * want
 
 
+def test_a_copy_of_a_set_scales_its_own_tensors():
+    import copy
+
+    from autoresearch_b200.optim.clip import GradSet, clip_grad_norm
+    grads = _grads(SIZES[:6], torch.float32)
+    source = [t.clone() for t in grads]
+    other = copy.deepcopy(GradSet(grads))
+    norm = clip_grad_norm(other, 0.25 * _norm(source))
+    assert abs(float(norm) - _norm(source)) <= 2.0 ** -19 * _norm(source)
+    assert all(torch.equal(a, b) for a, b in zip(grads, source))
+    _check_scaled(other.tensors, source, 0.25)
+
+
 def test_more_elements_than_32_bits_count():
     from autoresearch_b200.optim.clip import clip_grad_norm
     n = (1 << 31) + 4099
