@@ -188,7 +188,7 @@ class PackedQKVAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, seqs, window, scale, d, keep):
         out, lse, rest = _forward(*_blocks(qkv, seqs, d), (qkv.shape[1], d) * 3, seqs, window, scale, keep)
-        out = out.view(qkv.shape[0], -1)
+        out = out.view(qkv.shape[0], seqs.n_head * d)
         if keep:
             ctx.save_for_backward(qkv, out, lse, rest)
             ctx.call = (seqs, window, scale)

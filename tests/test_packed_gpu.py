@@ -425,6 +425,16 @@ def test_no_rows_and_no_sequences():
         assert bool((x == 0).all())
 
 
+def test_no_rows_in_the_projection_form():
+    from autoresearch_b200.ops.packed import PackedSequences, packed_qkv_attention
+    for heads, d in ((2, 64), (4, 128)):
+        qkv = torch.zeros(0, (heads + 2) * d, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        out = packed_qkv_attention(qkv, PackedSequences([0], 0, heads, 1), head_dim=d)
+        assert out.shape == (0, heads * d)
+        out.sum().backward()
+        assert qkv.grad.shape == qkv.shape
+
+
 def test_refusals():
     from autoresearch_b200.ops.packed import PackedSequences, packed_attention, packed_qkv_attention
     rows, H, KV, d = 64, 4, 2, 128
