@@ -1287,8 +1287,10 @@ static int make_key_tmap(CUtensorMap* m, const void* base, const ArbPacked& a, l
 }
 
 static int check_packed(const ArbPacked& a) {
+  // masked scores are -inf, rows take the largest score; in fp32 neither the scale nor its reciprocal nears the ends of the range
+  constexpr double TOP = 18446744073709551616.0;         // 2^64
+  if (!(a.scale >= 1.0 / TOP && a.scale <= TOP)) return -3;
   // positions plus a window stay within 31 bits
-  if (!(a.scale > 0.0)) return -3;                       // masked scores are -inf, rows take the largest score
   if (a.rows <= 0 || a.rows > PACKED_MAX_ROWS || a.KV <= 0 || a.KV > 65535 || a.G <= 0 || a.G > 128 || (a.D != 64 && a.D != 128) || a.window < 0) return -3;
   if (!a.items || bad_ptr(a.items) || a.cap_q <= 0 || a.cap_k <= 0 || (a.cap_q + a.cap_k) * a.KV > 0x7fffffffll) return -3;
   const void* ptrs[] = {a.q, a.k, a.v, a.o, a.o_lo, a.d_o, a.dq, a.dk, a.dv};

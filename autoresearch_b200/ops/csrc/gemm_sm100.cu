@@ -496,6 +496,7 @@ constexpr float CE_LOG2E = 1.4426950408889634f, CE_LN2 = 0.6931471805599453f;
 constexpr float CE_FIXED_MAX = 40.f;
 // s = cap (1 - 2 r) loses what r = 1/2 + ... rounds: 2^-22 of the cap
 constexpr double CE_MAX_CAP = 100.0;
+constexpr double CE_MIN_CAP = 1.0 / 18446744073709551616.0;      // 2^-64: 1 / cap is a normal fp32 number
 __device__ __forceinline__ float ce_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -1461,7 +1462,7 @@ static int ce_operands(const ArbLinearCE* a, GemmArgs& g, CUtensorMap& ta, CUten
   if (a->rows > 0x7fffff00ll || a->vocab > 0x7fffff00ll || a->dim > 0x7fffff00ll || a->cols > a->vocab - a->col0) return -3;
   if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->w)) & 15) return -4;
   if ((a->ldx % 8) || (a->ldw % 8) || a->ldx < a->dim || a->ldw < a->dim) return -4;
-  if (!(a->softcap >= 0.0 && a->softcap <= CE_MAX_CAP)) return -3;
+  if (a->softcap != 0.0 && !(a->softcap >= CE_MIN_CAP && a->softcap <= CE_MAX_CAP)) return -3;
   if (g_num_sms == 0) {
     int dev = 0;
     cudaGetDevice(&dev);

@@ -24,6 +24,7 @@ _ARGS = struct.Struct("=9q9qd")         # ArbLinearCE of csrc/api.h: 9 pointers,
 PIECE_BYTES = 1 << 29                   # bf16 gradient of a piece of logits
 TILE = 256
 MAX_SOFTCAP = 100.0                     # a capped logit is off by up to 2^-22 of the cap
+MIN_SOFTCAP = 2.0 ** -64                # its reciprocal is a normal fp32 number, and the cap is not taken for none
 
 
 def piece_columns(rows: int, vocab: int) -> int:
@@ -124,7 +125,7 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     """Per-token losses [N] (fp32) of the head ``w`` [V, D] on ``x`` [N, D], both bf16, D a multiple of 8; differentiable in both.
 
     ``targets`` [N], int32 or int64: a value outside of [0, V) marks a token that does not count (loss 0, no gradient).
-    ``softcap`` > 0 (at most 100): the logits are softcap * tanh(. / softcap).  Every row of ``x`` has to be finite, those that do not count
+    ``softcap`` > 0 (2^-64 to 100): the logits are softcap * tanh(. / softcap).  Every row of ``x`` has to be finite, those that do not count
     too: the gradient of ``w`` sums over all of them."""
     K._bf16(x, "x")
     K._bf16(w, "w")
@@ -137,7 +138,7 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
         raise ValueError(f"targets must be int32 or int64 [{N}], got {targets.dtype} {tuple(targets.shape)}")
     if w.device != x.device or targets.device != x.device:
         raise ValueError("x, w and targets must be on one device")
-    if not 0.0 <= softcap <= MAX_SOFTCAP:
-        raise ValueError(f"softcap must lie in [0, {MAX_SOFTCAP}], got {softcap}")
+    if softcap != 0 and not MIN_SOFTCAP <= softcap <= MAX_SOFTCAP:
+        raise ValueError(f"softcap must be 0 or lie in [{MIN_SOFTCAP}, {MAX_SOFTCAP}], got {softcap}")
     keep = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
     return LinearCEFn.apply(x, w, targets.contiguous(), float(softcap), keep)

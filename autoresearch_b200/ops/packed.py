@@ -23,6 +23,8 @@ from . import kernels as K
 
 _ARGS = struct.Struct("=31qd")          # ArbPacked of csrc/api.h: 12 pointers, 7 sizes, 12 strides, the scale
 MAX_ROWS = 1 << 30
+MIN_SCALE = 2.0 ** -64                  # in fp32 neither it nor its reciprocal nears the ends of the range (a score that is not seen
+                                        # is -inf times the scale: NaN for a scale that has become 0)
 L2_SPAN_BYTES = 48 << 20                # keys and values whose tiles run together (126 MB of L2; attn_common.cuh)
 
 
@@ -223,8 +225,8 @@ def _common(device, rows, d, seqs, window, scale):
         window = rows
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
-    if scale is not None and not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if scale is not None and not MIN_SCALE <= scale <= 1.0 / MIN_SCALE:
+        raise ValueError(f"scale must be positive and lie in [{MIN_SCALE}, {1.0 / MIN_SCALE}], got {scale}")
     return min(int(window), rows), 1.0 / math.sqrt(d) if scale is None else float(scale)
 
 
@@ -233,8 +235,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: Pa
     """Attention of packed sequences: q [rows, H, d], k and v [rows, KV, d], bf16, d = 64 or 128, any strides -> [rows, H, d].
 
     Query head h reads key head h // (H / KV).  ``window``: how many positions back a query sees (None: all); ``scale``
-    (positive) defaults to 1 / sqrt(d).  The inputs of a sequence reach no other sequence's outputs or gradients, not even as NaN.
-    Within a sequence every row has to be finite: a weight of zero does not silence a NaN in a later key's value."""
+    (positive, 2^-64 to 2^64) defaults to 1 / sqrt(d).  The inputs of a sequence reach no other sequence's outputs or gradients, not even as NaN.
+    Within a sequence every row has to be finite: a weight of zero does not silence a NaN in a later key's value.  Scores are
+    fp32 and have to stay below 2^30 in magnitude (their rounding, 2^-24 of the score, is a relative error of the weights)."""
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         K._bf16(t, name)
         if t.dim() != 3:

@@ -40,7 +40,8 @@ def no_device_check(monkeypatch):
 
 @pytest.mark.parametrize("x,w,t,cap", [((4, 8), (5, 16), 4, 0.0), ((4, 12), (5, 12), 4, 0.0), ((4, 0), (5, 0), 4, 0.0), ((4, 8), (0, 8), 4, 0.0),
                                        ((4, 8), (5, 8), 3, 0.0), ((4, 8), (5, 8), 4, -1.0), ((4, 8), (5, 8), 4, float("inf")),
-                                       ((4, 8), (5, 8), 4, float("nan")), ((4, 8), (5, 8), 4, 101.0)])
+                                       ((4, 8), (5, 8), 4, float("nan")), ((4, 8), (5, 8), 4, 101.0), ((4, 8), (5, 8), 4, 2.0 ** -65),
+                                       ((4, 8), (5, 8), 4, 5e-324), ((4, 8), (5, 8), 4, -0.5)])
 def test_shapes_and_caps_that_are_refused(no_device_check, x, w, t, cap):
     with pytest.raises(ValueError):
         L.linear_cross_entropy(torch.zeros(x, dtype=torch.bfloat16), torch.zeros(w, dtype=torch.bfloat16), torch.zeros(t, dtype=torch.int64), cap)

@@ -100,6 +100,11 @@ def test_logits_far_apart(cap):
     _check(400, 128, 3000, cap, scale=40.0)
 
 
+@pytest.mark.parametrize("cap", [2.0 ** -64, 2.0 ** -10])
+def test_small_caps(cap):
+    _check(257, 64, 600, cap, 0.1)
+
+
 def test_pieces_of_the_vocabulary(monkeypatch):
     """Pieces that end inside a tile and a last piece of a single id give what one piece gives."""
     from autoresearch_b200.ops import linear_ce as L

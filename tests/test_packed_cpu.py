@@ -51,6 +51,15 @@ def test_cpu_tensors_are_refused():
         P.packed_qkv_attention(t.view(4, -1), None)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.5, 5e-324, 1e-50, 2.0 ** -65, 2.0 ** 65, 1e300, math.inf, math.nan])
+def test_scales_that_fp32_does_not_hold_are_refused(scale):
+    seqs = object.__new__(P.PackedSequences)
+    seqs.rows, seqs.device = 4, torch.device("cpu")
+    assert P._common(seqs.device, 4, 64, seqs, None, 2.0 ** -64) == (4, 2.0 ** -64)
+    with pytest.raises(ValueError, match="scale"):
+        P._common(seqs.device, 4, 64, seqs, None, scale)
+
+
 def test_strides_that_the_copy_engine_can_read():
     t = torch.zeros(6, 3, 64, dtype=torch.bfloat16)
     same, row, head = P._layout(t)

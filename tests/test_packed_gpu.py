@@ -176,6 +176,12 @@ def test_scale_is_the_callers():
     _check([400], 2, 1, 128, scale=0.02)
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -64, 2.0 ** -30])
+def test_small_scales(scale):
+    """Every key counts alike."""
+    _check([300, 1, 77], 4, 2, 64, window=200, scale=scale)
+
+
 @pytest.mark.parametrize("H,KV,d", [(2, 2, 128), (6, 2, 64), (8, 2, 128)])
 def test_a_sequence_does_not_see_its_neighbours(H, KV, d):
     """Bit for bit the same alone, beside other sequences, and beside NaN and infinities in them and in the rows behind."""
