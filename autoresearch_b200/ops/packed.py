@@ -91,12 +91,13 @@ class PackedSequences:
         items = 4 * (self.cap_q + self.cap_k)
         self.items = torch.empty(items + 4 * (self.n_seq + 3), dtype=torch.int32, device=self.device)
         self._err_ptr = self._err.data_ptr()
-        if rows:
-            span = max(128, L2_SPAN_BYTES // (512 * min(n_kv_head, 8)))
-            with K.on_device(self.device):
+        with K.on_device(self.device):
+            self._stream = K._stream()
+            if rows:
+                span = max(128, L2_SPAN_BYTES // (512 * min(n_kv_head, 8)))
                 K._check(K.lib().arb_packed_plan(self.cu_seqlens.data_ptr(), self.n_seq, rows, self.group, span, self.items.data_ptr(),
                                                  self.cap_q, self.cap_k, self.items.data_ptr() + 4 * items,
-                                                 self._err_ptr, K._stream()), "packed_plan")
+                                                 self._err_ptr, self._stream), "packed_plan")
 
 
 def _layout(t: torch.Tensor):
@@ -130,7 +131,10 @@ def _forward(q, k, v, strides, seqs, window, scale, keep):
 
 def _launch(entry, args, seqs):
     with K.on_device(seqs.device):
-        K._check(getattr(K.lib(), entry)(args, seqs._err_ptr, K._stream()), entry)
+        stream = K._stream()
+        if stream != seqs._stream:       # the lists' memory is the other stream's: not given away before this one is done with it
+            seqs.items.record_stream(torch.cuda.current_stream())
+        K._check(getattr(K.lib(), entry)(args, seqs._err_ptr, stream), entry)
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:

@@ -318,6 +318,24 @@ def test_other_stream():
         assert torch.equal(x, y)
 
 
+def test_lists_outlive_the_work_of_another_stream():
+    """A packing that is dropped while another stream still has work with it: its memory is not given away before that is done."""
+    from autoresearch_b200.ops.packed import PackedSequences, packed_attention
+    q, k, v, _ = _inputs(1000, 2, 1, 128)
+    seqs = PackedSequences([0] * 20_000 + [1000], 1000, 2, 1)
+    at, n = seqs.items.data_ptr(), seqs.items.numel()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.no_grad():
+        torch.cuda._sleep(200_000_000)                     # about 0.1 s
+        out = packed_attention(q, k, v, seqs)
+    del seqs
+    held = [torch.empty(n, dtype=torch.int32, device="cuda") for _ in range(64)]
+    assert not s.query() and at not in [t.data_ptr() for t in held]
+    s.synchronize()
+    del out, held
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^31 elements of q: the last sequences come out as they do alone."""
     from autoresearch_b200.ops.packed import PackedSequences
