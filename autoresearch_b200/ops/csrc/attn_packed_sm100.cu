@@ -292,21 +292,29 @@ __device__ __forceinline__ void load_q(uint8_t* dst, const CUtensorMap* m, uint6
 // bytes a column of shared memory of the warp's own, so that neighbouring lanes write neighbouring bytes and not each 16 bytes of
 // another row (32768 rows, window 256, 8 heads on 4: forward with both parts of O 131 -> 121 us, backward 316 -> 291 us).
 template <int COLS>
-__device__ __forceinline__ void store_rows(__nv_bfloat16* dst, long long off, const uint32_t* w, uint32_t stage, int lane) {
+__device__ __forceinline__ uint32_t stage_at(uint32_t stage, int row, int piece) {
   constexpr int PIECES = COLS / 8;                       // 16 bytes each
-  // pieces of a row change places with its number, so that eight lanes meet no bank twice
-  auto at = [&](int row, int piece) { return stage + uint32_t(row * COLS * 2 + ((piece ^ (PIECES == 8 ? row & 7 : (row >> 1) & 3)) << 4)); };
-  __syncwarp();                                          // the previous use has been read
+  // pieces of a row change places with its number, so that eight lanes meet no bank twice; as the copy engine's swizzles do
+  return stage + uint32_t(row * COLS * 2 + ((piece ^ (PIECES == 8 ? row & 7 : (row >> 1) & 3)) << 4));
+}
+template <int COLS>
+__device__ __forceinline__ void stage_rows(const uint32_t* w, uint32_t stage, int lane) {
 #pragma unroll
-  for (int j = 0; j < PIECES; ++j)
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(lane, j)), "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+  for (int j = 0; j < COLS / 8; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_at<COLS>(stage, lane, j)), "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+}
+template <int COLS>
+__device__ __forceinline__ void store_rows(__nv_bfloat16* dst, long long off, const uint32_t* w, uint32_t stage, int lane) {
+  constexpr int PIECES = COLS / 8;
+  __syncwarp();                                          // the previous use has been read
+  stage_rows<COLS>(w, stage, lane);
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int row = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
     const long long o = __shfl_sync(0xffffffffu, off, row);
     uint4 u;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at(row, piece)) : "memory");
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(stage_at<COLS>(stage, row, piece)) : "memory");
     if (o >= 0) *reinterpret_cast<uint4*>(dst + o + piece * 8) = u;
   }
 }
@@ -357,7 +365,8 @@ struct QueryTile {
 template <int D>
 __global__ void __launch_bounds__(ATT_THREADS, 2)
 attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const PackedArgs p) {
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                  const __grid_constant__ CUtensorMap tmR, const PackedArgs p) {
   using L = PackedFwdSmem<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {   // the swizzled tiles need 1 KB alignment; nothing has been allocated yet
@@ -600,27 +609,40 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int head = slot.kv * p.G + (r - at * p.G);
       const long long off = live_row ? (long long)(slot.start + pos) * p.ldo + (long long)head * D : -1;
       const uint32_t stage = smem_u32(smem + L::OUT) + uint32_t(q) * 4096u;
+      const bool whole = 32 % p.G == 0 && __all_sync(0xffffffffu, live_row);
 #pragma unroll 1
-      for (int cc = 0; cc < D; cc += 64) {
-        uint32_t v[32], w[32], rest[32];
+      for (int cc = 0; cc < D; cc += 32) {
+        uint32_t v[32], w[16], rest[16];
+        tmem_ld32(TM_O + lane_addr + uint32_t(cc), v);
+        tmem_wait_ld();
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          tmem_ld32(TM_O + lane_addr + uint32_t(cc + hf * 32), v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float x = __uint_as_float(v[2 * j]) * inv_l, y = __uint_as_float(v[2 * j + 1]) * inv_l;
-            const uint32_t u = pack_bf16(x, y);
-            const float2 r2 = unpack_bf16(u);
-            w[hf * 16 + j] = u;
-            rest[hf * 16 + j] = pack_bf16(x - r2.x, y - r2.y);
-          }
+        for (int j = 0; j < 16; ++j) {
+          const float x = __uint_as_float(v[2 * j]) * inv_l, y = __uint_as_float(v[2 * j + 1]) * inv_l;
+          w[j] = pack_bf16(x, y);
+          const float2 r2 = unpack_bf16(w[j]);
+          rest[j] = pack_bf16(x - r2.x, y - r2.y);
         }
-        store_rows<64>(p.o + cc, off, w, stage, lane);
-        if (p.o_lo) store_rows<64>(p.o_lo + cc, off, rest, stage, lane);
+        if (lane == 0) tma_store_wait_read();              // the columns before have left the stage
+        if (whole) {
+          __syncwarp();
+          stage_rows<32>(w, stage, lane);
+          if (p.o_lo) stage_rows<32>(rest, stage + 2048u, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            const int row = slot.start + qt.m0 + q * (32 / p.G);
+            tma_store_4d(&tmO, smem + L::OUT + q * 4096, cc, 0, slot.kv, row);
+            if (p.o_lo) tma_store_4d(&tmR, smem + L::OUT + q * 4096 + 2048, cc, 0, slot.kv, row);
+            tma_store_commit();
+          }
+        } else {
+          store_rows<32>(p.o + cc, off, w, stage, lane);
+          if (p.o_lo) store_rows<32>(p.o_lo + cc, off, rest, stage + 2048u, lane);
+        }
       }
       if (live_row) p.lse[(long long)(slot.start + pos) * H + head] = (l > 0.f) ? (m_used * p.scale + __logf(l)) : -INFINITY;
     }
+    if (lane == 0) tma_store_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -1279,6 +1301,13 @@ static int make_group_tmap(CUtensorMap* m, const void* base, const ArbPacked& a,
   uint32_t box[4] = {64, uint32_t(a.G), 1, P};
   return make_tmap_bf16(m, base, 4, dims, str, box);
 }
+// the same of the output; one box is 32 columns of the 32 rows of a warp (G divides 32)
+static int make_out_tmap(CUtensorMap* m, const void* base, const ArbPacked& a) {
+  uint64_t dims[4] = {uint64_t(a.D), uint64_t(a.G), uint64_t(a.KV), uint64_t(a.rows)};
+  uint64_t str[3] = {uint64_t(a.D) * 2, uint64_t(a.D) * uint64_t(a.G) * 2, uint64_t(a.o_row) * 2};
+  uint32_t box[4] = {32, uint32_t(a.G), 1, 32 / uint32_t(a.G)};
+  return make_tmap_bf16(m, base, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
 static int make_key_tmap(CUtensorMap* m, const void* base, const ArbPacked& a, long long row, long long head) {
   uint64_t dims[3] = {uint64_t(a.D), uint64_t(a.KV), uint64_t(a.rows)};
   uint64_t str[2] = {uint64_t(head) * 2, uint64_t(row) * 2};
@@ -1327,15 +1356,19 @@ template <int D>
 static int packed_fwd(const ArbPacked& a, int* err, cudaStream_t stream) {
   static PerDeviceOnce cfg;
   if (cfg.first()) { if (int r = set_smem(attn_packed_fwd_k<D>, PackedFwdSmem<D>::TOTAL)) return r; }
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to{}, tr{};
   int r;
   if ((r = make_group_tmap(&tq, a.q, a, a.q_row, a.q_head))) return 1000 + r;
   if ((r = make_key_tmap(&tk, a.k, a, a.k_row, a.k_head))) return 1000 + r;
   if ((r = make_key_tmap(&tv, a.v, a, a.v_row, a.v_head))) return 1000 + r;
+  if (32 % a.G == 0) {
+    if ((r = make_out_tmap(&to, a.o, a))) return 1000 + r;
+    if (a.o_lo && (r = make_out_tmap(&tr, a.o_lo, a))) return 1000 + r;
+  }
   PackedArgs p = packed_args(a, err);
   p.o = reinterpret_cast<__nv_bfloat16*>(a.o); p.ldo = a.o_row;
   p.o_lo = reinterpret_cast<__nv_bfloat16*>(a.o_lo);
-  return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(a.cap_q * a.KV), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk, tv, p);
+  return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(a.cap_q * a.KV), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk, tv, to, tr, p);
 }
 
 template <int D>

@@ -26,7 +26,7 @@ inline EncodeTiledFn get_encode_fn() {
 // Returns 0 on success, the CUresult (or -1) otherwise.
 inline int make_tmap_typed(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                            const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapDataType dtype,
-                           bool swizzle128 = true) {
+                           CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -1;
   // The encoder is a driver call and needs a context current in the calling thread.  A thread that has made no
@@ -44,7 +44,7 @@ inline int make_tmap_typed(CUtensorMap* out, const void* base, int rank, const u
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides_bytes[i];
   auto encode = [&]() {
     return fn(out, dtype, cuuint32_t(rank), const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
@@ -56,8 +56,9 @@ inline int make_tmap_typed(CUtensorMap* out, const void* base, int rank, const u
 }
 
 inline int make_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
-                          const uint64_t* strides_bytes, const uint32_t* box, bool swizzle128 = true) {
-  return make_tmap_typed(out, base, rank, dims, strides_bytes, box, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, swizzle128);
+                          const uint64_t* strides_bytes, const uint32_t* box,
+                          CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+  return make_tmap_typed(out, base, rank, dims, strides_bytes, box, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, swizzle);
 }
 
 }  // namespace arb
