@@ -163,7 +163,7 @@ int arb_attn_bwd(const void* q, const void* k, const void* v, const void* o, con
 // together stay in L2.
 typedef struct ArbPacked {
   const void *q, *k, *v;
-  void *o, *o_lo;                    // o_lo: what rounding left over of o, which the backward pass reads; null where none follows
+  void *o, *o_lo;                    // o_lo: what rounding left over of o (8 bits an element), which the backward pass reads; null where none follows
   float* lse;
   const void* d_o;                   // backward, as everything down to dv
   float* delta;                      // scratch of rows x KV x G + 2 words

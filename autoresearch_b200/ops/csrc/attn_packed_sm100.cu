@@ -39,7 +39,7 @@ struct PackedArgs {
   float scale;
   __nv_bfloat16* o;                  // forward: O; backward: dQ.  Row stride in elements, heads D apart
   long long ldo;
-  __nv_bfloat16* o_lo;               // forward: what the rounding of O to bf16 left over, or null
+  int8_t* o_lo;                      // forward: what the rounding of O to bf16 left over (rest_of), or null
   int* next;                         // backward: [2] next tile of the key and of the query list
   float* lse;                        // [rows, H]
   const float* delta;                // [rows, H]
@@ -288,6 +288,19 @@ __device__ __forceinline__ void load_q(uint8_t* dst, const CUtensorMap* m, uint6
   if (D == 128) tma_load_4d(dst + 16384, m, bar, 64, 0, kv, row);
 }
 
+// What four fp32 values lose when they are rounded to bf16 (as the pairs w01, w23), in steps of 2^-8 of the last bf16 bit: a byte
+// each.  In the integers that hold them a value is (bf16 << 16) + what is left; that is kept to 8 of its 16 bits, which leaves
+// 2^-16 of the value (2^-15 where the byte would be 128).  0 stands for none.
+__device__ __forceinline__ uint32_t rest_of(const uint32_t* v, uint32_t w01, uint32_t w23) {
+  const int a = min(int(v[0] - (w01 << 16) + 128u), 32767), b = min(int(v[1] - (w01 & 0xffff0000u) + 128u), 32767);
+  const int c = min(int(v[2] - (w23 << 16) + 128u), 32767), d = min(int(v[3] - (w23 & 0xffff0000u) + 128u), 32767);
+  return __byte_perm(__byte_perm(uint32_t(a), uint32_t(b), 0x0051), __byte_perm(uint32_t(c), uint32_t(d), 0x0051), 0x5410);
+}
+// a value from its bf16 bits (upper half of `hi`, lower half zero) and byte k of `rest`
+__device__ __forceinline__ float with_rest(uint32_t hi, uint32_t rest, int k) {
+  return __uint_as_float(hi + (uint32_t(int(rest << (24 - 8 * k)) >> 24) << 8));
+}
+
 // 32 rows of COLS (32 or 64) bf16 columns, a row in each lane, to rows `off` elements from `dst` (off < 0: not written).  Through 64
 // bytes a column of shared memory of the warp's own, so that neighbouring lanes write neighbouring bytes and not each 16 bytes of
 // another row (32768 rows, window 256, 8 heads on 4: forward with both parts of O 131 -> 121 us, backward 316 -> 291 us).
@@ -426,7 +439,7 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       } else if (tile.it.tile < 0) {                     // rows of no sequence
         request();
         zero_out(p.o + (long long)kv * p.G * D, p.ldo, start, len, p.G * D, lane);
-        if (p.o_lo) zero_out(p.o_lo + (long long)kv * p.G * D, p.ldo, start, len, p.G * D, lane);
+        if (p.o_lo) zero_out(reinterpret_cast<__nv_bfloat16*>(p.o_lo + (long long)kv * p.G * D), p.ldo / 2, start, len, p.G * D / 2, lane);
         for (int e = lane; e < len * p.G; e += 32) p.lse[(long long)(start + e / p.G) * H + kv * p.G + e % p.G] = -INFINITY;
       } else {
         const QueryTile qt(p, len, tile.it.tile);
@@ -612,21 +625,25 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const bool whole = 32 % p.G == 0 && __all_sync(0xffffffffu, live_row);
 #pragma unroll 1
       for (int cc = 0; cc < D; cc += 32) {
-        uint32_t v[32], w[16], rest[16];
+        uint32_t v[32], w[16], rest[8];
         tmem_ld32(TM_O + lane_addr + uint32_t(cc), v);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float x = __uint_as_float(v[2 * j]) * inv_l, y = __uint_as_float(v[2 * j + 1]) * inv_l;
-          w[j] = pack_bf16(x, y);
-          const float2 r2 = unpack_bf16(w[j]);
-          rest[j] = pack_bf16(x - r2.x, y - r2.y);
-        }
+        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * inv_l);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rest[j] = rest_of(v + 4 * j, w[2 * j], w[2 * j + 1]);
         if (lane == 0) tma_store_wait_read();              // the columns before have left the stage
         if (whole) {
           __syncwarp();
           stage_rows<32>(w, stage, lane);
-          if (p.o_lo) stage_rows<32>(rest, stage + 2048u, lane);
+          if (p.o_lo) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + 2048u + uint32_t(lane * 32 + j * 16)), "r"(rest[4 * j]),
+                           "r"(rest[4 * j + 1]), "r"(rest[4 * j + 2]), "r"(rest[4 * j + 3]) : "memory");
+          }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -637,7 +654,11 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         } else {
           store_rows<32>(p.o + cc, off, w, stage, lane);
-          if (p.o_lo) store_rows<32>(p.o_lo + cc, off, rest, stage + 2048u, lane);
+          if (p.o_lo && live_row) {
+            uint4* dst = reinterpret_cast<uint4*>(p.o_lo + off + cc);
+            dst[0] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+            dst[1] = make_uint4(rest[4], rest[5], rest[6], rest[7]);
+          }
         }
       }
       if (live_row) p.lse[(long long)(slot.start + pos) * H + head] = (l > 0.f) ? (m_used * p.scale + __logf(l)) : -INFINITY;
@@ -1263,28 +1284,30 @@ attn_packed_bwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 }
 
 // delta[row, head] = sum_d dO * O in fp32, with the part of O that its rounding left over: dS = P (dP - delta) cancels, and the error
-// of delta would add as much to dQ and dK as the rounding of dS itself.  D / 8 lanes per (row, head).  Also starts the two lists of
+// of delta would add as much to dQ and dK as the rounding of dS itself.  D / 16 lanes per (row, head).  Also starts the two lists of
 // the kernel behind it.
 template <int D>
-__global__ void __launch_bounds__(256) attn_packed_delta_k(const __nv_bfloat16* o, const __nv_bfloat16* o_lo, long long ldo,
+__global__ void __launch_bounds__(256) attn_packed_delta_k(const __nv_bfloat16* o, const int8_t* o_lo, long long ldo,
                                                            const __nv_bfloat16* d_o, long long row_do, long long head_do, float* delta, int* next,
                                                            long long n, int H) {
-  constexpr int LANES = D / 8;
+  constexpr int LANES = D / 16;
   grid_enter();
   if (blockIdx.x == 0 && threadIdx.x < 2) next[threadIdx.x] = 0;
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const long long i = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int l = threadIdx.x % LANES;
   float acc = 0.f;
   if (i < n) {
-    const long long row = i / H, head = i - row * H;
-    const uint4 a = *reinterpret_cast<const uint4*>(o + row * ldo + head * D + l * 8);
-    const uint4 a2 = *reinterpret_cast<const uint4*>(o_lo + row * ldo + head * D + l * 8);
-    const uint4 b = *reinterpret_cast<const uint4*>(d_o + row * row_do + head * head_do + l * 8);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {a2.x, a2.y, a2.z, a2.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    const long long row = n >> 32 ? i / H : (long long)(uint32_t(i) / uint32_t(H)), head = i - row * H;
+    const long long at = row * ldo + head * D + l * 16;
+    const uint4* a = reinterpret_cast<const uint4*>(o + at);
+    const uint4* b = reinterpret_cast<const uint4*>(d_o + row * row_do + head * head_do + l * 16);
+    const uint4 a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1], c = *reinterpret_cast<const uint4*>(o_lo + at);
+    const uint32_t aw[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w}, bw[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+    const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 x = unpack_bf16(aw[e]), z = unpack_bf16(cw[e]), y = unpack_bf16(bw[e]);
-      acc += (x.x + z.x) * y.x + (x.y + z.y) * y.y;
+    for (int e = 0; e < 8; ++e) {
+      const float2 y = unpack_bf16(bw[e]);
+      acc += with_rest(aw[e] << 16, cw[e / 2], 2 * (e & 1)) * y.x + with_rest(aw[e] & 0xffff0000u, cw[e / 2], 2 * (e & 1) + 1) * y.y;
     }
   }
 #pragma unroll
@@ -1301,12 +1324,14 @@ static int make_group_tmap(CUtensorMap* m, const void* base, const ArbPacked& a,
   uint32_t box[4] = {64, uint32_t(a.G), 1, P};
   return make_tmap_bf16(m, base, 4, dims, str, box);
 }
-// the same of the output; one box is 32 columns of the 32 rows of a warp (G divides 32)
-static int make_out_tmap(CUtensorMap* m, const void* base, const ArbPacked& a) {
+// the same of O (two bytes an element) or its rest (one), as they are written; one box is 32 columns of the 32 rows of a warp
+// (G divides 32)
+static int make_out_tmap(CUtensorMap* m, const void* base, const ArbPacked& a, int bytes) {
   uint64_t dims[4] = {uint64_t(a.D), uint64_t(a.G), uint64_t(a.KV), uint64_t(a.rows)};
-  uint64_t str[3] = {uint64_t(a.D) * 2, uint64_t(a.D) * uint64_t(a.G) * 2, uint64_t(a.o_row) * 2};
+  uint64_t str[3] = {uint64_t(a.D) * bytes, uint64_t(a.D) * uint64_t(a.G) * bytes, uint64_t(a.o_row) * bytes};
   uint32_t box[4] = {32, uint32_t(a.G), 1, 32 / uint32_t(a.G)};
-  return make_tmap_bf16(m, base, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_64B);
+  return make_tmap_typed(m, base, 4, dims, str, box, bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                         bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 static int make_key_tmap(CUtensorMap* m, const void* base, const ArbPacked& a, long long row, long long head) {
   uint64_t dims[3] = {uint64_t(a.D), uint64_t(a.KV), uint64_t(a.rows)};
@@ -1326,6 +1351,7 @@ static int check_packed(const ArbPacked& a) {
   const long long strides[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.v_row, a.v_head, a.o_row, a.do_row, a.do_head, a.dq_row, a.dk_row, a.dv_row};
   for (const void* p : ptrs) if (bad_ptr(p)) return -4;
   for (long long s : strides) if (s < 0 || (s & 7)) return -4;
+  if (a.o_lo && (a.o_row & 15)) return -4;               // a byte an element
   return 0;
 }
 
@@ -1362,12 +1388,12 @@ static int packed_fwd(const ArbPacked& a, int* err, cudaStream_t stream) {
   if ((r = make_key_tmap(&tk, a.k, a, a.k_row, a.k_head))) return 1000 + r;
   if ((r = make_key_tmap(&tv, a.v, a, a.v_row, a.v_head))) return 1000 + r;
   if (32 % a.G == 0) {
-    if ((r = make_out_tmap(&to, a.o, a))) return 1000 + r;
-    if (a.o_lo && (r = make_out_tmap(&tr, a.o_lo, a))) return 1000 + r;
+    if ((r = make_out_tmap(&to, a.o, a, 2))) return 1000 + r;
+    if (a.o_lo && (r = make_out_tmap(&tr, a.o_lo, a, 1))) return 1000 + r;
   }
   PackedArgs p = packed_args(a, err);
   p.o = reinterpret_cast<__nv_bfloat16*>(a.o); p.ldo = a.o_row;
-  p.o_lo = reinterpret_cast<__nv_bfloat16*>(a.o_lo);
+  p.o_lo = reinterpret_cast<int8_t*>(a.o_lo);
   return launch_dependent(true, attn_packed_fwd_k<D>, unsigned(a.cap_q * a.KV), ATT_THREADS, PackedFwdSmem<D>::TOTAL, stream, tq, tk, tv, to, tr, p);
 }
 
@@ -1382,11 +1408,11 @@ static int packed_bwd(const ArbPacked& a, int* err, cudaStream_t stream) {
   if ((r = make_key_tmap(&tv, a.v, a, a.v_row, a.v_head))) return 1000 + r;
   if ((r = make_group_tmap(&tdo, a.d_o, a, a.do_row, a.do_head))) return 1000 + r;
   const int H = int(a.KV * a.G);
-  const long long n = a.rows * H, blocks = (n * (D / 8) + 255) / 256;
+  const long long n = a.rows * H, blocks = (n * (D / 16) + 255) / 256;
   if (blocks > 0x7fffffffll) return -3;
   int* next = reinterpret_cast<int*>(a.delta + n);
   if ((r = launch_dependent(n * D * 2 <= EARLY_BYTES, attn_packed_delta_k<D>, unsigned(blocks), 256, 0, stream,
-                            reinterpret_cast<const __nv_bfloat16*>(a.o), reinterpret_cast<const __nv_bfloat16*>(a.o_lo), a.o_row,
+                            reinterpret_cast<const __nv_bfloat16*>(a.o), reinterpret_cast<const int8_t*>(a.o_lo), a.o_row,
                             reinterpret_cast<const __nv_bfloat16*>(a.d_o), a.do_row, a.do_head, a.delta, next, n, H)))
     return r;
   PackedArgs p = packed_args(a, err);

@@ -120,7 +120,7 @@ def _forward(q, k, v, strides, seqs, window, scale, keep):
     rows, H, d = q.shape
     out = q.new_empty((rows, H, d))
     lse = q.new_empty((rows, H), dtype=torch.float32)
-    rest = q.new_empty((rows, H, d)) if keep else None
+    rest = q.new_empty((rows, H, d), dtype=torch.int8) if keep else None
     if rows:
         _launch("arb_packed_attn_fwd", _ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr() if keep else 0, lse.data_ptr(), 0, 0, 0, 0, 0,

@@ -104,7 +104,7 @@ def plan(mcfg: ModelConfig, micro_batch: int, *, dp: int = 1, tp: int = 1, ep: i
         ("layer: xn2", Ns * D * a),
     ]
     if documents:
-        layer.append(("layer: rest of the attention out", N * Dl * a))       # ops/packed.py
+        layer.append(("layer: rest of the attention out", N * Dl))           # ops/packed.py, a byte an element
     if tp > 1:
         layer += [("layer: gathered xn (TP)", 2 * N * D * a)]
     if moe is None:

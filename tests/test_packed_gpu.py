@@ -204,6 +204,27 @@ def test_a_sequence_does_not_see_its_neighbours(H, KV, d):
             assert bool((x[sum(lengths):] == 0).all())
 
 
+@pytest.mark.parametrize("d,H,KV", [(64, 2, 2), (128, 2, 2), (128, 8, 2), (64, 3, 1), (128, 96, 1)])
+def test_what_the_rounding_of_the_output_leaves_is_kept(d, H, KV):
+    """With q = 0 every key counts alike, P is 1 without a rounding and O a mean of at most 16 values: off by 16 x 2^-22 of their mean
+    size (16 sums in fp32, rounded or cut), and 2^-15 of itself for the 8 bits kept beyond bf16.  Whole and ragged tiles."""
+    from autoresearch_b200.ops import packed as P
+    lengths = [16] * 40 + [5, 1, 0, 9]
+    bounds = _bounds(lengths)
+    rows = bounds[-1]
+    _, _, v, _ = _inputs(rows, H, KV, d)
+    q, k = torch.zeros(rows, H, d, dtype=torch.bfloat16, device="cuda"), v.roll(1, 0).contiguous()
+    out, _, rest = P._forward(q, k, v, (H * d, d) + (KV * d, d) * 2, P.PackedSequences(bounds, rows, H, KV), rows, 0.125, True)
+    assert rest.dtype is torch.int8
+    both = ((out.view(torch.int16).int() << 16) + (rest.int() << 8)).view(torch.float32).double()
+    want, size = torch.zeros_like(both), torch.zeros_like(both)
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        n = torch.arange(1, b - a + 1, device="cuda").double()[:, None, None]
+        x = v[a:b].double().repeat_interleave(H // KV, 1)
+        want[a:b], size[a:b] = x.cumsum(0) / n, x.abs().cumsum(0) / n
+    assert bool(((both - want).abs() <= 2.0 ** -15 * want.abs() + 2.0 ** -18 * size).all())
+
+
 def test_twice_the_same_bits():
     from autoresearch_b200.ops.packed import PackedSequences
     q, k, v, g = _inputs(3000, 6, 2, 128)
@@ -393,7 +414,7 @@ class _Elsewhere(torch.autograd.graph.saved_tensors_hooks):
 
     def spoil(self):
         for t in self.seen:
-            t.data.fill_(math.nan)
+            t.data.fill_(math.nan if t.is_floating_point() else 77)
 
 
 @pytest.mark.parametrize("form", ["separate", "projection"])
