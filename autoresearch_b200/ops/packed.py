@@ -116,17 +116,19 @@ def _layout(t: torch.Tensor):
 
 
 def _forward(q, k, v, strides, seqs, window, scale, keep):
-    """(O, lse, what O's rounding left over where ``keep``).  ``strides``: row and head stride of q, k and v."""
+    """(O, kept).  ``strides``: row and head stride of q, k and v.  ``kept``, for the backward pass, is one buffer (each tensor that
+    autograd keeps costs microseconds): where ``keep``, what O's rounding left over (a byte an element), then lse [rows, H] (fp32)."""
     rows, H, d = q.shape
     out = q.new_empty((rows, H, d))
-    lse = q.new_empty((rows, H), dtype=torch.float32)
-    rest = q.new_empty((rows, H, d), dtype=torch.int8) if keep else None
+    rest = rows * H * d if keep else 0
+    kept = q.new_empty(rest + rows * H * 4, dtype=torch.int8)
     if rows:
+        at = kept.data_ptr()
         _launch("arb_packed_attn_fwd", _ARGS.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr() if keep else 0, lse.data_ptr(), 0, 0, 0, 0, 0,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), at if keep else 0, at + rest, 0, 0, 0, 0, 0,
             seqs.items.data_ptr(), rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k,
             *strides, H * d, 0, 0, 0, 0, 0, scale), seqs)
-    return out, lse, rest
+    return out, kept
 
 
 def _launch(entry, args, seqs):
@@ -141,20 +143,21 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _backward(q, k, v, strides, out, lse, rest, d_out, grads, grad_rows, seqs, window, scale):
+def _backward(q, k, v, strides, out, kept, d_out, grads, grad_rows, seqs, window, scale):
     """Writes ``grads`` (dq, dk, dv), whose rows are ``grad_rows`` apart and whose heads are dense.  All that the forward call read
     or wrote comes in as autograd kept it: hooks on saved tensors (checkpointing, offloading) hand back others than the call had."""
     rows, H, d = q.shape
     if not rows:
         return
-    for t in (q, k, v, out, lse, rest):
+    for t in (q, k, v, out, kept):
         if t.device != seqs.device:
             raise ValueError(f"a saved tensor came back on {t.device}, the sequences are on {seqs.device}")
     d_out, do_row, do_head = _layout(d_out)
-    out, rest, lse = _dense(out), _dense(rest), _dense(lse)
-    delta = lse.new_empty(lse.numel() + 2)
+    out, kept = _dense(out), _dense(kept)
+    at = kept.data_ptr()
+    delta = q.new_empty(rows * H + 2, dtype=torch.float32)
     _launch("arb_packed_attn_bwd", _ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), d_out.data_ptr(), delta.data_ptr(),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), at, at + rows * H * d, d_out.data_ptr(), delta.data_ptr(),
         *[g.data_ptr() for g in grads], seqs.items.data_ptr(), rows, seqs.n_kv_head, seqs.group, d, window, seqs.cap_q, seqs.cap_k,
         *strides, H * d, do_row, do_head, *grad_rows, scale), seqs)
     K.count_launch()                     # the row sums of dO o O and the gradient grid
@@ -171,20 +174,20 @@ class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, seqs, window, scale, keep):
         (q, q0, q1), (k, k0, k1), (v, v0, v1) = _layout(q), _layout(k), _layout(v)
-        out, lse, rest = _forward(q, k, v, (q0, q1, k0, k1, v0, v1), seqs, window, scale, keep)
+        out, kept = _forward(q, k, v, (q0, q1, k0, k1, v0, v1), seqs, window, scale, keep)
         if keep:
-            ctx.save_for_backward(q, k, v, out, lse, rest)
+            ctx.save_for_backward(q, k, v, out, kept)
             ctx.call = (seqs, window, scale)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
         _first_order_only()
-        q, k, v, out, lse, rest = ctx.saved_tensors
+        q, k, v, out, kept = ctx.saved_tensors
         (q, q0, q1), (k, k0, k1), (v, v0, v1) = _layout(q), _layout(k), _layout(v)
         grads = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         row, kv_row = q.shape[1] * q.shape[2], k.shape[1] * k.shape[2]
-        _backward(q, k, v, (q0, q1, k0, k1, v0, v1), out, lse, rest, d_out, grads, (row, kv_row, kv_row), *ctx.call)
+        _backward(q, k, v, (q0, q1, k0, k1, v0, v1), out, kept, d_out, grads, (row, kv_row, kv_row), *ctx.call)
         return (*grads, None, None, None, None)
 
 
@@ -193,21 +196,21 @@ class PackedQKVAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, seqs, window, scale, d, keep):
-        out, lse, rest = _forward(*_blocks(qkv, seqs, d), (qkv.shape[1], d) * 3, seqs, window, scale, keep)
+        out, kept = _forward(*_blocks(qkv, seqs, d), (qkv.shape[1], d) * 3, seqs, window, scale, keep)
         out = out.view(qkv.shape[0], seqs.n_head * d)
         if keep:
-            ctx.save_for_backward(qkv, out, lse, rest)
+            ctx.save_for_backward(qkv, out, kept)
             ctx.call = (seqs, window, scale)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
         _first_order_only()
-        qkv, out, lse, rest = ctx.saved_tensors
-        qkv, d = _dense(qkv), rest.shape[2]
-        d_qkv, ld = qkv.new_empty(qkv.shape), qkv.shape[1]
+        qkv, out, kept = ctx.saved_tensors
         seqs = ctx.call[0]
-        _backward(*_blocks(qkv, seqs, d), (ld, d) * 3, out, lse, rest, d_out.view(-1, seqs.n_head, d), _blocks(d_qkv, seqs, d), (ld,) * 3,
+        qkv, d = _dense(qkv), out.shape[1] // seqs.n_head
+        d_qkv, ld = qkv.new_empty(qkv.shape), qkv.shape[1]
+        _backward(*_blocks(qkv, seqs, d), (ld, d) * 3, out, kept, d_out.view(-1, seqs.n_head, d), _blocks(d_qkv, seqs, d), (ld,) * 3,
                   *ctx.call)
         return d_qkv, None, None, None, None, None
 
