@@ -303,7 +303,8 @@ __device__ __forceinline__ float with_rest(uint32_t hi, uint32_t rest, int k) {
 
 // 32 rows of COLS (32 or 64) bf16 columns, a row in each lane, to rows `off` elements from `dst` (off < 0: not written).  Through 64
 // bytes a column of shared memory of the warp's own, so that neighbouring lanes write neighbouring bytes and not each 16 bytes of
-// another row (32768 rows, window 256, 8 heads on 4: forward with both parts of O 131 -> 121 us, backward 316 -> 291 us).
+// another row (32768 rows, window 256, 8 heads on 4: backward 316 -> 291 us; the forward gave 10 us before whole tiles went by TMA,
+// which the gradients gain nothing by).
 template <int COLS>
 __device__ __forceinline__ uint32_t stage_at(uint32_t stage, int row, int piece) {
   constexpr int PIECES = COLS / 8;                       // 16 bytes each
@@ -622,6 +623,9 @@ attn_packed_fwd_k(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int head = slot.kv * p.G + (r - at * p.G);
       const long long off = live_row ? (long long)(slot.start + pos) * p.ldo + (long long)head * D : -1;
       const uint32_t stage = smem_u32(smem + L::OUT) + uint32_t(q) * 4096u;
+      // where the warp's 32 rows all exist, 32 columns at a time go to the copy engine and the next are read and packed meanwhile: where
+      // all CTAs write at once the warps' own stores waited 1 to 2 K clk per 64 columns (32768 rows, window 256, 8 heads on 4: 108 -> 98 us;
+      // 64 sequences of 512, 4 heads: 60 -> 54 us; long sequences 1 to 2 %)
       const bool whole = 32 % p.G == 0 && __all_sync(0xffffffffu, live_row);
 #pragma unroll 1
       for (int cc = 0; cc < D; cc += 32) {
