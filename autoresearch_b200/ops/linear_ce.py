@@ -8,6 +8,9 @@ joins; no logit is written.  The backward pass multiplies again, a piece of the 
 piece of logits into d = g[n] (softmax(s) - [v = target]) ds/dx (bf16, at most ``PIECE_BYTES``), which the two gradient
 products dx += d w and dw = d^T x read.  What is kept between the passes is one fp32 number per row.
 
+Logits are fp32 sums of the tensor cores, which cut every partial sum (of 16 columns) to 24 bits instead of rounding it: a loss is off
+by about 2e-7 of itself at 256 columns and 1.2e-6 at 2048.
+
 Beside ``LMHeadCEFn`` (ops/sm100.py), which keeps whole rows of logits for a chunk of tokens and makes the gradients in its
 forward pass, this form returns per-token losses with any later weighting and needs no memory that grows with the vocabulary.
 """
