@@ -194,12 +194,7 @@ def prepare(case, seed):
         out_bufs, outs = _flat_views(shapes, to, lambda n, t: torch.zeros(n, dtype=t, device=DEVICE))
     # the expected norm, from the distribution that the gradients were drawn from
     norm = math.sqrt(sum(math.prod(s) * (1e-3 * (1 + i % 5)) ** 2 for i, s in enumerate(shapes)))
-    st = dict(kind=kind, grads=grads, outs=outs, out_bufs=out_bufs, max_norm=norm / case["ratio"] if case["ratio"] else None)
-    if own:
-        # the list of gradient buffers, which stay where they are from step to step
-        from autoresearch_b200.optim.clip import GradSet
-        st["set"] = GradSet(grads, out=outs)
-    return st
+    return dict(kind=kind, grads=grads, outs=outs, out_bufs=out_bufs, max_norm=norm / case["ratio"] if case["ratio"] else None)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -284,8 +279,8 @@ def _own(st):
         return dict(losses=losses.detach(), dx=dx, dw=dw)
     from autoresearch_b200.optim.clip import clip_grad_norm, grad_norm
     if st["max_norm"] is None:
-        return dict(norm=grad_norm(st["set"]))
-    return dict(norm=clip_grad_norm(st["set"], st["max_norm"]), clipped=st["out_bufs"])
+        return dict(norm=grad_norm(st["grads"]))
+    return dict(norm=clip_grad_norm(st["grads"], st["max_norm"], out=st["outs"]), clipped=st["out_bufs"])
 
 
 def run(state):
