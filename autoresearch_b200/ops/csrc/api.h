@@ -13,7 +13,7 @@ enum ArbEpilogue {
   EPI_ATOMIC_F32 = 2,   // C += acc   (fp32, red.global; split-K allowed)
   EPI_NS_COMBINE = 3,   // C = alpha*I + beta*aux + gamma*acc   (bf16)
   EPI_RELU2_BWD = 4,    // C = acc * 2*sqrt(max(aux, 0)): aux = relu(h)^2 saved by the forward (bf16)
-  EPI_STORE_F32 = 5,    // C = acc                      (fp32; splitk > 1 of an unbatched product: the parts stride_c apart)
+  EPI_STORE_F32 = 5,    // C = acc                      (fp32)
   EPI_ADD_AUX = 6,      // C = aux + acc                (bf16)
   EPI_QKV_POST = 7,     // packed q|k|v projection: RoPE + RMS norm on q and k heads, value embedding on v heads (bf16);
                         // 2-CTA tiles, NT layout; parameters from arb_gemm_qkv_post_args

@@ -1551,6 +1551,10 @@ extern "C" int arb_linear_ce_parts(long long rows, long long dim, long long piec
   return best;
 }
 
+// `parts` sums over cuts of K, fp32, stride_c apart; defined with the product's entry points below
+static int gemm_parts(const void* A, const void* B, float* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
+                      long long stride_c, int b_mn_major, int parts, int* err_flag, cudaStream_t stream);
+
 extern "C" int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx, float* acc, void* dw, float* main, long long ld_main,
                                  int* err_flag, cudaStream_t stream) {
   if (!a || a->col0 != 0 || a->cols != a->vocab || piece <= 0 || (piece < a->vocab && piece % 256)) return -3;
@@ -1569,11 +1573,13 @@ extern "C" int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx
     b.col0 = c;
     b.cols = piece < a->vocab - c ? piece : a->vocab - c;
     if (int r = ce_grad(b, err_flag, stream)) return r;
-    if (dx) {
+    if (dx && parts > 1) {
+      if (int r = gemm_parts(a->d_logits, b.w, acc, N, D, int(b.cols), a->ldd, a->ldw, D, (long long)N * D, 1, parts, err_flag, stream)) return r;
+    } else if (dx) {
       // several pieces meet in fp32, one after the other and without a split of the summed dimension: the same bits every time
-      const int epi = one && parts == 1 ? EPI_STORE_BF16 : c == 0 ? EPI_STORE_F32 : EPI_ATOMIC_F32;
-      if (int r = arb_gemm_bf16(a->d_logits, b.w, one && parts == 1 ? dx : acc, nullptr, N, D, int(b.cols), 1, a->ldd, a->ldw, D, 0, 0,
-                                parts > 1 ? (long long)N * D : 0, 0, 1, epi, parts, 0.f, 0.f, 1.f, err_flag, stream))
+      const int epi = one ? EPI_STORE_BF16 : c == 0 ? EPI_STORE_F32 : EPI_ATOMIC_F32;
+      if (int r = arb_gemm_bf16(a->d_logits, b.w, one ? dx : acc, nullptr, N, D, int(b.cols), 1, a->ldd, a->ldw, D, 0, 0, 0, 0, 1, epi, 1, 0.f,
+                                0.f, 1.f, err_flag, stream))
         return r;
     }
     if (main) {
@@ -1670,12 +1676,13 @@ extern "C" int arb_gemm_bf16_ex(const void* A, const void* B, void* C, const voi
                               ahead_bytes, nullptr, 1, nullptr, 0);
 }
 
-extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const void* aux, int M, int N, int K, int batch,
-                                    long long lda, long long ldb, long long ldc, long long stride_a, long long stride_b,
-                                    long long stride_c, int a_mn_major, int b_mn_major, int epi, int splitk, float alpha,
-                                    float beta, float gamma, int* err_flag, cudaStream_t stream, const void* pull_src,
-                                    long long pull_bytes, const void* ahead_src, void* ahead_dst, long long ahead_bytes,
-                                    const int* m_valid, int b_div, const int* k_valid, int k_seg_rows) {
+// slabs: of an EPI_STORE_F32 product, the `splitk` > 1 sums over cuts of K side by side, stride_c apart.  Not to be had through the entry
+// points, whose splitk is a hint to the accumulating epilogue: there C is one matrix, and a second one would land behind it.
+static int gemm_any(const void* A, const void* B, void* C, const void* aux, int M, int N, int K, int batch, long long lda, long long ldb,
+                    long long ldc, long long stride_a, long long stride_b, long long stride_c, int a_mn_major, int b_mn_major, int epi,
+                    int splitk, float alpha, float beta, float gamma, int* err_flag, cudaStream_t stream, const void* pull_src,
+                    long long pull_bytes, const void* ahead_src, void* ahead_dst, long long ahead_bytes, const int* m_valid, int b_div,
+                    const int* k_valid, int k_seg_rows, bool slabs) {
   if (M <= 0 || N <= 0 || K <= 0 || batch <= 0) return -3;
   if (b_div < 1 || batch % b_div) return -3;
   if (k_valid && (k_seg_rows <= 0 || (k_seg_rows % BK) || (K % k_seg_rows) || epi != EPI_ATOMIC_F32)) return -3;
@@ -1699,7 +1706,6 @@ extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const
   // 128 x 128, operands from HBM: 2048 x 512 x 2048 22.5 -> 18.4, 2048 x 512 x 1536 19.3 -> 17.3, 1024 x 1024 x 4096 32.8 -> 28.7,
   // 1024 x 256 x 256 15.2 -> 13.2; with 256 tiles of 128 x 128, i.e. two waves, 2048 x 2048 x 512 gains nothing).
   const long long tiles128 = (long long)batch * ((M + 127) / 128) * ((N + 127) / 128);
-  const bool slabs = epi == EPI_STORE_F32 && splitk > 1;      // the parts of a split sum side by side, stride_c apart
   const bool few = g_gemm_mode == 0 && tiles128 <= 148 && epi != EPI_ATOMIC_F32 && epi != EPI_QKV_POST && !slabs;
   const int BN = (N > 128 && !few) ? 256 : 128;
   const bool pair = (g_gemm_mode != 1) && (g_gemm_mode == 2 || (M >= 512 && N >= 256 && !few));
@@ -1716,14 +1722,16 @@ extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const
   a.m_tiles = (M + bm_eff - 1) / bm_eff;
   a.n_tiles = pair ? (N + 255) / 256 : (N + BN - 1) / BN;
   a.kb_total = (K + BK - 1) / BK;
-  if (slabs && (batch != 1 || stride_c <= 0 || (stride_c % 4))) return -3;
+  if (slabs && (epi != EPI_STORE_F32 || batch != 1 || splitk < 2 || splitk > a.kb_total || stride_c < (M - 1) * ldc + N || (stride_c % 4)))
+    return -3;
+  const int slabs_wanted = splitk;
   if (epi != EPI_ATOMIC_F32 && !slabs) splitk = 1;
   if (splitk <= 0)  // automatic: fill the SMs when there are few output tiles
     splitk = pick_split(batch * a.m_tiles * a.n_tiles, a.kb_total, pair ? g_num_sms / 2 : g_num_sms);
   if (splitk > a.kb_total) splitk = a.kb_total;
   a.kb_per_split = (a.kb_total + splitk - 1) / splitk;
   a.splitk = (a.kb_total + a.kb_per_split - 1) / a.kb_per_split;
-  if (slabs && a.splitk != splitk) return -3;                 // the caller sums that many
+  if (slabs && a.splitk != slabs_wanted) return -3;           // the caller sums that many
   a.C = C; a.aux = aux; a.ldc = ldc; a.stride_c = stride_c;
   a.alpha = alpha; a.beta = beta; a.gamma = gamma; a.err = err_flag;
   a.pull_src = reinterpret_cast<const uint4*>(pull_src);
@@ -1776,4 +1784,20 @@ extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const
   if (a_mn_major && b_mn_major) return ARB_DISPATCH(true, true);
   return ARB_DISPATCH(true, false);
 #undef ARB_DISPATCH
+}
+
+extern "C" int arb_gemm_bf16_ragged(const void* A, const void* B, void* C, const void* aux, int M, int N, int K, int batch,
+                                    long long lda, long long ldb, long long ldc, long long stride_a, long long stride_b,
+                                    long long stride_c, int a_mn_major, int b_mn_major, int epi, int splitk, float alpha,
+                                    float beta, float gamma, int* err_flag, cudaStream_t stream, const void* pull_src,
+                                    long long pull_bytes, const void* ahead_src, void* ahead_dst, long long ahead_bytes,
+                                    const int* m_valid, int b_div, const int* k_valid, int k_seg_rows) {
+  return gemm_any(A, B, C, aux, M, N, K, batch, lda, ldb, ldc, stride_a, stride_b, stride_c, a_mn_major, b_mn_major, epi, splitk, alpha, beta,
+                  gamma, err_flag, stream, pull_src, pull_bytes, ahead_src, ahead_dst, ahead_bytes, m_valid, b_div, k_valid, k_seg_rows, false);
+}
+
+static int gemm_parts(const void* A, const void* B, float* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
+                      long long stride_c, int b_mn_major, int parts, int* err_flag, cudaStream_t stream) {
+  return gemm_any(A, B, C, nullptr, M, N, K, 1, lda, ldb, ldc, 0, 0, stride_c, 0, b_mn_major, EPI_STORE_F32, parts, 0.f, 0.f, 1.f, err_flag,
+                  stream, nullptr, 0, nullptr, nullptr, 0, nullptr, 1, nullptr, 0, true);
 }

@@ -324,3 +324,20 @@ def test_symmetric_product_of_an_odd_side_writes_what_the_plain_product_writes()
         K.gemm(full[:, :d], full[:, :d], out=got[-1][:, :d], epi=epi, aux=aux[:, :d], alpha=3.4, beta=-4.7, gamma=2.0)
     assert torch.equal(*got)
     K.check_err_flag()
+
+
+@pytest.mark.parametrize("batched", [False, True])
+def test_an_fp32_store_stays_inside_of_its_output_whatever_the_split(batched):
+    """`splitk` is for accumulating products: a stored one is one sum, and what stands behind the output stays (here it belongs to
+    the same allocation)."""
+    from autoresearch_b200.ops import kernels as K_
+    torch.manual_seed(5)
+    M, N, K = 520, 264, 448
+    a, b = _rand(1, M, K), _rand(1, N, K)
+    want = K_.gemm(a, b, epi=K_.EPI_STORE_F32)
+    buf = torch.full((4, M, N), 7.0, device="cuda")
+    for splitk in (2, 3):
+        out = buf[:1] if batched else buf[0]
+        K_.gemm(a if batched else a[0], b if batched else b[0], out=out, epi=K_.EPI_STORE_F32, splitk=splitk)
+        K_.check_err_flag()
+        assert torch.equal(buf[:1], want) and bool((buf[1:] == 7.0).all())
