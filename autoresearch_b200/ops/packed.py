@@ -29,12 +29,31 @@ L2_SPAN_BYTES = 48 << 20                # keys and values whose tiles run togeth
 
 
 def check_bounds(bounds, rows: int) -> None:
-    """Raises unless ``bounds`` (host values) ascend from at least 0 to at most ``rows``."""
-    last = 0
-    for b in bounds:
-        if not last <= b <= rows:
-            raise ValueError(f"sequence bounds must ascend within [0, {rows}]: got {list(bounds)[:16]}")
-        last = b
+    """Raises unless ``bounds`` (host values, or a tensor on the host) ascend from at least 0 to at most ``rows``."""
+    if torch.is_tensor(bounds):
+        fine = 0 <= int(bounds[0]) and int(bounds[-1]) <= rows and bool((bounds[1:] >= bounds[:-1]).all())
+    else:
+        last = 0
+        for b in bounds:
+            if not last <= b <= rows:
+                break
+            last = b
+        else:
+            return
+        fine = False
+    if not fine:
+        raise ValueError(f"sequence bounds must ascend within [0, {rows}]: got {list(bounds[:16])}")
+
+
+def _to_device(bounds: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """A copy of host bounds on ``device``, made in the order of its current stream and without waiting for what runs there: they travel
+    through pinned memory of their own, which the allocator gives away again behind the copy only."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("under graph capture cu_seqlens must be a CUDA tensor: every replay would read the host's memory again")
+        pinned = torch.empty(bounds.shape, dtype=torch.int32, pin_memory=True)
+        pinned.copy_(bounds)
+        return pinned.to(device, non_blocking=True)
 
 
 def document_bounds(ids: torch.Tensor, bos: int) -> torch.Tensor:
@@ -51,7 +70,7 @@ class PackedSequences:
     """Which tiles the sequences of a packed batch have.
 
     ``cu_seqlens``: n + 1 ascending row numbers, an int32 CUDA tensor, or host values (a list, a CPU tensor), which are checked
-    here.  Bounds that only the device knows are not read back: where they descend or leave the rows they are moved inside,
+    and copied here, without waiting for the device.  Bounds that only the device knows are not read back: where they descend or leave the rows they are moved inside,
     and ``kernels.check_err_flag()`` reports it.  Empty sequences are allowed.  Rows of no sequence (before the first bound
     and behind the last) get zero outputs and gradients, whatever their inputs hold.
 
@@ -67,14 +86,15 @@ class PackedSequences:
         if not (torch.is_tensor(cu_seqlens) and cu_seqlens.is_cuda):
             if torch.is_tensor(cu_seqlens) and (cu_seqlens.dim() != 1 or cu_seqlens.dtype not in (torch.int32, torch.int64)):
                 raise TypeError("cu_seqlens must be a 1-D tensor of integers")
-            values = cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else [operator.index(b) for b in cu_seqlens]
-            if not values:
+            if not torch.is_tensor(cu_seqlens):
+                cu_seqlens = [operator.index(b) for b in cu_seqlens]
+            if not len(cu_seqlens):
                 raise ValueError("cu_seqlens needs at least one bound")
-            check_bounds(values, rows)
+            check_bounds(cu_seqlens, rows)
             device = torch.device(device if device is not None else "cuda")
             if device.type != "cuda":
                 raise ValueError(f"the sequences must be packed on a CUDA device, not {device}")
-            cu_seqlens = torch.tensor(values, dtype=torch.int32, device=device)
+            cu_seqlens = _to_device(torch.as_tensor(cu_seqlens), device)
         elif cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype is not torch.int32:
             raise TypeError("cu_seqlens must be a 1-D int32 tensor of at least one element")
         self.cu_seqlens = cu_seqlens.contiguous()

@@ -168,3 +168,21 @@ def test_the_operators_in_a_chain():
     for got, clipped, t in zip(grads, out, want):
         assert float((got.double() - t).norm()) <= tol * float(t.norm())
         assert float((clipped.double() - t * (0.01 / norm64)).norm()) <= tol * float(t.norm()) * 0.01 / norm64
+
+
+def test_a_training_step_on_documents_does_not_wait_for_the_device():
+    from autoresearch_b200.config import TrainConfig, model_preset
+    from autoresearch_b200.trainer import Trainer
+    cfg = model_preset("small")
+    t = TrainConfig(device_batch_size=4, total_batch_size=4 * cfg.seq_len * 2, max_steps=6, cooldown_steps=2, synthetic_data=True,
+                    synthetic_kind="zipf", impl="sm100", cooldown_trigger_file="", grad_clip=0.05, doc_bos=3)
+    tr = Trainer(cfg, t, device="cuda", quiet=True)
+    for _ in range(2):
+        tr.train_step()
+    torch.cuda.synchronize()
+    assert tr.prefetch.wait_for(2)
+    torch.cuda._sleep(1_000_000_000)                        # about 0.5 s
+    loss = tr.train_step()
+    assert not torch.cuda.current_stream().query(), "the step waited for the stream"
+    assert math.isfinite(float(loss))
+    tr.prefetch.close()

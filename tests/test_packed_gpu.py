@@ -512,3 +512,38 @@ def test_refusals():
         packed_qkv_attention(torch.cat([q, k, v], 1).view(rows, -1)[:, 1:], seqs)
     with pytest.raises(ValueError):
         packed_qkv_attention(q.view(rows, -1), seqs)
+
+
+@pytest.mark.parametrize("kind", ["list", "int32", "int64", "pinned"])
+def test_host_bounds_are_taken_up_without_waiting(kind):
+    """While the stream is busy the call returns, and what the caller writes to the bounds afterwards does not count."""
+    from autoresearch_b200.ops.packed import PackedSequences
+    bounds = [0, 300, 301, 700]
+    make = {"list": list, "int32": lambda b: torch.tensor(b, dtype=torch.int32), "int64": torch.tensor,
+            "pinned": lambda b: torch.tensor(b, dtype=torch.int32).pin_memory()}[kind]
+    want = PackedSequences(torch.tensor(bounds, dtype=torch.int32, device="cuda"), 777, 4, 2)
+    PackedSequences(make(bounds), 777, 4, 2)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)                          # about 0.2 s
+    given = make(bounds)
+    seqs = PackedSequences(given, 777, 4, 2)
+    busy = not torch.cuda.current_stream().query()
+    given[1] = 5
+    assert busy, "the call waited for the stream"
+    torch.cuda.synchronize()
+    assert torch.equal(seqs.cu_seqlens, want.cu_seqlens)
+    for a, b in zip(_plan_lists(seqs), _plan_lists(want)):
+        assert torch.equal(a, b)
+
+
+def test_host_bounds_are_refused_under_graph_capture():
+    from autoresearch_b200.ops.packed import PackedSequences
+    x = torch.zeros(8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1.0)
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            PackedSequences([0, 4], 4, 2, 1)
+    graph.replay()
+    assert float(x[0]) == 1.0
