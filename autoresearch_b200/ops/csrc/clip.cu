@@ -172,8 +172,18 @@ __global__ void __launch_bounds__(CLIP_THREADS, 5) grad_squares_k(const __grid_c
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
+// min(1, max_norm / norm) as a product of two fp32 numbers: by itself it may be smaller than the normal numbers, and fast math takes those
+// for zero.  (The first factor is normal down to 2^-252; below that no element comes out above 2^-124.)
+struct GradFactor {
+  float a, b;
+  __device__ __forceinline__ explicit GradFactor(double c) : a(float(c)), b(1.f) {
+    if (c < 0x1p-126) { a = float(c * 0x1p126); b = 0x1p-126f; }
+  }
+  __device__ __forceinline__ float operator()(float x) const { return x * a * b; }
+};
+
 template <typename TI, typename TO, int W>
-__device__ __forceinline__ void item_scale(const TI* p, TO* q, int n, float c) {
+__device__ __forceinline__ void item_scale(const TI* p, TO* q, int n, GradFactor c) {
   constexpr int STEP = CLIP_THREADS * W * 4;
   int at = 0;
 #pragma unroll 1
@@ -185,16 +195,16 @@ __device__ __forceinline__ void item_scale(const TI* p, TO* q, int n, float c) {
     for (int k = 0; k < 4; ++k) {
       Vec<TO, W> o;
 #pragma unroll
-      for (int e = 0; e < W; ++e) from_f32(to_f32(v[k].v[e]) * c, o.v[e]);
+      for (int e = 0; e < W; ++e) from_f32(c(to_f32(v[k].v[e])), o.v[e]);
       *reinterpret_cast<Vec<TO, W>*>(q + at + (k * CLIP_THREADS + int(threadIdx.x)) * W) = o;
     }
   }
 #pragma unroll 1
-  for (int i = at + int(threadIdx.x); i < n; i += CLIP_THREADS) from_f32(to_f32(p[i]) * c, q[i]);
+  for (int i = at + int(threadIdx.x); i < n; i += CLIP_THREADS) from_f32(c(to_f32(p[i])), q[i]);
 }
 
 template <typename TI, typename TO>
-__device__ __forceinline__ void tensor_scale(const void* in, void* out, long long from, int n, float c) {
+__device__ __forceinline__ void tensor_scale(const void* in, void* out, long long from, int n, GradFactor c) {
   const TI* p = reinterpret_cast<const TI*>(in) + from;
   TO* q = reinterpret_cast<TO*>(out) + from;
   switch (min(grad_width<TI>(p), grad_width<TO>(q))) {
@@ -205,7 +215,7 @@ __device__ __forceinline__ void tensor_scale(const void* in, void* out, long lon
   }
 }
 template <typename TI>
-__device__ __forceinline__ void tensor_scale_to(int to, const void* in, void* out, long long from, int n, float c) {
+__device__ __forceinline__ void tensor_scale_to(int to, const void* in, void* out, long long from, int n, GradFactor c) {
   switch (to) {
     case GRAD_F32: tensor_scale<TI, float>(in, out, from, n, c); break;
     case GRAD_BF16: tensor_scale<TI, __nv_bfloat16>(in, out, from, n, c); break;
@@ -224,10 +234,10 @@ __global__ void __launch_bounds__(CLIP_THREADS, 5) grad_scale_k(const __grid_con
   const double norm = sqrt(block_sum(acc, sh));
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) *norm_out = narrow(norm);
   if (max_norm < 0.f) return;
-  const float c = norm > double(max_norm) && norm <= 1.7976931348623157e308 ? float(double(max_norm) / norm) : 1.f;
+  const GradFactor c(norm > double(max_norm) && norm <= 1.7976931348623157e308 ? double(max_norm) / norm : 1.0);
   for (int i = t.first[t.count] - 1 - int(blockIdx.x); i >= 0; i -= gridDim.x) {
     const int k = grad_tensor(t, i);
-    if (c == 1.f && t.out[k] == t.in[k]) continue;          // in place and nothing to do
+    if (c.a == 1.f && t.out[k] == t.in[k]) continue;          // in place and nothing to do
     const long long from = (long long)(i - t.first[k]) * CLIP_ITEM, left = t.n[k] - from;
     const int n = left < CLIP_ITEM ? int(left) : CLIP_ITEM;
     const int to = t.type[k] >> 2;

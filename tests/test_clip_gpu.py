@@ -204,3 +204,21 @@ def test_refusals():
         clip_grad_norm(GradSet([t]), 1.0, out=[t.clone()])
     clip_grad_norm([t, t.clone()], 1.0, out=[t, torch.zeros(10, 10, device="cuda")])      # one of them in place
     assert float(grad_norm([])) == 0.0 and float(grad_norm([torch.zeros(0, device="cuda")])) == 0.0
+
+
+@pytest.mark.parametrize("size,max_norm", [(1e36, 1e-3), (3e35, 2e-6), (1e37, 1e-8), (1e30, 1e-30), (1e36, 30.0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_factors_below_the_normal_numbers_of_fp32(dtype, size, max_norm):
+    """max_norm / norm may be smaller than 2^-126 while the scaled elements are not."""
+    from autoresearch_b200.optim.clip import clip_grad_norm
+    g = torch.Generator(device="cuda").manual_seed(0)
+    grads = [((torch.rand(n, generator=g, device="cuda") + 0.5) * size).to(dtype) for n in (1000, 20001)]
+    source = [t.clone() for t in grads]
+    factor = max_norm / _norm(source)
+    out = [torch.zeros_like(t, dtype=torch.bfloat16 if dtype is torch.float32 else torch.float32) for t in grads]
+    clip_grad_norm(grads, max_norm, out=out)
+    _check_scaled(out, source, factor)
+    clip_grad_norm(grads, max_norm)
+    _check_scaled(grads, source, factor)
+    if max_norm * 2e-3 > 2.0 ** -126:
+        assert min(float(t.float().abs().min()) for t in grads + out) > 0
