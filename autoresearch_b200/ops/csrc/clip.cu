@@ -173,13 +173,14 @@ __global__ void __launch_bounds__(CLIP_THREADS, 5) grad_squares_k(const __grid_c
 }
 
 // min(1, max_norm / norm) as a product of two fp32 numbers: by itself it may be smaller than the normal numbers, and fast math takes those
-// for zero.  (The first factor is normal down to 2^-252; below that no element comes out above 2^-124.)
+// for zero.  (The first factor is normal down to 2^-252; below that no element comes out above 2^-124.)  1 is no multiplication at all,
+// so that copies keep subnormal elements as they are.
 struct GradFactor {
   float a, b;
   __device__ __forceinline__ explicit GradFactor(double c) : a(float(c)), b(1.f) {
     if (c < 0x1p-126) { a = float(c * 0x1p126); b = 0x1p-126f; }
   }
-  __device__ __forceinline__ float operator()(float x) const { return x * a * b; }
+  __device__ __forceinline__ float operator()(float x) const { return a == 1.f ? x : x * a * b; }
 };
 
 template <typename TI, typename TO, int W>

@@ -222,3 +222,19 @@ def test_factors_below_the_normal_numbers_of_fp32(dtype, size, max_norm):
     _check_scaled(grads, source, factor)
     if max_norm * 2e-3 > 2.0 ** -126:
         assert min(float(t.float().abs().min()) for t in grads + out) > 0
+
+
+@pytest.mark.parametrize("bad", [None, float("inf")])
+@pytest.mark.parametrize("to", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradients_that_are_not_scaled_are_copied_as_they_are(dtype, to, bad):
+    """Subnormal elements among them: bit for bit in their own type, rounded once into another."""
+    from autoresearch_b200.optim.clip import clip_grad_norm
+    n = 20003
+    t = torch.randn(n, dtype=torch.float64, generator=torch.Generator().manual_seed(0)) * 2.0 ** -(torch.arange(n) % 150).double()
+    t = t.to(dtype)
+    if bad is not None:
+        t[777] = bad
+    out = torch.zeros(n, dtype=to, device="cuda")
+    clip_grad_norm([t.cuda()], 1e4, out=[out])
+    assert torch.equal(out.cpu(), t.to(to))
