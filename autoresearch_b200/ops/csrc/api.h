@@ -127,7 +127,7 @@ int arb_linear_ce_bwd(const ArbLinearCE* a, long long piece, void* dx, float* ac
 // Types: 0 fp32, 1 bf16, 2 fp16.  At most 1024 tensors a call; longer lists go in parts, each with `blocks` partial sums of its own.
 // squares: partial[0 .. blocks) = sums of squares that add up to the squared norm of these tensors.
 // scale: norm (may be null) = sqrt of the sum of all partials; max_norm >= 0: out = in * min(1, max_norm / norm), out = in left
-// alone where that is 1 or the norm is not finite (another out is then a copy); max_norm < 0: the norm alone.
+// alone where that is 1 or an element is not finite (another out is then a copy); max_norm < 0: the norm alone.
 typedef struct ArbGrad {
   const void* in;
   void* out;

@@ -224,7 +224,8 @@ __device__ __forceinline__ void tensor_scale_to(int to, const void* in, void* ou
   }
 }
 
-// max_norm < 0: the norm alone.  A norm that is not finite scales nothing.
+// max_norm < 0: the norm alone.  A norm that is not finite scales nothing (in 64 bits that of finite elements always is, also where it is
+// infinite as the fp32 number that is handed out).
 template <int CAP>
 __global__ void __launch_bounds__(CLIP_THREADS, 5) grad_scale_k(const __grid_constant__ GradTable<CAP> t, const double* partial, int partials,
                                                              double max_norm, float* norm_out) {

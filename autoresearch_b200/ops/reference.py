@@ -110,7 +110,7 @@ def linear_cross_entropy(x, w, targets, softcap: float):
 
 
 def clip_grad_norm(grads, max_norm: float):
-    """Scales the tensors in place by min(1, max_norm / norm) and returns their 2-norm; one that is not finite scales nothing."""
+    """Scales the tensors in place by min(1, max_norm / norm) and returns their 2-norm; elements that are not finite scale nothing."""
     norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
     scale = torch.where(torch.isfinite(norm) & (norm > max_norm), max_norm / norm, torch.ones_like(norm))
     for g in grads:

@@ -116,8 +116,8 @@ def grad_norm(grads: Grads) -> torch.Tensor:
 
 def clip_grad_norm(grads: Grads, max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the gradients by min(1, max_norm / norm), in place or into ``out`` (where they are converted to its types), and
-    returns their norm before that.  Where the norm is not finite they are left as they are (``out`` gets copies), for the
-    caller to see in the result."""
+    returns their norm before that.  Where a gradient is infinite or NaN they are left as they are (``out`` gets copies), for the
+    caller to see in the result; finite gradients are scaled, also those whose norm is infinite as an fp32 number."""
     if not 0.0 < max_norm:
         raise ValueError(f"max_norm must be positive, got {max_norm}")
     if isinstance(grads, GradSet):

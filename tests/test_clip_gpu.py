@@ -238,3 +238,13 @@ def test_gradients_that_are_not_scaled_are_copied_as_they_are(dtype, to, bad):
     out = torch.zeros(n, dtype=to, device="cuda")
     clip_grad_norm([t.cuda()], 1e4, out=[out])
     assert torch.equal(out.cpu(), t.to(to))
+
+
+def test_finite_gradients_of_a_norm_beyond_fp32_are_scaled():
+    from autoresearch_b200.optim.clip import clip_grad_norm
+    grads = [torch.full((5000,), 3e38, device="cuda"), torch.full((100,), -2e36, device="cuda", dtype=torch.bfloat16)]
+    source = [t.clone() for t in grads]
+    assert math.isinf(float(clip_grad_norm(grads, 1.0)))
+    _check_scaled(grads, source, 1.0 / _norm(source))
+    one = [torch.full((1,), 3.4e38, device="cuda")]
+    assert math.isfinite(float(clip_grad_norm(one, 1.0))) and abs(float(one[0]) - 1.0) <= 2.0 ** -18
