@@ -73,7 +73,7 @@ class GradSet:
                     ins.discard(t.data_ptr())                       # in place, this one
             _apart([t for t, _ in live if t.data_ptr() in ins] + [o for _, o in live], "outputs and gradients")
         self.tensors, self.out = tensors, out if out is None else outs
-        self._where = self._addresses()
+        self._where = self._layout()
         self.device = tensors[0].device if tensors else None
         rows = [_ENTRY.pack(t.data_ptr(), o.data_ptr(), t.numel(), _TYPES[t.dtype], _TYPES[o.dtype]) for t, o in live]
         # (argument block, tensors in it, blocks of its grid)
@@ -84,11 +84,11 @@ class GradSet:
                 items = sum(-(-t.numel() // ITEM) for t, _ in live[a:a + MAX_TENSORS])
                 self._parts.append((b"".join(rows[a:a + MAX_TENSORS]), len(rows[a:a + MAX_TENSORS]), min(items, most)))
 
-    def _addresses(self):
-        return [t.data_ptr() for t in self.tensors] + [t.data_ptr() for t in self.out or ()]
+    def _layout(self):
+        return [(t.data_ptr(), t.numel(), t.dtype) for t in (self.tensors if self.out is None else self.tensors + self.out)]
 
     def _run(self, max_norm: float) -> torch.Tensor:
-        if self._addresses() != self._where:         # a tensor was given other memory since, or the set is a copy
+        if self._layout() != self._where:            # a tensor was given other memory, another size or type since, or the set is a copy
             self.__init__(self.tensors, self.out)
         if not self._parts:
             return torch.zeros((), dtype=torch.float32, device=self.device if self.device is not None else "cuda")

@@ -248,3 +248,23 @@ def test_finite_gradients_of_a_norm_beyond_fp32_are_scaled():
     _check_scaled(grads, source, 1.0 / _norm(source))
     one = [torch.full((1,), 3.4e38, device="cuda")]
     assert math.isfinite(float(clip_grad_norm(one, 1.0))) and abs(float(one[0]) - 1.0) <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("how", ["resize", "data", "type"])
+def test_tensors_that_kept_their_address_but_not_their_size(how):
+    """All of it inside of one allocation: what lies behind the smaller tensor stays as it was."""
+    from autoresearch_b200.optim.clip import GradSet, clip_grad_norm
+    buf = torch.full((40000,), 2.0, device="cuda")
+    t, other = buf[:40000], _grads([(500,)], torch.float32)[0]
+    s = GradSet([t, other])
+    if how == "resize":
+        t.resize_(1000)
+    elif how == "data":
+        t.data = buf[:1000].view(10, 100)
+    else:
+        t.data = buf.view(torch.bfloat16)[:40000]
+    source = [t.clone(), other.clone()]
+    want = _norm(source)
+    assert abs(float(clip_grad_norm(s, want / 4)) - want) <= 2.0 ** -19 * want
+    _check_scaled([t, other], source, 0.25)
+    assert bool((buf[20000 if how == "type" else 1000:] == 2.0).all())
