@@ -36,6 +36,11 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _order(t: torch.Tensor):
+    """Strides of the dimensions that have any use for one."""
+    return [s for s, n in zip(t.stride(), t.shape) if n != 1]
+
+
 def _apart(tensors, what: str) -> None:
     """Refuses tensors that share memory: an element in two of them would count, or be scaled, twice."""
     spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors)
@@ -61,7 +66,7 @@ class GradSet:
             if not _dense(t):
                 raise ValueError(f"gradients must be dense, got strides {t.stride()} of {tuple(t.shape)}")
         for t, o in zip(tensors, outs):
-            if o.shape != t.shape or (o is not t and o.stride() != t.stride() and t.numel() > 1):
+            if o.shape != t.shape or (o is not t and o.stride() != t.stride() and t.numel() > 1 and _order(o) != _order(t)):
                 raise ValueError(f"output {tuple(o.shape)} {o.stride()} does not match its gradient {tuple(t.shape)} {t.stride()}")
         live = [(t, o) for t, o in zip(tensors, outs) if t.numel()]
         _apart([t for t, _ in live], "gradients")

@@ -268,3 +268,14 @@ def test_tensors_that_kept_their_address_but_not_their_size(how):
     assert abs(float(clip_grad_norm(s, want / 4)) - want) <= 2.0 ** -19 * want
     _check_scaled([t, other], source, 0.25)
     assert bool((buf[20000 if how == "type" else 1000:] == 2.0).all())
+
+
+def test_strides_of_dimensions_of_one_do_not_count():
+    from autoresearch_b200.optim.clip import clip_grad_norm
+    grads = [torch.randn(1, 300, device="cuda"), torch.randn(7, 1, 20, device="cuda")]
+    out = [torch.zeros(300, 1, device="cuda").t(), torch.zeros(1, 7, 20, device="cuda", dtype=torch.bfloat16).transpose(0, 1)]
+    assert all(o.shape == t.shape and o.stride() != t.stride() for t, o in zip(grads, out))
+    clip_grad_norm(grads, _norm(grads) / 2, out=out)
+    _check_scaled(out, grads, 0.5)
+    with pytest.raises(ValueError, match="does not match"):
+        clip_grad_norm([torch.zeros(3, 1, 5, device="cuda")], 1.0, out=[torch.zeros(5, 1, 3, device="cuda").permute(2, 1, 0)])
