@@ -263,7 +263,7 @@ class TrainConfig:
     heartbeat_timeout_s: float = 0.0  # > 0: watch peer liveness through the process group's store
     grad_clip: float = 0.0  # > 0: all gradients together are scaled to at most this 2-norm before the optimizer step (one GPU)
     doc_bos: Optional[int] = None  # token id that begins a document: attention stays inside of documents (data parallel only)
-    vocab_pieces: bool = False  # the head's loss in pieces of the vocabulary, without logits in memory
+    vocab_pieces: bool = False  # the head's loss in pieces of the vocabulary, without logits in memory (impl sm100)
     peak_flops: Optional[float] = None  # MFU denominator per GPU; None = ARB_PEAK_TFLOPS or the nominal B200 peak
     parallel: ParallelConfig = field(default_factory=ParallelConfig)
 

@@ -37,7 +37,7 @@ class DeviceFault(RuntimeError):
 
 
 class TrainerBase:
-    # ---- filled by the subclass before _init_common --------------------------------------------
+    # ---- filled by the subclass before _init_common, beside `model` (of several, the one with the head) ------------
     mcfg: ModelConfig
     tcfg: TrainConfig
     device: torch.device
@@ -61,6 +61,13 @@ class TrainerBase:
             raise ValueError(f"grad_clip={t.grad_clip}: a norm that is not negative, in training on one GPU")
         if t.doc_bos is not None and not self.masks_documents:
             raise ValueError("doc_bos: attention inside of documents needs the data-parallel trainer")
+        # the head's loss in pieces of the vocabulary: asked for, or because the backend has no other form for this vocabulary
+        head = self.model.backend
+        if hasattr(head, "takes_vocab_pieces"):
+            head.vocab_pieces = t.vocab_pieces
+        elif t.vocab_pieces:
+            raise ValueError(f"vocab_pieces: {type(head).__name__} computes the head's loss from whole rows of logits only")
+        self.by_vocab_pieces = hasattr(head, "takes_vocab_pieces") and head.takes_vocab_pieces(m.vocab)
         self.step = 0
         self.loss_ema = 0.0
         self.ema_steps = 0
@@ -100,7 +107,7 @@ class TrainerBase:
         cannot fit is refused here, before step 0) and prints the reference's start-up line
         ``Allocated N MB GPU memory (B=..)`` (brain/src/train.rs:721)."""
         from .utils import memplan
-        self.mem_plan = memplan.plan(self.mcfg, self.micro_batch, **kw)
+        self.mem_plan = memplan.plan(self.mcfg, self.micro_batch, vocab_pieces=self.by_vocab_pieces, **kw)
         self.mem_reserved = {"reserved_mb": 0.0}
         if self.device.type == "cuda" and self.impl == "sm100" and os.environ.get("ARB_NO_RESERVE", "0") != "1":
             self.mem_reserved = memplan.reserve(self.mem_plan.step_bytes, self.device)

@@ -111,13 +111,10 @@ class Trainer(TrainerBase):
         self._grads = None
         self.grad_norm = None         # of the last step, where gradients are clipped (a device scalar)
         self._init_common()
-        if hasattr(self.backend, "vocab_pieces"):
-            self.backend.vocab_pieces = tcfg.vocab_pieces
-        pieces = getattr(self.backend, "takes_vocab_pieces", None)
         self.plan_memory(dp=self.world, ep=self.ep, fused_dp=(self.comm.name == "fused"),
                          act_bytes=2 if self.dtype == torch.bfloat16 else 4,
                          ce_chunk=max(mcfg.ce_chunk, getattr(self.backend, "big_ce_chunk", 0)),
-                         documents=tcfg.doc_bos is not None, vocab_pieces=pieces is not None and pieces(mcfg.vocab))
+                         documents=tcfg.doc_bos is not None)
         if tcfg.resume and tcfg.checkpoint_dir:
             self._resume()
 

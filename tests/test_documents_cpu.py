@@ -122,3 +122,57 @@ def test_clip_of_the_oracle():
     assert float(R.clip_grad_norm(g, 100.0)) == 6.5 and float(g[1]) == 6.0
     g[0][0] = float("nan")
     assert math.isnan(float(R.clip_grad_norm(g, 1.0))) and float(g[1]) == 6.0
+
+
+class _HeadByPieces(type(get_backend("oracle"))):
+    """The oracle with the choice that the kernels' backend has."""
+    vocab_pieces = False
+
+    def takes_vocab_pieces(self, vocab):
+        return self.vocab_pieces or vocab > 32768
+
+
+@pytest.fixture
+def one_process(tmp_path):
+    import torch.distributed as dist
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    yield
+    dist.destroy_process_group()
+
+
+def _of_kind(kind, cfg, **kw):
+    from autoresearch_b200.parallel.pipeline import PipelineTrainer
+    from autoresearch_b200.parallel.pipeline_inproc import InProcPipelineTrainer
+    from autoresearch_b200.parallel.tp import TPTrainer
+    t = TrainConfig(device_batch_size=2, total_batch_size=2 * cfg.seq_len, max_steps=2, cooldown_steps=1, synthetic_data=True, impl="oracle",
+                    cooldown_trigger_file="", **kw)
+    if kind == "data":
+        return Trainer(cfg, t, device="cpu", quiet=True)
+    if kind == "tensor":
+        return TPTrainer(cfg, t, tp=1, device="cpu", quiet=True)
+    if kind == "pipeline":
+        return PipelineTrainer(cfg, t, pp=1, device="cpu", quiet=True)
+    return InProcPipelineTrainer(cfg, t, ["cpu", "cpu"], quiet=True)
+
+
+@pytest.mark.parametrize("kind", ["data", "tensor", "pipeline", "in one process"])
+def test_every_trainer_passes_vocab_pieces_on(kind, monkeypatch, one_process):
+    """To the backend and to the memory plan, also where the vocabulary alone decides."""
+    import sys
+    for name in ("autoresearch_b200.trainer", "autoresearch_b200.parallel.tp", "autoresearch_b200.parallel.pipeline",
+                 "autoresearch_b200.parallel.pipeline_inproc"):
+        __import__(name)
+        monkeypatch.setattr(sys.modules[name], "get_backend", lambda impl, cfg: _HeadByPieces().configure(cfg))
+    for vocab, asked, pieces in ((64, True, True), (64, False, False), (32776, False, True)):
+        tr = _of_kind(kind, model_preset("tiny", vocab=vocab), vocab_pieces=asked)
+        assert tr.model.backend.vocab_pieces is asked
+        if kind != "in one process":             # which plans no memory
+            assert ("vocabulary piece, row statistics" in dict(tr.mem_plan.step)) is pieces
+            assert ("logits chunk" in dict(tr.mem_plan.step)) is not pieces
+        tr.prefetch.close()
+
+
+@pytest.mark.parametrize("kind", ["data", "tensor", "pipeline", "in one process"])
+def test_vocab_pieces_are_refused_where_no_kernel_makes_them(kind, one_process):
+    with pytest.raises(ValueError, match="vocab_pieces"):
+        _of_kind(kind, model_preset("tiny"), vocab_pieces=True)
