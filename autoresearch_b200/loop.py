@@ -52,6 +52,7 @@ class TrainerBase:
     impl: str = "oracle"
     clips_gradients: bool = False    # whether this trainer sees all gradients before the optimizer step
     masks_documents: bool = False    # whether its attention can stay inside of documents
+    grad_norm: Optional[torch.Tensor] = None    # of the last step, where gradients are clipped (a device scalar)
 
     # -------------------------------------------------------------------------------------------
     def _init_common(self) -> None:
@@ -274,6 +275,9 @@ class TrainerBase:
                           f"tok/s {int(tok_s)} | mfu {mfu:.1f}% | vram {vram:.0f}MB | steps_left {left}")
                 self._say(f"timing | fwd+bwd {fb_ms:.1f}ms  opt {opt_ms:.1f}ms  gpu {gpu_ms:.1f}ms  "
                           f"wall_gap {max(dt * 1e3 - gpu_ms, 0.0):.1f}ms")
+                norm = None if self.grad_norm is None else float(self.grad_norm)
+                if norm is not None:
+                    self._say(f"clip | grad_norm {norm:.6g}" + ("" if math.isfinite(norm) else " | not finite"))
                 if step > 10:
                     self.total_train_s += step_s
                     self.steady_steps += 1
@@ -281,7 +285,8 @@ class TrainerBase:
                     self.metrics_f.write(json.dumps(dict(
                         step=step, loss=lv, loss_ema=debiased, lr_mult=lrm, dt_device_max_s=step_s,
                         tok_s=tok_s, mfu=mfu, fwd_bwd_ms=fb_ms, opt_ms=opt_ms, vram_mb=vram,
-                        comm_bytes=int(getattr(self, "comm_bytes", 0)))) + "\n")
+                        comm_bytes=int(getattr(self, "comm_bytes", 0)),
+                        **({} if norm is None else dict(grad_norm=norm)))) + "\n")
                     self.metrics_f.flush()
                 if lv > 100 or math.isnan(lv):
                     self._say(f"loss {lv} blew up at step {step}; stopping")

@@ -109,7 +109,6 @@ class Trainer(TrainerBase):
         self.clips_gradients = self.world == 1
         self.masks_documents = True
         self._grads = None
-        self.grad_norm = None         # of the last step, where gradients are clipped (a device scalar)
         self._init_common()
         self.plan_memory(dp=self.world, ep=self.ep, fused_dp=(self.comm.name == "fused"),
                          act_bytes=2 if self.dtype == torch.bfloat16 else 4,

@@ -176,3 +176,35 @@ def test_every_trainer_passes_vocab_pieces_on(kind, monkeypatch, one_process):
 def test_vocab_pieces_are_refused_where_no_kernel_makes_them(kind, one_process):
     with pytest.raises(ValueError, match="vocab_pieces"):
         _of_kind(kind, model_preset("tiny"), vocab_pieces=True)
+
+
+def test_the_norm_is_logged_and_written(tmp_path, capsys):
+    import json
+    for clip, f in ((1e-3, tmp_path / "a"), (0.0, tmp_path / "b")):
+        tr = _trainer(grad_clip=clip, metrics_jsonl=str(f), diagnostic_steps=None)
+        tr.quiet = False
+        norms = []
+        step = tr.train_step
+
+        def spy():
+            loss = step()
+            norms.append(tr.grad_norm)
+            return loss
+        tr.train_step = spy
+        tr.run()
+        said = [ln for ln in capsys.readouterr().out.splitlines() if ln.startswith("clip | grad_norm")]
+        rows = [json.loads(ln) for ln in f.read_text().splitlines()]
+        assert len(rows) == len(norms) >= 4
+        if clip:
+            assert [r["grad_norm"] for r in rows] == [float(n) for n in norms] and min(r["grad_norm"] for r in rows) > 0
+            assert len(said) == len(rows)
+        else:
+            assert not said and all("grad_norm" not in r for r in rows)
+
+
+def test_a_norm_that_is_not_finite_is_said(capsys):
+    tr = _trainer(grad_clip=1.0)
+    tr.quiet = False
+    tr._clip_gradients = lambda top: torch.tensor(math.inf)
+    tr.run()
+    assert "grad_norm inf | not finite" in capsys.readouterr().out
