@@ -5,14 +5,18 @@
 
 The forward product hands out the maximum and the exponential sum of every row and tile of 256 ids, which one small kernel
 joins; no logit is written.  The backward pass multiplies again, a piece of the vocabulary at a time: the epilogue turns a
-piece of logits into d = g[n] (softmax(s) - [v = target]) ds/dx (bf16, at most ``PIECE_BYTES``), which the two gradient
-products dx += d w and dw = d^T x read.  What is kept between the passes is one fp32 number per row.
+piece of logits into d = g[n] (softmax(s) - [v = target]) ds/dx in bf16, which the two gradient products dx += d w and
+dw = d^T x read.  What is kept between the passes is one fp32 number per row.
+
+Scratch: the forward pass takes 8 bytes per row and tile of 256 ids (N V / 32 bytes: 67 MB for 16384 x 131072, a 64th of bf16 logits); the
+backward pass a piece, at most ``PIECE_BYTES`` or, where there are so many rows that a single tile takes more, 512 bytes a row, and
+fp32 sums of dx where the vocabulary has several pieces or the sum has several parts (up to four).
 
 Logits are fp32 sums of the tensor cores, which cut every partial sum (of 16 columns) to 24 bits instead of rounding it: a loss is off
 by about 2e-7 of itself at 256 columns and 1.2e-6 at 2048.
 
 Beside ``LMHeadCEFn`` (ops/sm100.py), which keeps whole rows of logits for a chunk of tokens and makes the gradients in its
-forward pass, this form returns per-token losses with any later weighting and needs no memory that grows with the vocabulary.
+forward pass, this form returns per-token losses with any later weighting, and keeps no logits.
 """
 from __future__ import annotations
 
@@ -24,7 +28,7 @@ import torch
 from . import kernels as K
 
 _ARGS = struct.Struct("=9q9qd")         # ArbLinearCE of csrc/api.h: 9 pointers, 9 sizes, the soft cap
-PIECE_BYTES = 1 << 29                   # bf16 gradient of a piece of logits
+PIECE_BYTES = 1 << 29                   # bf16 gradient of a piece of logits; never less than one tile of every row
 TILE = 256
 MAX_SOFTCAP = 100.0                     # a capped logit is off by up to 2^-22 of the cap
 MIN_SOFTCAP = 2.0 ** -64                # its reciprocal is a normal fp32 number, and the cap is not taken for none
