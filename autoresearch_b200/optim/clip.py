@@ -54,6 +54,10 @@ class GradSet:
     any of the types).  fp32, bf16 or fp16, dense, on one CUDA device, no two sharing memory."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
+        self._take(tensors, out)
+        self._where = self._layout()
+
+    def _take(self, tensors, out) -> None:
         tensors = list(tensors)
         outs = tensors if out is None else list(out)
         if len(outs) != len(tensors):
@@ -78,7 +82,6 @@ class GradSet:
                     ins.discard(t.data_ptr())                       # in place, this one
             _apart([t for t, _ in live if t.data_ptr() in ins] + [o for _, o in live], "outputs and gradients")
         self.tensors, self.out = tensors, out if out is None else outs
-        self._where = self._layout()
         self.device = tensors[0].device if tensors else None
         rows = [_ENTRY.pack(t.data_ptr(), o.data_ptr(), t.numel(), _TYPES[t.dtype], _TYPES[o.dtype]) for t, o in live]
         # (argument block, tensors in it, blocks of its grid)
@@ -95,6 +98,9 @@ class GradSet:
     def _run(self, max_norm: float) -> torch.Tensor:
         if self._layout() != self._where:            # a tensor was given other memory, another size or type since, or the set is a copy
             self.__init__(self.tensors, self.out)
+        return self._launch(max_norm)
+
+    def _launch(self, max_norm: float) -> torch.Tensor:
         if not self._parts:
             return torch.zeros((), dtype=torch.float32, device=self.device if self.device is not None else "cuda")
         with K.on_device(self.device):
@@ -114,9 +120,17 @@ class GradSet:
 Grads = Union[GradSet, Sequence[torch.Tensor]]
 
 
+def _run(grads: Grads, out, max_norm: float) -> torch.Tensor:
+    if isinstance(grads, GradSet):
+        return grads._run(max_norm)
+    once = GradSet.__new__(GradSet)          # for this call alone: nothing to compare it with later
+    once._take(grads, out)
+    return once._launch(max_norm)
+
+
 def grad_norm(grads: Grads) -> torch.Tensor:
     """The 2-norm of all gradients together, a 0-dimensional fp32 tensor on their device."""
-    return (grads if isinstance(grads, GradSet) else GradSet(grads))._run(-1.0)
+    return _run(grads, None, -1.0)
 
 
 def clip_grad_norm(grads: Grads, max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
@@ -125,9 +139,6 @@ def clip_grad_norm(grads: Grads, max_norm: float, out: Optional[Sequence[torch.T
     caller to see in the result; finite gradients are scaled, also those whose norm is infinite as an fp32 number."""
     if not 0.0 < max_norm:
         raise ValueError(f"max_norm must be positive, got {max_norm}")
-    if isinstance(grads, GradSet):
-        if out is not None:
-            raise ValueError("a GradSet holds its outputs already")
-    else:
-        grads = GradSet(grads, out)
-    return grads._run(float(max_norm))
+    if isinstance(grads, GradSet) and out is not None:
+        raise ValueError("a GradSet holds its outputs already")
+    return _run(grads, out, float(max_norm))
