@@ -11,6 +11,7 @@ The norm stays on the device: nothing is read back.  A program whose gradients l
 from __future__ import annotations
 
 import struct
+from operator import attrgetter
 from typing import Optional, Sequence, Union
 
 import torch
@@ -19,6 +20,7 @@ from ..ops import kernels as K
 
 _ENTRY = struct.Struct("=3q2i")         # ArbGrad of csrc/api.h
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_dtype = attrgetter("dtype")
 MAX_TENSORS = 1024                      # per launch
 BLOCKS_PER_SM = 5
 ITEM = 16384                            # elements of a work item
@@ -93,7 +95,9 @@ class GradSet:
                 self._parts.append((b"".join(rows[a:a + MAX_TENSORS]), len(rows[a:a + MAX_TENSORS]), min(items, most)))
 
     def _layout(self):
-        return [(t.data_ptr(), t.numel(), t.dtype) for t in (self.tensors if self.out is None else self.tensors + self.out)]
+        """Where the tensors lie, of which size and type: a fifth of a microsecond a tensor, in every call."""
+        every = self.tensors if self.out is None else self.tensors + self.out
+        return [*map(torch.Tensor.data_ptr, every), *map(torch.Tensor.numel, every), *map(_dtype, every)]
 
     def _run(self, max_norm: float) -> torch.Tensor:
         if self._layout() != self._where:            # a tensor was given other memory, another size or type since, or the set is a copy
