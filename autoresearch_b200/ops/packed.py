@@ -45,14 +45,17 @@ def check_bounds(bounds, rows: int) -> None:
         raise ValueError(f"sequence bounds must ascend within [0, {rows}]: got {list(bounds[:16])}")
 
 
-def _to_device(bounds: torch.Tensor, device: torch.device) -> torch.Tensor:
-    """A copy of host bounds on ``device``, made in the order of its current stream and without waiting for what runs there: they travel
-    through pinned memory of their own, which the allocator gives away again behind the copy only."""
+def _to_device(bounds, device: torch.device) -> torch.Tensor:
+    """A copy of host bounds (a list or a tensor) on ``device``, made in the order of its current stream and without waiting for what runs
+    there: they travel through pinned memory of their own, which the allocator gives away again behind the copy only."""
     with torch.cuda.device(device):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("under graph capture cu_seqlens must be a CUDA tensor: every replay would read the host's memory again")
-        pinned = torch.empty(bounds.shape, dtype=torch.int32, pin_memory=True)
-        pinned.copy_(bounds)
+        if torch.is_tensor(bounds):
+            pinned = torch.empty(bounds.shape, dtype=torch.int32, pin_memory=True)
+            pinned.copy_(bounds)
+        else:
+            pinned = torch.tensor(bounds, dtype=torch.int32, pin_memory=True)
         return pinned.to(device, non_blocking=True)
 
 
@@ -88,13 +91,15 @@ class PackedSequences:
                 raise TypeError("cu_seqlens must be a 1-D tensor of integers")
             if not torch.is_tensor(cu_seqlens):
                 cu_seqlens = [operator.index(b) for b in cu_seqlens]
+            elif cu_seqlens.numel() <= 256:                    # a short list is looked through faster than three tensor operations start
+                cu_seqlens = cu_seqlens.tolist()
             if not len(cu_seqlens):
                 raise ValueError("cu_seqlens needs at least one bound")
             check_bounds(cu_seqlens, rows)
             device = torch.device(device if device is not None else "cuda")
             if device.type != "cuda":
                 raise ValueError(f"the sequences must be packed on a CUDA device, not {device}")
-            cu_seqlens = _to_device(torch.as_tensor(cu_seqlens), device)
+            cu_seqlens = _to_device(cu_seqlens, device)
         elif cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype is not torch.int32:
             raise TypeError("cu_seqlens must be a 1-D int32 tensor of at least one element")
         self.cu_seqlens = cu_seqlens.contiguous()
