@@ -52,10 +52,10 @@ def _to_device(bounds, device: torch.device) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("under graph capture cu_seqlens must be a CUDA tensor: every replay would read the host's memory again")
         if torch.is_tensor(bounds):
-            pinned = torch.empty(bounds.shape, dtype=torch.int32, pin_memory=True)
+            pinned = torch.empty(bounds.shape, dtype=torch.int32, device="cpu", pin_memory=True)
             pinned.copy_(bounds)
         else:
-            pinned = torch.tensor(bounds, dtype=torch.int32, pin_memory=True)
+            pinned = torch.tensor(bounds, dtype=torch.int32, device="cpu", pin_memory=True)
         return pinned.to(device, non_blocking=True)
 
 
@@ -73,7 +73,8 @@ class PackedSequences:
     """Which tiles the sequences of a packed batch have.
 
     ``cu_seqlens``: n + 1 ascending row numbers, an int32 CUDA tensor, or host values (a list, a CPU tensor), which are checked
-    and copied here, without waiting for the device.  Bounds that only the device knows are not read back: where they descend or leave the rows they are moved inside,
+    and copied here, without waiting for the device (under graph capture: a CUDA tensor only).  Bounds that only the device
+    knows are not read back: where they descend or leave the rows they are moved inside,
     and ``kernels.check_err_flag()`` reports it.  Empty sequences are allowed.  Rows of no sequence (before the first bound
     and behind the last) get zero outputs and gradients, whatever their inputs hold.
 

@@ -547,3 +547,13 @@ def test_host_bounds_are_refused_under_graph_capture():
             PackedSequences([0, 4], 4, 2, 1)
     graph.replay()
     assert float(x[0]) == 1.0
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_host_bounds_where_another_device_is_the_default(many):
+    from autoresearch_b200.ops.packed import PackedSequences
+    bounds = list(range(301)) if many else [0, 300]
+    with torch.device("cuda"):
+        got = [PackedSequences(b, 300, 2, 1) for b in (bounds, torch.tensor(bounds, device="cpu"))]
+    for s in got:
+        assert s.cu_seqlens.is_cuda and s.cu_seqlens.tolist() == bounds
