@@ -491,7 +491,7 @@ __device__ __forceinline__ void qkv_post_head(float (&f)[128], const QkvPostArgs
 // s = cap tanh(x / cap) = cap (1 - 2 r), r = 1 / (1 + e), e = exp(2 x / cap); ds/dx = 4 e r^2.  tanhf under fast math is one instruction with an error of 2^-11, 0.007 in a
 // logit at cap 15, which would go into the loss.  Scores, and what is kept of a row between the passes, are in units of log 2: a
 // probability is then one subtraction and one exponential away, without a rounding in between.
-constexpr float CE_LOG2E = 1.4426950408889634f, CE_LN2 = 0.6931471805599453f;
+constexpr float CE_LOG2E = 1.4426950408889634f;
 // capped scores lie in [-cap, cap]: up to this cap 2^(s - cap) neither overflows nor vanishes in fp32 and no maximum is needed
 constexpr float CE_FIXED_MAX = 40.f;
 // s = cap (1 - 2 r) loses what r = 1/2 + ... rounds: 2^-22 of the cap
@@ -1461,10 +1461,15 @@ __global__ void __launch_bounds__(256) ce_join_k(const float2* part, const float
   __syncthreads();
   if (w == 0 && row < rows) {
     for (int k = 1; k < 8; ++k) add(sh[k][lane]);
-    const float l = m + log2f(s);
-    lse[row] = l;
+    // log2 s as exponent and logarithm of a mantissa in [1/2, 1): fast math's logarithm is off by 2^-22 there, and by 2^-22 of its result
+    // elsewhere, where a fixed maximum leaves sums around 2^-58 and m + log2 s cancels.  Once a row, so in 64 bits.
+    const uint32_t bits = __float_as_uint(s);
+    const bool normal = s >= 1.17549435e-38f && s < INFINITY;
+    const double l = normal ? double(m) + double(int(bits >> 23) - 126) + double(log2f(__uint_as_float((bits & 0x007fffffu) | 0x3f000000u)))
+                            : double(m + log2f(s));
+    lse[row] = float(l);
     const long long target = ce_target(c, int(row));
-    loss[row] = target >= 0 && target < c.vocab ? (l - target_score[row]) * CE_LN2 : 0.f;
+    loss[row] = target >= 0 && target < c.vocab ? float((l - double(target_score[row])) * 0.69314718055994531) : 0.f;
   }
 }
 

@@ -313,3 +313,10 @@ def test_values_that_are_not_finite_show_in_their_row_and_in_no_other(cap):
     assert not bool(torch.isfinite(got[131])) or cap > 0          # a capped logit of an infinity is the cap
     rest = [i for i in range(300) if i not in (7, 131)]
     assert torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.parametrize("cap", [15.0, 30.0, 40.0, 41.0])
+@pytest.mark.parametrize("N,D", [(1993, 64), (256, 352)])
+def test_one_id_under_caps_with_and_without_a_fixed_maximum(N, D, cap):
+    """The softmax is one; what a gradient has left is the error of the log sum."""
+    _check(N, D, 1, cap)
